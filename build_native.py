@@ -24,6 +24,10 @@ OUT_DIR = os.path.join(ROOT, "trustworthy_dl", "_native")
 BUILD_DIR = os.path.join(ROOT, "build", "native")
 NO_NAN_FLAGS = {"attention.hip": ["-fno-honor-nans"]}
 AGPR_FORM = {"gemm.hip"}
+# no v_pk_add / mul / fma_f32: hipcc -O3 forms them from ordinary float code, and some of their forms
+# have been seen to return wrong values on this hardware now and then (the host pass warns that it
+# does not know the feature: harmless)
+NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def hipcc() -> str:
@@ -71,7 +75,7 @@ def build(arch: str = "gfx950", jobs: int = 8, debug: bool = False, verbose: boo
             # of an MFMA result needs no canonicalising v_max in front of it (csrc/attention.hip)
             form += NO_NAN_FLAGS.get(os.path.basename(src), [])
             jobs_list.append([cc, f"--offload-arch={arch}", "-std=c++17", "-fPIC", *opt, "-munsafe-fp-atomics",
-                              *form, "-I", CSRC, "-c", src, "-o", obj])
+                              *NO_PACKED_F32, *form, "-I", CSRC, "-c", src, "-o", obj])
     for src in rt_srcs:
         obj = os.path.join(BUILD_DIR, "rt_" + os.path.basename(src) + ".o")
         robjs.append(obj)
