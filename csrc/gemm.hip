@@ -164,14 +164,17 @@ struct Stager {
         }
         return __builtin_amdgcn_make_buffer_rsrc((void*)b, 0, nrec, 0x00020000);
     }
-    // piece i of this wave
-    __device__ __forceinline__ void piece(__amdgpu_buffer_rsrc_t r, char* lds_tile, int w, int i) const {
+    // byte offset of the lane's 16 bytes of piece i
+    __device__ __forceinline__ uint32_t offset(int i) const {
         // opaque copy of the base: keeps the compiler from hoisting all NP offsets out of the K loop
         // (it did, and spilled them: a scratch reload + vmcnt(0) in front of every copy)
         uint32_t b = base[TR ? (i & 1) : 0];
         asm volatile("" : "+v"(b));
-        const uint32_t off = b + (uint32_t)i * delta;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void_t*)(lds_tile + (w + NW * i) * 1024), 16, off, 0, 0, 0);
+        return b + (uint32_t)i * delta;
+    }
+    // piece i of this wave
+    __device__ __forceinline__ void piece(__amdgpu_buffer_rsrc_t r, char* lds_tile, int w, int i) const {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void_t*)(lds_tile + (w + NW * i) * 1024), 16, offset(i), 0, 0, 0);
     }
     __device__ __forceinline__ void issue(const bf16_t* G, int ld, int r0, int rmax, int k0, char* lds_tile, int w) const {
         const __amdgpu_buffer_rsrc_t r = rsrc(G, ld, r0, rmax, k0);
@@ -1112,35 +1115,36 @@ __global__ __launch_bounds__(PNTHR, 1) void gemm_p4(GemmParams p) {
 
 // ============================================================================ persistent 4-wave, LDS-DMA
 // gemm_p4's geometry (one wave per SIMD owning 128 x 128, AGPR accumulators, persistent grid) with
-// the operands copied by LDS-DMA (buffer_load ... lds, no VGPR staging) into two 64-KiB stages, on
-// the schedule of the library kernel our step profiles name for these products (its disassembly: a
-// K step = 128 MFMAs, 16 one-KiB copies spread one per ~5 MFMAs, three barriers, ONE vmcnt wait):
-//   half 0 (64 MFMAs on F0 = k-half 0 of step s, read at the end of step s - 1):
-//     T 0..15 : read F1 = k-half 1 of step s from stage cur, one fragment per MFMA
-//     T 18    : own LDS reads retired + barrier: no wave reads stage cur any more
-//     T 20..62: copies 0-6 of step s + 2 into stage cur, one every 7 MFMAs (spread: a copy's issue
-//               costs ~60 cycles, MI355X_MICROARCH.md; denser placements measured slower)
-//   half 1 (64 MFMAs on F1):
-//     T 5..33 : copies 7-11
-//     T 36    : vmcnt(12) — every copy of step s + 1 (issued during step s - 1) landed, the 12
-//               issued since stay in flight — + barrier: all waves' copies of step s + 1 visible
-//     T 37..52: read F0 = k-half 0 of step s + 1 from stage nxt; copies 12-15 at T 40..61
-// (variants of these slots: TDL_PD_SCHED, profiles/r5_gemm_pd_sched_ab.jsonl)
-// So a copy has about a K step to land and the wave waits for copies once per step (gemm_p4 waits
-// for each staged register ahead of its LDS write, inside the MFMA stream: 46 % of its wave cycles).
-// NT operands only (TA = TB = false: the forward / input-gradient products).
-// ORD 0: MFMA T = (A tile T / 8, B tile T % 8) — the MFMA's second source (an A fragment) held for
-// 8 MFMAs; ORD 1: (A tile T % 8, B tile T / 8) — its first source (a B fragment) held, as in the
-// library kernel.  Either way accumulator 8 i + j is tile (i, j).
-template <int T, bool ZERO, int ORD, class Hook>
+// the operands copied by LDS-DMA (buffer_load ... lds, no VGPR staging) into two 64-KiB stages.  A
+// K step is 128 MFMA slots per wave; what stands in them follows from four counts:
+//   * a fragment read moves 1 KiB per wave; the four waves share 128 B per clock of LDS, so a read
+//     takes 32 clocks of its share = two 16-clock MFMA slots (PD_READ), and the 16 reads of a k-half
+//     32 slots;
+//   * F1 (k-half 1 of step s) is read from stage cur in the first 32 slots; two slots later the
+//     last one has returned: barrier at PD_FREE, after which no wave reads stage cur any more;
+//   * the 16 copies of step s + 2 into stage cur are spread evenly over all slots that remain
+//     (PD_PITCH): the memory system sees one constant stream instead of a burst per step;
+//   * F0 (k-half 0 of step s + 1) has to be in registers when the step ends: its 32 slots of reads
+//     are the last ones, and the wait for step s + 1's copies + barrier stands right before them
+//     (PD_LAND).  The copies issued since the previous step's PD_LAND stay in flight: vmcnt counts
+//     down to the ones of this step that precede the wait.
+// So a copy has more than a K step to land, and a wave waits for copies once per step.  k-contiguous
+// operands take any epilogue; row-contiguous ones (the weight gradients) fp32 outputs.
+constexpr int PD_SLOTS = 128, PD_READ = 2, PD_FRAGS = 16, PD_COPIES = 16;
+constexpr int PD_FREE = PD_READ * PD_FRAGS + 2;
+constexpr int PD_COPY0 = PD_FREE + 2;
+constexpr int PD_PITCH = (PD_SLOTS - PD_COPY0) / PD_COPIES;
+constexpr int PD_LAND = PD_SLOTS - PD_READ * PD_FRAGS - 1;
+// MFMA T of a k-half: A tile T / 8, B tile T % 8 (accumulator 8 i + j is tile (i, j))
+template <int T, bool ZERO, class Hook>
 __device__ __forceinline__ void mfma_run_pd(Acc& acc, const bf16x8_t (&a)[8], const bf16x8_t (&b)[8], Hook& hook) {
     if constexpr (T < 64) {
-        constexpr int i = ORD == 0 ? T / 8 : T % 8, j = ORD == 0 ? T % 8 : T / 8;
+        constexpr int i = T / 8, j = T % 8;
         if constexpr (ZERO) amfma0<8 * i + j>(acc, b[j], a[i]);
         else amfma<8 * i + j>(acc, b[j], a[i]);
         hook(std::integral_constant<int, T>{});
         __builtin_amdgcn_sched_barrier(0);
-        mfma_run_pd<T + 1, ZERO, ORD>(acc, a, b, hook);
+        mfma_run_pd<T + 1, ZERO>(acc, a, b, hook);
     }
 }
 
@@ -1292,27 +1296,21 @@ __device__ __forceinline__ void pd_store_x4_dgelu(const GemmParams& p, Get& get,
 
 // s_waitcnt vmcnt(n) with expcnt / lgkmcnt at their no-wait maxima (gfx9 encoding)
 constexpr int vmcnt_enc(int n) { return (n & 15) | ((n >> 4) << 14) | (7 << 4) | (15 << 8); }
-// copies of a step issued before global MFMA slot wg (slots ds + dp i, i < 16)
-constexpr int copies_before(int ds, int dp, int wg) {
+// copies of a step issued before slot PD_LAND
+constexpr int pd_copies_before_land() {
     int n = 0;
-    for (int i = 0; i < 16; ++i) n += (ds + dp * i < wg) ? 1 : 0;
+    for (int i = 0; i < PD_COPIES; ++i) n += (PD_COPY0 + PD_PITCH * i < PD_LAND) ? 1 : 0;
     return n;
 }
 
-// Schedule (global MFMA slot g = 64 half + T of a K step): RP = MFMAs per F1 fragment read at the
-// head of half 0, then lgkmcnt(0) + barrier; copy i at slot DS + DP i; the vmcnt wait + barrier at
-// slot WG; F0 reads after it.
-template <int EPI, int RP = 1, int DS = 20, int DP = 7, int WG = 100, bool X4 = false, int ORD = 0, int B1 = 16 * RP + 2,
-          bool TA = false, bool TB = false, bool NOEPI = false, bool NOBIAS = false, bool GROUPED = false>
+template <int EPI, bool X4 = false, bool TA = false, bool TB = false, bool NOBIAS = false, bool GROUPED = false>
 __global__ __launch_bounds__(PNTHR, 1) void gemm_pd(GemmParams p) {
-    static_assert(B1 >= 16 * RP + 2 && DS > B1 && DS + 15 * DP <= 127 && WG + 16 <= 127, "schedule must fit one K step");
-    constexpr int NB = copies_before(DS, DP, WG);          // this step's copies in flight at the wait
-    constexpr int RP2 = 127 - WG >= 32 ? 2 : 1;          // MFMAs per F0 fragment read
+    constexpr int NB = pd_copies_before_land();          // this step's copies in flight at the wait
     static_assert(!X4 || EPI == EPI_BF16 || EPI == EPI_GELU || EPI == EPI_DGELU, "16-byte epilogues: bf16, GELU, dGELU");
     // the first wait after an epilogue: the copies it waits for precede the epilogue's VMEM ops
     // (>= 64 per wave for the per-tile-row epilogue, exactly PD_X4_VMEM for pd_store_x4) and the NB
     // copies issued since; vmcnt counts in issue order, so vmcnt(that sum) retires exactly the copies
-    constexpr int EV = NOEPI ? 0 : X4 ? pd_x4_vmem(EPI) : 64;
+    constexpr int EV = X4 ? pd_x4_vmem(EPI) : 64;
     constexpr int NB_EPI = EV + NB < 63 ? EV + NB : 63;
     __shared__ __attribute__((aligned(16))) char smem[LDS_BYTES];
     const int tid = threadIdx.x, lane = tid & 63;
@@ -1388,28 +1386,23 @@ __global__ __launch_bounds__(PNTHR, 1) void gemm_pd(GemmParams p) {
             pleft = 0;
         }
     };
-    // copy i (< 8: A piece i, else B piece i - 8): the lane's base offset in the VGPR operand, the
-    // piece's uniform offset in the SGPR one (no per-copy address arithmetic in the K loop)
+    // copy i: A piece i (i < 8), else B piece i - 8
     auto copy_piece = [&](char* stage, auto ic) {
         constexpr int i = decltype(ic)::value;
         constexpr int j = i & 7;
-        constexpr bool TR = i < 8 ? TA : TB;
-        const uint32_t vo = i < 8 ? sa.base[TR ? (j & 1) : 0] : sb.base[TR ? (j & 1) : 0];
-        const uint32_t dl = i < 8 ? sa.delta : sb.delta;
         char* dst = stage + (i < 8 ? 0 : TILE_BYTES) + (w + 4 * j) * 1024;
-        if constexpr (TR) {
+        const uint32_t off = i < 8 ? sa.offset(j) : sb.offset(j);
+        if constexpr (i < 8 ? TA : TB) {
             // Row-contiguous images are read with ds_read_b64_tr_b16, whose builtin hipcc cannot tell
             // apart from the DMA's destination: it drained every copy in flight (s_waitcnt vmcnt(0))
             // in front of the transposed reads, 10 times per K step — 62 % of the wave cycles parked,
             // 0.62x gemm_p4 (profiles/r6_pmc_wgrad_pd.txt).  Issued from asm, the copy is invisible
             // to that alias check; its completion is still counted by the explicit vmcnt waits.
             const uint32_t la = __builtin_amdgcn_readfirstlane((uint32_t)(size_t)(lds_void_t*)dst);
-            const uint32_t so = __builtin_amdgcn_readfirstlane((uint32_t)j * dl);
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-                         :: "s"(la), "v"(vo), "s"(i < 8 ? qa : qb), "s"(so) : "memory", "m0");
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                         :: "s"(la), "v"(off), "s"(i < 8 ? qa : qb) : "memory", "m0");
         } else {
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(i < 8 ? qa : qb, (lds_void_t*)dst, 16, vo,
-                                                     __builtin_amdgcn_readfirstlane((uint32_t)j * dl), 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(i < 8 ? qa : qb, (lds_void_t*)dst, 16, off, 0, 0, 0);
         }
     };
     auto frag_base = [&](bool isB, int buf, int ks) -> uint32_t {
@@ -1464,37 +1457,37 @@ __global__ __launch_bounds__(PNTHR, 1) void gemm_pd(GemmParams p) {
         produce_rsrc();
         auto slot = [&](auto gc, const uint32_t* fb) {
             constexpr int g = decltype(gc)::value;
-            if constexpr (g < 16 * RP && g % RP == RP - 1) {   // F1 = k-half 1 of step s (stage cur)
-                constexpr int k = g / RP;
-                if constexpr ((k < 8) == (ORD == 0)) b1[k & 7] = frag_x(true, fb[0], cur, k & 7, 1);
-                else a1[k & 7] = frag_x(false, fb[1], cur, k & 7, 1);
+            if constexpr (g < PD_READ * PD_FRAGS && g % PD_READ == PD_READ - 1) {   // F1 = k-half 1 of step s (stage cur)
+                constexpr int k = g / PD_READ;
+                if constexpr (k < 8) b1[k] = frag_x(true, fb[0], cur, k, 1);
+                else a1[k - 8] = frag_x(false, fb[1], cur, k - 8, 1);
             }
-            if constexpr (g == B1) {   // own reads of stage cur retired; then all waves'
+            if constexpr (g == PD_FREE) {   // own reads of stage cur retired; then all waves'
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 __builtin_amdgcn_s_barrier();
             }
-            if constexpr (g >= DS && (g - DS) % DP == 0 && (g - DS) / DP < 16)
-                copy_piece(cstage, std::integral_constant<int, (g - DS) / DP>{});
-            if constexpr (g == WG) {   // copies of step s + 1 landed (this step's NB stay in flight)
+            if constexpr (g >= PD_COPY0 && (g - PD_COPY0) % PD_PITCH == 0 && (g - PD_COPY0) / PD_PITCH < PD_COPIES)
+                copy_piece(cstage, std::integral_constant<int, (g - PD_COPY0) / PD_PITCH>{});
+            if constexpr (g == PD_LAND) {   // copies of step s + 1 landed (this step's NB stay in flight)
                 if (ZERO && after_epi) __builtin_amdgcn_s_waitcnt(vmcnt_enc(NB_EPI));
                 else __builtin_amdgcn_s_waitcnt(vmcnt_enc(NB));
                 __builtin_amdgcn_s_barrier();
             }
-            if constexpr (!LAST && g > WG && (g - WG - 1) % RP2 == 0 && (g - WG - 1) / RP2 < 16) {
-                constexpr int k = (g - WG - 1) / RP2;   // F0 = k-half 0 of step s + 1 (stage nxt)
-                if constexpr ((k < 8) == (ORD == 0)) b0[k & 7] = frag_x(true, fb[2], nxt, k & 7, 0);
-                else a0[k & 7] = frag_x(false, fb[3], nxt, k & 7, 0);
+            if constexpr (!LAST && g > PD_LAND && (g - PD_LAND - 1) % PD_READ == 0 && (g - PD_LAND - 1) / PD_READ < PD_FRAGS) {
+                constexpr int k = (g - PD_LAND - 1) / PD_READ;   // F0 = k-half 0 of step s + 1 (stage nxt)
+                if constexpr (k < 8) b0[k] = frag_x(true, fb[2], nxt, k, 0);
+                else a0[k - 8] = frag_x(false, fb[3], nxt, k - 8, 0);
             }
         };
         const uint32_t fb[4] = {frag_base(true, cur, 1), frag_base(false, cur, 1), frag_base(true, nxt, 0),
                                 frag_base(false, nxt, 0)};
         {
             auto hook = [&](auto tc) { slot(tc, fb); };
-            mfma_run_pd<0, ZERO, ORD>(acc, a0, b0, hook);
+            mfma_run_pd<0, ZERO>(acc, a0, b0, hook);
         }
         {
             auto hook = [&](auto tc) { slot(std::integral_constant<int, 64 + decltype(tc)::value>{}, fb); };
-            mfma_run_pd<0, false, ORD>(acc, a1, b1, hook);
+            mfma_run_pd<0, false>(acc, a1, b1, hook);
         }
         produce_advance();
         ++s;
@@ -1515,8 +1508,7 @@ __global__ __launch_bounds__(PNTHR, 1) void gemm_pd(GemmParams p) {
         acc_fence<48>(acc);
         __builtin_amdgcn_sched_barrier(0);
         auto get = [&](auto ic, auto jc) { return acc[8 * decltype(ic)::value + decltype(jc)::value]; };
-        if constexpr (NOEPI) {   // diagnostics only (TDL_PD_SCHED=10): the K loop without the epilogue
-        } else if constexpr (X4 && EPI == EPI_DGELU) pd_store_x4_dgelu(p, get, cm0 + wm * 128, cn0 + wn * 128, lane);
+        if constexpr (X4 && EPI == EPI_DGELU) pd_store_x4_dgelu(p, get, cm0 + wm * 128, cn0 + wn * 128, lane);
         else if constexpr (X4) pd_store_x4<EPI, !NOBIAS>(p, get, cm0 + wm * 128, cn0 + wn * 128, lane, braw);
         else epilogue_store<EPI, 8>(p, get, cm0 + wm * 128, cn0 + wn * 128, csp, lane);
         __builtin_amdgcn_sched_barrier(0);
@@ -1589,11 +1581,11 @@ TDL_API int tdl_gemm(const void* A, const void* B, void* C, const void* bias, vo
 #define P4_LEPI false
 #endif
 #ifdef PD_ISA   // the 16-byte-store gemm_pd epilogues instead (register / spill inspection)
-    gemm_pd<EPI_BF16, 1, 20, 7, 100, true><<<256, PNTHR, 0, s>>>(p);
-    gemm_pd<EPI_BF16, 1, 20, 7, 100, true, 0, 18, false, false, false, true><<<256, PNTHR, 0, s>>>(p);
-    gemm_pd<EPI_GELU, 1, 20, 7, 100, true><<<256, PNTHR, 0, s>>>(p);
-    gemm_pd<EPI_DGELU, 1, 20, 7, 100, true><<<256, PNTHR, 0, s>>>(p);
-    gemm_pd<EPI_F32, 1, 20, 7, 100, false, 0, 18, true, true><<<256, PNTHR, 0, s>>>(p);
+    gemm_pd<EPI_BF16, true><<<256, PNTHR, 0, s>>>(p);
+    gemm_pd<EPI_BF16, true, false, false, true><<<256, PNTHR, 0, s>>>(p);
+    gemm_pd<EPI_GELU, true><<<256, PNTHR, 0, s>>>(p);
+    gemm_pd<EPI_DGELU, true><<<256, PNTHR, 0, s>>>(p);
+    gemm_pd<EPI_F32, false, true, true><<<256, PNTHR, 0, s>>>(p);
 #else
     gemm_p4<P4_TA, P4_TB, P4_EPI, P4_LEPI><<<256, PNTHR, 0, s>>>(p);
 #endif
@@ -1605,27 +1597,9 @@ TDL_API int tdl_gemm(const void* A, const void* B, void* C, const void* bias, vo
         const int grid = items < num_cus() ? items : num_cus();
         if (ta) {
             switch (epi) {
-                case EPI_F32: gemm_pd<EPI_F32, 1, 20, 7, 100, false, 0, 18, true, true><<<grid, PNTHR, 0, s>>>(p); break;
-                case EPI_F32ACC: gemm_pd<EPI_F32ACC, 1, 20, 7, 100, false, 0, 18, true, true><<<grid, PNTHR, 0, s>>>(p); break;
-                default: gemm_pd<EPI_F32ATOM, 1, 20, 7, 100, false, 0, 18, true, true><<<grid, PNTHR, 0, s>>>(p); break;
-            }
-            TDL_LAUNCH_CHECK();
-        }
-        // schedule variants (plain bf16 epilogue only): TDL_PD_SCHED, read per launch (in-process A/B)
-        const char* sv = std::getenv("TDL_PD_SCHED");
-        const int v = (sv && epi == EPI_BF16) ? std::atoi(sv) : 0;
-        if (v > 0) {
-            switch (v) {
-                case 1: gemm_pd<0, 2, 36, 6, 110><<<grid, PNTHR, 0, s>>>(p); break;
-                case 2: gemm_pd<0, 2, 40, 5, 96><<<grid, PNTHR, 0, s>>>(p); break;
-                case 3: gemm_pd<0, 2, 36, 6, 100><<<grid, PNTHR, 0, s>>>(p); break;
-                case 4: gemm_pd<0, 1, 19, 7, 104><<<grid, PNTHR, 0, s>>>(p); break;
-                case 6: gemm_pd<0, 1, 20, 7, 100, true, 1><<<grid, PNTHR, 0, s>>>(p); break;
-                case 7: gemm_pd<0, 1, 26, 6, 100, true, 0, 24><<<grid, PNTHR, 0, s>>>(p); break;
-                case 8: gemm_pd<0, 1, 24, 6, 100, true, 0, 22><<<grid, PNTHR, 0, s>>>(p); break;
-                case 9: gemm_pd<0, 1, 30, 6, 104, true, 0, 28><<<grid, PNTHR, 0, s>>>(p); break;
-                case 10: gemm_pd<0, 1, 20, 7, 100, true, 0, 18, false, false, true><<<grid, PNTHR, 0, s>>>(p); break;
-                default: gemm_pd<0, 1, 20, 7, 108><<<grid, PNTHR, 0, s>>>(p); break;
+                case EPI_F32: gemm_pd<EPI_F32, false, true, true><<<grid, PNTHR, 0, s>>>(p); break;
+                case EPI_F32ACC: gemm_pd<EPI_F32ACC, false, true, true><<<grid, PNTHR, 0, s>>>(p); break;
+                default: gemm_pd<EPI_F32ATOM, false, true, true><<<grid, PNTHR, 0, s>>>(p); break;
             }
             TDL_LAUNCH_CHECK();
         }
@@ -1635,10 +1609,10 @@ TDL_API int tdl_gemm(const void* A, const void* B, void* C, const void* bias, vo
             // (a bias / no-bias branch inside one kernel pushed it past 256 VGPRs: 13 spills whose
             // reloads drained every copy in flight, so the two are separate instantiations)
             if (epi == EPI_BF16 && bias == nullptr)
-                gemm_pd<EPI_BF16, 1, 20, 7, 100, true, 0, 18, false, false, false, true><<<grid, PNTHR, 0, s>>>(p);
-            else if (epi == EPI_BF16) gemm_pd<EPI_BF16, 1, 20, 7, 100, true><<<grid, PNTHR, 0, s>>>(p);
-            else if (epi == EPI_GELU) gemm_pd<EPI_GELU, 1, 20, 7, 100, true><<<grid, PNTHR, 0, s>>>(p);
-            else gemm_pd<EPI_DGELU, 1, 20, 7, 100, true><<<grid, PNTHR, 0, s>>>(p);
+                gemm_pd<EPI_BF16, true, false, false, true><<<grid, PNTHR, 0, s>>>(p);
+            else if (epi == EPI_BF16) gemm_pd<EPI_BF16, true><<<grid, PNTHR, 0, s>>>(p);
+            else if (epi == EPI_GELU) gemm_pd<EPI_GELU, true><<<grid, PNTHR, 0, s>>>(p);
+            else gemm_pd<EPI_DGELU, true><<<grid, PNTHR, 0, s>>>(p);
             TDL_LAUNCH_CHECK();
         }
         switch (epi) {
@@ -1746,6 +1720,6 @@ TDL_API int tdl_gemm_wgrad_grouped(const void* A1, const void* B1, float* C1, in
     const int items = p.items1 + p.g2.tiles * split;
     if (items > num_cus()) return (int)hipErrorInvalidValue;   // one item per workgroup (the caller splits less)
     const int grid = items;
-    gemm_pd<EPI_F32, 1, 20, 7, 100, false, 0, 18, true, true, false, false, true><<<grid, PNTHR, 0, s>>>(p);
+    gemm_pd<EPI_F32, false, true, true, false, true><<<grid, PNTHR, 0, s>>>(p);
     TDL_LAUNCH_CHECK();
 }

@@ -28,7 +28,7 @@ BK = 64
 # Kernel (csrc/gemm.hip): "p4" = the persistent 4-wave kernel (one wave per SIMD owning 128 x 128,
 # register-staged operands), "pp" = the staggered 8-wave ping-pong kernel (LDS-DMA staging,
 # LDS-staged row-contiguous epilogue on NT operands), "pd" = the persistent 4-wave kernel with
-# LDS-DMA staging on the library kernel's schedule (NT operands only).
+# LDS-DMA staging (NT operands, or TT with fp32 outputs).
 KERNELS = {"p4": 0, "pp": 1, "p4l": 2, "pd": 3}
 KERNEL = os.environ.get("TDL_GEMM_KERNEL", "pp")        # bf16-output products (matmul)
 # the bias + GELU product (the MLP fc forward) on the LDS-DMA kernel's 16-byte-store epilogue: +0.4 %
