@@ -22,7 +22,7 @@ ROOT = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(ROOT, "csrc")
 OUT_DIR = os.path.join(ROOT, "trustworthy_dl", "_native")
 BUILD_DIR = os.path.join(ROOT, "build", "native")
-NO_NAN_FLAGS = {"attention.hip": ["-fno-honor-nans"]}
+NO_NAN_FLAGS = {n: ["-fno-honor-nans"] for n in ("attention.hip", "masked_attention_fwd.hip", "masked_attention_bwd.hip")}
 AGPR_FORM = {"gemm.hip"}
 # no v_pk_add / mul / fma_f32: hipcc -O3 forms them from ordinary float code, and some of their forms
 # have been seen to return wrong values on this hardware now and then (the host pass warns that it

@@ -1,0 +1,282 @@
+// Shared parts of the masked attention kernels (masked_attention_fwd.hip, masked_attention_bwd.hip).
+//
+//   x_ij = scale q_i . k_j        y_ij = cap tanh(x_ij / cap)        s_ij = y_ij - slope_h |p_i - j|
+//   o_i = sum_j softmax_j(s_ij) v_j over the visible keys  lo_i <= j < hi_i
+//
+// Every mask the op offers (causal, documents packed into a row, a prefix that is seen both ways,
+// padded rows, a cache's valid length) leaves each query ONE interval of visible keys, so the kernels
+// know masks only as two integers per query: a tile needs no per-key mask data, whole tiles are
+// skipped or taken without a test from the intervals' bounds over 32 queries (qtab), and the dK / dV
+// kernel finds the queries that see a block of keys in ktab.
+#pragma once
+#include "common.h"
+
+#include <type_traits>
+
+namespace mattn {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef short short8v __attribute__((ext_vector_type(8)));
+typedef unsigned short ushort2v __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));   // (a class like uint4 selected by ?: would be selected by address: scratch)
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr int QT = 32;    // queries per qtab entry
+constexpr int KT = 128;   // keys per ktab entry
+
+// one argument block for every entry point (ops/masked_attention.py fills the same layout)
+struct Args {
+    const void *q, *k, *v, *dout;
+    void *o, *dq, *dk, *dv;
+    float *lse, *delta, *ws;
+    const float* slopes;
+    const int *lo, *hi, *pos;
+    const int4* qtab;    // [B][ceil(Tq / 32)]: lowest lo, highest hi (rows that see something), highest lo, lowest hi (all rows)
+    const int2* ktab;    // [B][ceil(Tk / 128)]: first and past-the-last qtab entry that sees a key of the block
+    int64_t qs[3], ks[3], vs[3], os[3], dos[3], dqs[3], dks[3], dvs[3];   // strides in elements: batch, token, head
+    int B, Tq, Tk, H, Hk, D, dtype, nsplit;
+    float scale, cap;
+};
+
+struct Bf16 {
+    typedef bf16x8 vec;
+    static constexpr uint32_t INF = 0x7f80, NANBITS = 0x7fc0;
+    static __device__ __forceinline__ f32x16 mfma(vec a, vec b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack2(a, b); }
+    static __device__ __forceinline__ void unpack(uint32_t w, float& a, float& b) {
+        a = __uint_as_float(w << 16);
+        b = __uint_as_float(w & 0xffff0000u);
+    }
+};
+struct F16 {
+    typedef f16x8 vec;
+    static constexpr uint32_t INF = 0x7c00, NANBITS = 0x7e00;
+    static __device__ __forceinline__ f32x16 mfma(vec a, vec b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {   // round to nearest even
+        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+        const h2 r = {(_Float16)a, (_Float16)b};
+        return __builtin_bit_cast(uint32_t, r);
+    }
+    static __device__ __forceinline__ void unpack(uint32_t w, float& a, float& b) {
+        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+        const h2 r = __builtin_bit_cast(h2, w);
+        a = (float)r[0];
+        b = (float)r[1];
+    }
+};
+
+template <class T>
+__device__ __forceinline__ typename T::vec as_vec(u32x4 u) {
+    return __builtin_bit_cast(typename T::vec, u);
+}
+// registers 8 half .. 8 half + 7 of an accumulator, rounded once to the input type: the operand that
+// the next product takes (probabilities in [0, 1]; their sum is taken before the rounding)
+template <class T>
+__device__ __forceinline__ typename T::vec round8(const f32x16& v, int half) {
+    u32x4 u;
+    u.x = T::pack(v[8 * half], v[8 * half + 1]);
+    u.y = T::pack(v[8 * half + 2], v[8 * half + 3]);
+    u.z = T::pack(v[8 * half + 4], v[8 * half + 5]);
+    u.w = T::pack(v[8 * half + 6], v[8 * half + 7]);
+    return as_vec<T>(u);
+}
+
+// One LDS image of a [rows][DP] 16-bit tile serves both readers, ds_read_b128 of a row (lane l takes
+// row l & 31) and the transposing ds_read_b64_tr_b16 (a 32-lane half takes 4 rows x 64 B): the 16-B
+// chunk c of a row stands at c ^ key(row).  The row read needs 16 rows of a lane group in 16
+// different 16-B slots of the 256-B bank line, the transposed one needs 4 neighbouring rows in 4
+// different 64-B quarters; with the row's low bits as the chunk's HIGH bits both hold.
+template <int DP>
+__device__ __forceinline__ int swz_key(int row) {
+    if (DP == 64) return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);   // two 128-B rows per bank line
+    return ((row & 3) << 2) | ((row >> 2) & 3);
+}
+template <int DP>
+__device__ __forceinline__ int chunk_at(int row, int c) {   // element offset of chunk c of a row
+    return row * DP + ((c ^ swz_key<DP>(row)) << 3);
+}
+template <int DP>
+__device__ __forceinline__ int elem_at(int row, int col) {
+    return row * DP + (((col >> 3) ^ swz_key<DP>(row)) << 3) + (col & 7);
+}
+__device__ __forceinline__ short4v tr_read(const bf16_t* p) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)(p));
+}
+// operand of 32 columns x 16 rows, columns on the lanes: rows r .. r + 3 and r + 8 .. r + 11 of the
+// lane's half, the order in which an accumulator holds its rows
+template <class T, int DP>
+__device__ __forceinline__ typename T::vec tr_pair(const bf16_t* img, int row, int col) {
+    const short4v a = tr_read(img + elem_at<DP>(row, col)), b = tr_read(img + elem_at<DP>(row + 8, col));
+    const short8v c = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    return __builtin_bit_cast(typename T::vec, c);
+}
+
+// whether one of 8 values is an infinity or NaN (integer test on the exponent field)
+template <class T>
+__device__ __forceinline__ bool not_finite8(u32x4 u) {
+    auto mag = [](uint32_t w) { return __builtin_bit_cast(ushort2v, w & 0x7fff7fffu); };
+    ushort2v m = __builtin_elementwise_max(mag(u.x), mag(u.y));
+    m = __builtin_elementwise_max(m, __builtin_elementwise_max(mag(u.z), mag(u.w)));
+    return m.x >= T::INF || m.y >= T::INF;
+}
+
+// its finite values, zeros for the others
+template <class T>
+__device__ __forceinline__ u32x4 finite_only(u32x4 u) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t w = u[i];
+        if ((w & 0x7fffu) >= T::INF) w &= 0xffff0000u;
+        if (((w >> 16) & 0x7fffu) >= T::INF) w &= 0x0000ffffu;
+        u[i] = w;
+    }
+    return u;
+}
+// The values that finite_only left out of a row (`row`: where it stands in memory), added to the lane's
+// accumulator where it sees the row: what a product with a weight > 0 makes of an infinity or NaN.
+template <class T, int NO>
+__device__ __forceinline__ void add_not_finite(f32x16 (&o)[NO], const bf16_t* row, int D, int h, bool see) {
+#pragma unroll
+    for (int i = 0; i < NO; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int d = 32 * i + 8 * g + 4 * h;
+            const uint2 u = *(const uint2*)(row + (d < D ? d : 0));
+            const uint32_t w[2] = {u.x, u.y};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t x = (w[k >> 1] >> (16 * (k & 1))) & 0xffffu;
+                float lo, hi;
+                T::unpack(x, lo, hi);
+                if (see && d < D && (x & 0x7fffu) >= T::INF) o[i][4 * g + k] += lo;
+            }
+            __builtin_amdgcn_sched_barrier(0);   // hardly ever run: one load at a time, no registers for more
+        }
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float max3(float a, float b, float c) { return __builtin_fmaxf(a, __builtin_fmaxf(b, c)); }
+__device__ __forceinline__ int wave_min_i(int v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, 64));
+    return v;
+}
+__device__ __forceinline__ int wave_max_i(int v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o, 64));
+    return v;
+}
+
+// Scores in units of log 2 (the softmax is taken with 2^x).  tanh u = 1 - 2 / (1 + e^(2 u)): exact to
+// 2^-23 of 1 from v_exp and v_rcp, so of a capped score to cap x 2^-23 (the op takes cap <= 1000:
+// 2^-13, below the rounding of a 16-bit probability), and it saturates without overflow.
+template <bool CAP, bool ALIBI>
+struct Score {
+    static constexpr bool PLAIN = !CAP && !ALIBI;
+    float mul;      // scale log2(e)
+    float c2;       // 2 log2(e) scale / cap
+    float capl;     // cap log2(e)
+    float slope;    // slope log2(e)
+    __device__ __forceinline__ void init(float scale, float cap, float sl) {
+        mul = scale * LOG2E;
+        if (CAP) {
+            c2 = 2.f * LOG2E * scale / cap;
+            capl = cap * LOG2E;
+        }
+        slope = ALIBI ? sl * LOG2E : 0.f;
+    }
+    // 1 / (1 + e^(2 u)), u = x / cap: tanh u = 1 - 2 r, its derivative 4 r (1 - r)
+    __device__ __forceinline__ float sat(float dot) const { return __builtin_amdgcn_rcpf(1.f + exp2_fast(dot * c2)); }
+    __device__ __forceinline__ float capped(float r) const { return fmaf(-2.f * capl, r, capl); }
+    __device__ __forceinline__ float biased(float y, float dist) const {
+        return ALIBI ? fmaf(-slope, fabsf(dist), y) : y;
+    }
+    __device__ __forceinline__ float operator()(float dot, float dist) const {
+        return biased(CAP ? capped(sat(dot)) : dot * mul, dist);
+    }
+};
+
+// Workgroup -> (batch, KV head, query head of the group, block): the blocks of equal index of all heads
+// are neighbours (the longest ones first, `flip`), and the dispatcher deals neighbours over the 8 XCDs,
+// so with a multiple of 8 (batch, KV head) pairs all work on one pair's keys stays on one XCD's L2.
+struct Where {
+    int b, hk, h, blk;
+};
+__device__ __forceinline__ Where place(int L, const Args& a, int nblk, bool flip) {
+    const int G = a.H / a.Hk, nkv = a.B * a.Hk, nbh = nkv * G;
+    const int x = L % nbh, y = L / nbh;
+    int kv, g;
+    if ((nkv & 7) == 0) {
+        const int j = x >> 3;
+        g = j % G;
+        kv = (j / G) * 8 + (x & 7);
+    } else {
+        kv = x / G;
+        g = x - kv * G;
+    }
+    Where w;
+    w.b = kv / a.Hk;
+    w.hk = kv - w.b * a.Hk;
+    w.h = w.hk * G + g;
+    w.blk = flip ? nblk - 1 - y : y;
+    return w;
+}
+
+// Staging of a [ROWS][DP] tile by NTHR threads: thread t takes the 16-B chunk t % (DP / 8) of rows
+// t / (DP / 8) + j RPP.  Rows past the tensor are clamped when loaded (every load stays in bounds)
+// and stored as zeros by put_masked.
+template <class T, int DP, int ROWS, int NTHR>
+struct Tile {
+    static constexpr int NCH = DP / 8, RPP = NTHR / NCH, N = ROWS / RPP;
+    static_assert(ROWS % RPP == 0, "whole passes");
+    static __device__ __forceinline__ int row(int tid, int j) { return tid / NCH + j * RPP; }
+    static __device__ __forceinline__ int chunk(int tid) { return tid % NCH; }
+    // rows r0 .. of `base` (token stride ld, `last` = highest row that exists, D <= DP columns)
+    static __device__ __forceinline__ void load(u32x4 (&v)[N], const bf16_t* base, int64_t ld, int r0, int last, int D, int tid) {
+        const int c = chunk(tid) * 8 < D ? chunk(tid) * 8 : 0;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int r = min(r0 + row(tid, j), last);
+            v[j] = *(const u32x4*)(base + (int64_t)r * ld + c);
+        }
+    }
+    static __device__ __forceinline__ void put(bf16_t* img, const u32x4 (&v)[N], int tid) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) *(u32x4*)(img + chunk_at<DP>(row(tid, j), chunk(tid))) = v[j];
+    }
+    // Tiles that not all of the block's rows see: rows outside [keep0, keep1) (relative to the tile)
+    // and columns past D are zeros, and so are infinities and NaN (a product with a masked
+    // probability 0 would make them NaN); `flags` gets a byte per chunk that says where.
+    static __device__ __forceinline__ void put_masked(bf16_t* img, const u32x4 (&v)[N], int tid, int keep0, int keep1, int D,
+                                                      uint8_t* flags) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int r = row(tid, j), c = chunk(tid);
+            const bool in = r >= keep0 && r < keep1 && c * 8 < D;
+            const bool bad = in && not_finite8<T>(v[j]);
+            const u32x4 z = (u32x4)(0u);
+            u32x4 u = in ? v[j] : z;
+            if (bad) u = finite_only<T>(u);
+            *(u32x4*)(img + chunk_at<DP>(r, c)) = u;
+            flags[r * NCH + c] = bad ? 1 : 0;
+        }
+    }
+};
+// the rows of a flagged tile of 64: bit r set where a chunk of row r was not finite
+template <int DP>
+__device__ __forceinline__ uint64_t flagged_rows(const uint8_t* flags, int lane) {
+    const uint2* p = (const uint2*)(flags + lane * (DP / 8));
+    uint32_t any = p[0].x | p[0].y;
+    if (DP == 128) any |= p[1].x | p[1].y;
+    return __ballot(any != 0);
+}
+__device__ __forceinline__ uint64_t bits_below(int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; }
+
+}  // namespace mattn

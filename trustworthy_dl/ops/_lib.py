@@ -152,6 +152,10 @@ _SIGNATURES = {
     # attention.hip
     "tdl_attn_fwd": [_P, _P, _P, _P, _I, _I, _I, _I, _F, _I, _P],
     "tdl_attn_bwd": [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _F, _I, _P],
+    # masked_attention_fwd.hip / masked_attention_bwd.hip
+    "tdl_attn_mask": [_P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P],
+    "tdl_masked_attn_fwd": [_P, _P],
+    "tdl_masked_attn_bwd": [_P, _P],
     # gemm.hip
     "tdl_gemm": [_P] * 6 + [_I] * 10 + [_L, _P],
     "tdl_gemm_wgrad_grouped": [_P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P],

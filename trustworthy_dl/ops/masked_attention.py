@@ -1,0 +1,409 @@
+"""Attention under document, prefix and length masks, with capped scores and a distance bias.
+
+``causal_attention`` is GPT-2's dense training attention on packed qkv.  The ops here take separate
+query / key / value heads (shared KV heads included) and the masks that packed fine-tuning batches and
+caches need, for whole sequences (forward and backward) and for single tokens against a cache:
+
+    mask = attention_mask(B, Tq, Tk, documents=ids)          # once per batch, for every layer
+    out  = masked_attention(q, k, v, mask, softcap=50.0, slopes=slopes)
+
+``documents``, ``prefix``, ``lengths`` and ``causal`` leave each query one interval of visible keys; the
+mask object holds those intervals and the tables that let the kernels skip whole tiles.  GPU tensors run
+csrc/masked_attention_fwd.hip / _bwd.hip (bf16 and fp16, head dims up to 128); CPU tensors run the same
+definition in PyTorch.  Results and gradients are the same bits in every run (no atomics).
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from ._lib import ptr, stream_ptr
+
+_Q_TILE, _K_TILE = 32, 128     # csrc/masked_attention.h QT, KT
+MAX_SOFTCAP = 1000.0
+
+
+class _on_device:
+    """Launch on the tensors' device, whichever device is current."""
+
+    def __init__(self, device: torch.device):
+        self.guard = None if device.index in (None, torch.cuda.current_device()) else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+        return False
+
+
+# ============================================================== the mask
+class AttentionMask:
+    """Which keys each query of a batch sees: ``lo[b, i] <= j < hi[b, i]`` (``attention_mask``).
+
+    Made from its inputs once; later changes of those tensors are not seen.  Like any tensor, a mask
+    built on one stream is used on another only after that stream has waited for the first."""
+
+    def __init__(self, batch: int, q_len: int, k_len: int, lo: torch.Tensor, hi: torch.Tensor, pos: torch.Tensor,
+                 q_table: Optional[torch.Tensor], k_table: Optional[torch.Tensor]):
+        self.batch, self.q_len, self.k_len = batch, q_len, k_len
+        self.lo, self.hi, self.pos = lo, hi, pos
+        self.q_table, self.k_table = q_table, k_table
+
+    @property
+    def device(self) -> torch.device:
+        return self.lo.device
+
+    def dense(self) -> torch.Tensor:
+        """[batch, q_len, k_len] booleans (for inspection and the CPU path)."""
+        j = torch.arange(self.k_len, device=self.device)
+        return (j >= self.lo[..., None]) & (j < self.hi[..., None])
+
+
+def _int_input(name: str, t: Optional[torch.Tensor], shape, device, dtypes=(torch.int32, torch.int64)):
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor) or t.dtype not in dtypes:
+        raise ValueError(f"{name} must be a tensor of {' or '.join(str(d) for d in dtypes)}, got "
+                         f"{t.dtype if isinstance(t, torch.Tensor) else type(t).__name__}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the mask on {device}")
+    return t.contiguous()
+
+
+def attention_mask(batch: int, q_len: int, k_len: Optional[int] = None, *, causal: bool = True,
+                   documents: Optional[torch.Tensor] = None, prefix: Optional[torch.Tensor] = None,
+                   lengths: Optional[torch.Tensor] = None, q_start: Optional[torch.Tensor] = None,
+                   device=None) -> AttentionMask:
+    """The mask of ``batch`` rows of ``q_len`` queries over ``k_len`` keys (default: as many).
+
+    ``causal``     a query at position p sees the keys at positions <= p (else all of its row / document)
+    ``documents``  int [batch, k_len]: document id of every position.  A document is a run of equal ids;
+                   positions see their own document only.  A negative id marks padding: it sees nothing
+                   and is seen by nothing.
+    ``prefix``     positions that are seen both ways under ``causal``: int [batch] = the row's first
+                   prefix[b] positions (without ``documents``), or bool [batch, k_len] marking the
+                   positions with which each document (or row) begins.
+    ``lengths``    int [batch]: valid positions of each row; keys behind them are never seen and queries
+                   behind them see nothing.
+    ``q_start``    int [batch]: position of each row's first query.  Default: the queries are the last
+                   ``q_len`` valid positions of the row (a cache), or with q_len == k_len start at 0.
+    """
+    k_len = q_len if k_len is None else k_len
+    if batch < 0 or q_len < 0 or k_len < q_len:
+        raise ValueError(f"attention_mask needs 0 <= q_len <= k_len, got batch {batch}, q_len {q_len}, k_len {k_len}")
+    if max(q_len, k_len) >= 1 << 30:
+        raise ValueError("attention_mask: at most 2^30 - 1 positions")
+    if device is None:
+        device = next((t.device for t in (documents, prefix, lengths, q_start) if isinstance(t, torch.Tensor)), torch.device("cpu"))
+    device = torch.device(device)
+    if device.type == "cuda" and device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
+    documents = _int_input("documents", documents, (batch, k_len), device)
+    lengths = _int_input("lengths", lengths, (batch,), device)
+    q_start = _int_input("q_start", q_start, (batch,), device)
+    rows = marks = None
+    if prefix is not None:
+        if not causal:
+            raise ValueError("prefix needs causal=True (without it every position is seen both ways already)")
+        if isinstance(prefix, torch.Tensor) and prefix.dim() == 2:
+            marks = _int_input("prefix", prefix, (batch, k_len), device, (torch.bool, torch.uint8))
+        else:
+            rows = _int_input("prefix", prefix, (batch,), device)
+            if documents is not None:
+                raise ValueError("with documents the prefix is given per position: bool [batch, k_len]")
+    small = [None if t is None else t.clamp(-(1 << 30), 1 << 30).to(torch.int32) if t.dtype == torch.int64 else t
+             for t in (lengths, q_start, rows)]
+    lengths, q_start, rows = small
+    if device.type != "cuda":
+        return _mask_reference(batch, q_len, k_len, causal, documents, rows, marks, lengths, q_start, device)
+
+    def ints(*shape):
+        return torch.empty(shape, dtype=torch.int32, device=device)
+    nq, nk = -(-q_len // _Q_TILE), -(-k_len // _K_TILE)
+    m = AttentionMask(batch, q_len, k_len, ints(batch, q_len), ints(batch, q_len), ints(batch), ints(batch, nq, 4),
+                      ints(batch, nk, 2))
+    if batch == 0 or q_len == 0:
+        return m
+    ws = ints(batch * 3 * k_len) if documents is not None or marks is not None else None
+    with _on_device(device):
+        _lib.call("tdl_attn_mask", ptr(documents), int(documents is not None and documents.dtype == torch.int64), ptr(rows),
+                  ptr(marks), ptr(lengths), ptr(q_start), batch, q_len, k_len, int(causal), ptr(ws), ptr(m.lo), ptr(m.hi),
+                  ptr(m.pos), ptr(m.q_table), ptr(m.k_table), stream_ptr(device))
+    return m
+
+
+def _mask_reference(B, Tq, Tk, causal, documents, rows, marks, lengths, q_start, device) -> AttentionMask:
+    j = torch.arange(Tk, device=device).expand(B, Tk)
+    length = (lengths.clamp(0, Tk) if lengths is not None else torch.full((B,), Tk, device=device)).long()
+    start, end = torch.zeros(B, Tk, dtype=torch.long, device=device), torch.full((B, Tk), Tk, device=device)
+    if documents is not None and Tk:
+        edge = torch.ones(B, Tk + 1, dtype=torch.bool, device=device)
+        edge[:, 1:Tk] = documents[:, 1:] != documents[:, :-1]
+        start = torch.cummax(torch.where(edge[:, :Tk], j, 0), 1)[0]
+        end = torch.flip(torch.cummin(torch.flip(torch.where(edge[:, 1:], j + 1, Tk), [1]), 1)[0], [1])
+    p0 = q_start.long() if q_start is not None else (length - Tq if Tq < Tk else torch.zeros_like(length))
+    p = p0[:, None] + torch.arange(Tq, device=device)
+    ok = (p >= 0) & (p < length[:, None])
+    pc = p.clamp(0, max(Tk - 1, 0))
+    if Tk and documents is not None:
+        ok &= documents.gather(1, pc) >= 0
+    if Tk == 0 or B == 0 or Tq == 0:
+        lo = hi = torch.zeros(B, Tq, dtype=torch.int32, device=device)
+        return AttentionMask(B, Tq, Tk, lo, hi, p0.int(), None, None)
+    e = torch.minimum(end.gather(1, pc), length[:, None])
+    lo, hi = start.gather(1, pc), e
+    if causal:
+        pe = torch.zeros_like(e)
+        if marks is not None:
+            free = torch.flip(torch.cummin(torch.flip(torch.where(marks == 0, j, Tk), [1]), 1)[0], [1])
+            pe = free.gather(1, lo)
+        elif rows is not None:
+            pe = rows.long()[:, None].expand_as(e)
+        hi = torch.maximum(p + 1, torch.minimum(pe, e))
+    zero = torch.zeros_like(lo)
+    return AttentionMask(B, Tq, Tk, torch.where(ok, lo, zero).int(), torch.where(ok, hi, zero).int(), p0.int(), None, None)
+
+
+# ============================================================== launches
+class _Args(ctypes.Structure):
+    """csrc/masked_attention.h mattn::Args"""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v", "dout", "o", "dq", "dk", "dv", "lse", "delta", "ws", "slopes",
+                                                "lo", "hi", "pos", "qtab", "ktab")]
+                + [(n, ctypes.c_int64 * 3) for n in ("qs", "ks", "vs", "os", "dos", "dqs", "dks", "dvs")]
+                + [(n, ctypes.c_int) for n in ("B", "Tq", "Tk", "H", "Hk", "D", "dtype", "nsplit")]
+                + [("scale", ctypes.c_float), ("cap", ctypes.c_float)])
+
+
+def _strides(t: torch.Tensor):
+    # a dimension of one element is never stepped over
+    return (ctypes.c_int64 * 3)(*[t.stride(i) if t.shape[i] > 1 else 0 for i in range(3)])
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """``t`` [B, T, heads, D] with unit column stride and 16-byte rows: as it is, or a contiguous copy."""
+    if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(t.stride(i) % 8 == 0 for i in range(3) if t.shape[i] > 1):
+        return t
+    return t.contiguous()
+
+
+def few_queries(batch: int, kv_heads: int, group: int, q_len: int, k_len: int) -> int:
+    """0: the tiled kernel (32 queries of one head per wave).  Else the number of key ranges of the
+    few-queries kernel, which reads K / V once for the rows (heads of a group x queries) of a tile of 32."""
+    if q_len > 16:
+        return 0
+    tiles = batch * kv_heads * -(-(group * q_len) // 32)
+    return max(1, min(1024 // tiles, -(-k_len // 128), 64))
+
+
+def _args(q, k, v, mask: AttentionMask, scale: float, cap: float, slopes) -> _Args:
+    a = _Args()
+    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    a.qs, a.ks, a.vs = _strides(q), _strides(k), _strides(v)
+    a.B, a.Tq, a.H, a.D = q.shape
+    a.Tk, a.Hk = k.shape[1], k.shape[2]
+    a.dtype = _lib.DTYPE_CODE[q.dtype]
+    a.scale, a.cap = scale, cap
+    a.slopes = 0 if slopes is None else slopes.data_ptr()
+    a.lo, a.hi, a.pos = mask.lo.data_ptr(), mask.hi.data_ptr(), mask.pos.data_ptr()
+    a.qtab, a.ktab = mask.q_table.data_ptr(), mask.k_table.data_ptr()
+    return a
+
+
+def _forward(q, k, v, mask, scale, cap, slopes, want_lse: bool):
+    B, Tq, H, D = q.shape
+    Tk, Hk = k.shape[1], k.shape[2]
+    out = torch.empty(B, Tq, H, D, dtype=q.dtype, device=q.device)
+    lse = torch.empty(B, H, Tq, dtype=torch.float32, device=q.device) if want_lse else None
+    if out.numel() == 0:
+        return out, lse
+    a = _args(q, k, v, mask, scale, cap, slopes)
+    a.o, a.os = out.data_ptr(), _strides(out)
+    a.lse = 0 if lse is None else lse.data_ptr()
+    a.nsplit = few_queries(B, Hk, H // Hk, Tq, Tk)
+    ws = None
+    if a.nsplit > 1:
+        ws = torch.empty(B * H * Tq * a.nsplit * ((64 if D <= 64 else 128) + 2), dtype=torch.float32, device=q.device)
+        a.ws = ws.data_ptr()
+    with _on_device(q.device):
+        _lib.call("tdl_masked_attn_fwd", ctypes.addressof(a), stream_ptr(q.device))
+    return out, lse
+
+
+def _backward(q, k, v, out, lse, dout, mask, scale, cap, slopes, dq, dk, dv):
+    """Writes dq and, unless both are None, dk and dv."""
+    if q.numel() == 0:
+        for g in (dk, dv):
+            if g is not None:
+                g.zero_()
+        return
+    a = _args(q, k, v, mask, scale, cap, slopes)
+    delta = torch.empty_like(lse)
+    a.o, a.os, a.lse, a.delta = out.data_ptr(), _strides(out), lse.data_ptr(), delta.data_ptr()
+    a.dout, a.dos = dout.data_ptr(), _strides(dout)
+    a.dq, a.dqs = dq.data_ptr(), _strides(dq)
+    if dk is not None:
+        a.dk, a.dv, a.dks, a.dvs = dk.data_ptr(), dv.data_ptr(), _strides(dk), _strides(dv)
+    with _on_device(q.device):
+        _lib.call("tdl_masked_attn_bwd", ctypes.addressof(a), stream_ptr(q.device))
+
+
+class _MaskedAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, mask, scale, cap, slopes, want_lse):
+        q, k, v = _aligned(q), _aligned(k), _aligned(v)
+        out, lse = _forward(q, k, v, mask, scale, cap, slopes, want_lse or any(ctx.needs_input_grad[:3]))
+        ctx.save_for_backward(q, k, v, out, lse, slopes)
+        ctx.mask, ctx.scale, ctx.cap = mask, scale, cap
+        if lse is not None:
+            ctx.mark_non_differentiable(lse)
+        return out, lse
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout, _dlse):
+        q, k, v, out, lse, slopes = ctx.saved_tensors
+        keys = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
+        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        dk = torch.empty(k.shape, dtype=k.dtype, device=k.device) if keys else None
+        dv = torch.empty(v.shape, dtype=v.dtype, device=v.device) if keys else None
+        _backward(q, k, v, out, lse, _aligned(dout), ctx.mask, ctx.scale, ctx.cap, slopes, dq, dk, dv)
+        return dq, dk, dv, None, None, None, None, None
+
+
+class _MaskedAttentionPacked(torch.autograd.Function):
+    """The gradients of q, k and v are written straight into one packed gradient."""
+
+    @staticmethod
+    def forward(ctx, qkv, n_head, n_kv_head, mask, scale, cap, slopes):
+        qkv = _aligned(qkv)
+        q, k, v = qkv.split((n_head, n_kv_head, n_kv_head), dim=2)
+        out, lse = _forward(q, k, v, mask, scale, cap, slopes, ctx.needs_input_grad[0])
+        ctx.save_for_backward(qkv, out, lse, slopes)
+        ctx.mask, ctx.scale, ctx.cap, ctx.heads = mask, scale, cap, (n_head, n_kv_head, n_kv_head)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        qkv, out, lse, slopes = ctx.saved_tensors
+        dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
+        _backward(*qkv.split(ctx.heads, dim=2), out, lse, _aligned(dout), ctx.mask, ctx.scale, ctx.cap, slopes,
+                  *dqkv.split(ctx.heads, dim=2))
+        return dqkv, None, None, None, None, None, None
+
+
+# ============================================================== CPU definition
+def _reference(q, k, v, mask, scale, cap, slopes):
+    """The definition with differentiable torch operations, in 32 bits (64 for double inputs)."""
+    wide = torch.float64 if q.dtype == torch.float64 else torch.float32
+    B, Tq, H, D = q.shape
+    G = H // k.shape[2]
+    seen = mask.dense()
+    # a key that no query of its row sees takes no part, whatever stands there
+    used = seen.any(1)[:, :, None, None] if Tq else torch.zeros(B, k.shape[1], 1, 1, dtype=torch.bool, device=k.device)
+    qf = q.to(wide).transpose(1, 2)
+    kf, vf = (torch.where(used, t.to(wide), torch.zeros((), dtype=wide)).transpose(1, 2).repeat_interleave(G, 1) for t in (k, v))
+    s = (qf @ kf.transpose(-1, -2)) * scale
+    if cap:
+        s = cap * torch.tanh(s / cap)
+    if slopes is not None:
+        p = mask.pos.long()[:, None] + torch.arange(Tq, device=q.device)
+        dist = (p[:, :, None] - torch.arange(mask.k_len, device=q.device)).abs()
+        s = s - slopes.to(wide).view(1, H, 1, 1) * dist[:, None].to(wide)
+    s = s.masked_fill(~seen[:, None], float("-inf"))
+    top = s.detach().amax(-1, keepdim=True) if mask.k_len else s.new_zeros(B, H, Tq, 1)
+    top = torch.where(torch.isinf(top), torch.zeros_like(top), top)
+    e = torch.exp(s - top)
+    z = e.sum(-1, keepdim=True)
+    out = (e / torch.where(z == 0, torch.ones_like(z), z)) @ vf
+    lse = torch.where(z == 0, torch.full_like(z, float("-inf")), top + torch.log(z))[..., 0].detach().float()
+    return out.transpose(1, 2).to(q.dtype), lse
+
+
+# ============================================================== entry points
+def _check(name: str, q, k, v, mask, scale, softcap, slopes):
+    if not isinstance(mask, AttentionMask):
+        raise ValueError(f"{name} needs a mask made by attention_mask, got {type(mask).__name__}")
+    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape:
+        raise ValueError(f"{name}: q [B, Tq, H, D], k and v [B, Tk, Hk, D], got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    B, Tq, H, D = q.shape
+    Hk = k.shape[2]
+    if k.shape[0] != B or k.shape[3] != D or Hk == 0 or H == 0 or H % Hk:
+        raise ValueError(f"{name}: {H} query heads of {tuple(q.shape)} do not share the KV heads of {tuple(k.shape)}")
+    if (mask.batch, mask.q_len, mask.k_len) != (B, Tq, k.shape[1]):
+        raise ValueError(f"{name}: the mask is for (batch, q_len, k_len) = {(mask.batch, mask.q_len, mask.k_len)}, the tensors have "
+                         f"{(B, Tq, k.shape[1])}")
+    if not (q.dtype == k.dtype == v.dtype):
+        raise ValueError(f"{name}: q, k and v differ in type ({q.dtype}, {k.dtype}, {v.dtype})")
+    if not (q.device == k.device == v.device == mask.device):
+        raise ValueError(f"{name}: q, k, v and the mask are on {q.device}, {k.device}, {v.device}, {mask.device}")
+    if q.is_cuda:
+        if q.dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError(f"native {name} supports bfloat16 and float16 (got {q.dtype})")
+        if D % 8 or not 8 <= D <= 128:
+            raise ValueError(f"native {name} supports head dims that are multiples of 8 up to 128 (got {D})")
+    elif not q.dtype.is_floating_point:
+        raise ValueError(f"{name}: floating-point inputs, got {q.dtype}")
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    if not (scale > 0 and math.isfinite(scale)):
+        raise ValueError(f"{name}: scale must be positive, got {scale}")
+    cap = 0.0 if softcap is None else float(softcap)
+    if softcap is not None and not 0 < cap <= MAX_SOFTCAP:
+        # cap tanh(x / cap) is evaluated to cap x 2^-23: beyond this the cap's own rounding would show
+        raise ValueError(f"{name}: softcap must lie in (0, {MAX_SOFTCAP:g}], got {softcap}")
+    if slopes is not None:
+        if slopes.shape != (H,) or slopes.device != q.device:
+            raise ValueError(f"{name}: slopes must be a [{H}] tensor on {q.device}, got {tuple(slopes.shape)} on {slopes.device}")
+        if slopes.requires_grad:
+            raise ValueError(f"{name}: slopes are constants (no gradient is computed for them); pass slopes.detach()")
+        slopes = slopes.to(torch.float32).contiguous()
+    return scale, cap, slopes
+
+
+def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: AttentionMask, *, scale: Optional[float] = None,
+                     softcap: Optional[float] = None, slopes: Optional[torch.Tensor] = None, return_lse: bool = False):
+    """softmax(s) v over the keys each query sees, ``s = cap tanh(scale q.k / cap) - slopes[h] |p - j|``.
+
+    q [B, Tq, H, D], k and v [B, Tk, Hk, D] with H a multiple of Hk (query head h reads KV head
+    h // (H / Hk)); any batch / token / head strides.  ``scale`` defaults to 1 / sqrt(D); without
+    ``softcap`` the scores are not capped, without ``slopes`` (fp32 [H]) there is no distance bias
+    (p, j: positions of query and key).  Returns [B, Tq, H, D] in q's type; a query that sees nothing
+    gives zeros, and keys it does not see have no effect on it, whatever they hold.  With
+    ``return_lse`` also the fp32 log-sum-exp of each query's scores [B, H, Tq] (-inf where it sees
+    nothing; not differentiable)."""
+    scale, cap, slopes = _check("masked_attention", q, k, v, mask, scale, softcap, slopes)
+    if q.is_cuda:
+        out, lse = _MaskedAttention.apply(q, k, v, mask, scale, cap, slopes, return_lse)
+    else:
+        out, lse = _reference(q, k, v, mask, scale, cap, slopes)
+    return (out, lse) if return_lse else out
+
+
+def masked_attention_packed(qkv: torch.Tensor, n_head: int, mask: AttentionMask, *, n_kv_head: Optional[int] = None,
+                            scale: Optional[float] = None, softcap: Optional[float] = None,
+                            slopes: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``masked_attention`` on a projection's packed output [B, T, (H + 2 Hk) D] -> [B, T, H D]: query
+    heads, then key heads, then value heads, as ``causal_attention`` takes them.  The gradient comes
+    back packed too."""
+    hk = n_head if n_kv_head is None else n_kv_head
+    if qkv.dim() != 3 or n_head < 1 or hk < 1 or qkv.shape[2] % (n_head + 2 * hk):
+        raise ValueError(f"masked_attention_packed: {tuple(qkv.shape)} does not hold {n_head} + 2 x {hk} heads")
+    B, T, C = qkv.shape
+    x = qkv.reshape(B, T, n_head + 2 * hk, C // (n_head + 2 * hk))
+    q, k, v = x.split((n_head, hk, hk), dim=2)
+    scale, cap, slopes = _check("masked_attention_packed", q, k, v, mask, scale, softcap, slopes)
+    if qkv.is_cuda:
+        out = _MaskedAttentionPacked.apply(x, n_head, hk, mask, scale, cap, slopes)
+    else:
+        out, _ = _reference(q, k, v, mask, scale, cap, slopes)
+    return out.reshape(B, T, -1)
