@@ -6,10 +6,11 @@
 //   loss = alpha mean_kd + (1 - alpha) mean_ce    (means over the rows that have entries / a label)
 //   dz_j = alpha tau / n_t (p_tau_j - sum_{k : i_k = j} q_k) + (1 - alpha) / n_l (p_j - [j = label])
 //
-// A row belongs to one workgroup that keeps it in REGISTERS between the statistics and the gradient, so
-// memory sees the logits once and the gradient once: the bound.  1024 threads hold a row of 50304
-// 16-bit logits in 7 16-byte registers each; two such workgroups fit a CU, one loading while the other
-// stores.  Rows too long for the registers are read a second time.
+// Bound by memory: the logits are read and their gradient written once each, 3.3 GB and 806 us (4.1 TB/s)
+// for 16384 rows of 50304 bf16 logits.  A row belongs to one workgroup (a wave, for short rows) that
+// keeps it in registers between the statistics and the gradient, or, where there are many long rows,
+// reads it a second time from the Infinity Cache: 5 rows of 100 KB a CU are 130 MB of its 256 MB, and the
+// gradient is stored past it (nontemporal: 834 instead of 886 us).
 //
 // The gradient at a row's few special columns (its teacher entries and label) is written over the
 // row's stores by threads that own an entry, from the same fp32 terms and with one rounding: the
@@ -135,17 +136,28 @@ __global__ __launch_bounds__(256) void distill_count_kernel(const DistillArgs a)
     }
 }
 
-// Adds the rows' shares (fixed order: thread t takes rows t, t + 1024, ...; then a tree).
+// Adds the rows' shares (fixed order: thread t takes rows 4 t .. 4 t + 3 of every 4096; then a tree).
 __global__ __launch_bounds__(1024) void distill_loss_kernel(const float* __restrict__ rows, float* __restrict__ loss, int M) {
     __shared__ float red[16];
     float s = 0.f;
-    for (int i = threadIdx.x; i < M; i += 1024) s += rows[i];
+    const int whole = M & ~4095;
+    int i = threadIdx.x * 4;
+#pragma unroll 4
+    for (; i < whole; i += 4096) {
+        const float4 v = *(const float4*)(rows + i);
+        s += (v.x + v.y) + (v.z + v.w);
+    }
+    for (int r = whole + threadIdx.x; r < M; r += 1024) s += rows[r];
     s = block_sum(s, red);
     if (threadIdx.x == 0) *loss = s;
 }
 
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
-
+// a value that all lanes hold alike, kept in a scalar register
+__device__ __forceinline__ float uniform(float x) {
+    return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x)));
+}
+__device__ __forceinline__ float zero_if_none(float m) { return m == -INFINITY ? 0.f : m; }
 // Opaque to the optimiser: a piece stays packed (4 registers) between the passes and is unpacked in
 // each, instead of living as 8 floats across them.
 template <int N>
@@ -154,25 +166,47 @@ __device__ __forceinline__ void keep_packed(u32x4 (&q)[N]) {
     for (int t = 0; t < N; ++t) asm volatile("" : "+v"(q[t]));
 }
 
-// the unpacked values of a piece die before the next piece's are made
-__device__ __forceinline__ void one_at_a_time() { __builtin_amdgcn_sched_barrier(0); }
+// The two softmaxes of a row, 2^(d ct) and 2^(d log2 e) for d = z - (some maximum).  MODE -1: no
+// cross-entropy, the first alone.  An exponential issues for 8 cycles where a product takes 4, so where
+// the temperature allows the second one is a power of the first, e^d = (e^(d / tau))^tau: MODE 1, 2, 4
+// for those temperatures.  MODE 0, any other one, takes both.
+// 16-bit logits take z c - m c in one fma (its rounding is 2^-24 of |m c|, alike in numerator and
+// sum); fp32 ones subtract first.
+template <class T, int MODE>
+struct Soft {
+    float ct;
+    static __device__ __forceinline__ float one(float f, float m, float c) {
+        return T::E == 8 ? exp2_(fmaf(f, c, -(m * c))) : exp2_((f - m) * c);
+    }
+    // t = 2^((f - m) ct), o = 2^((f - m) log2 e)
+    __device__ __forceinline__ void operator()(float f, float m, float& t, float& o) const {
+        t = one(f, m, ct);
+        if (MODE == 0) o = one(f, m, 1.4426950408889634f);
+        else if (MODE > 0) o = MODE == 1 ? t : MODE == 2 ? t * t : (t * t) * (t * t);
+    }
+};
 
-// NV: 16-byte pieces of the row per thread that stay in registers (0: the row is read twice).
-// MIX: the cross-entropy term takes part (beta > 0).
-template <class T, int NT, int NV, bool MIX, bool GRAD>
-__global__ __launch_bounds__(NT, NV <= 8 ? 8 : 4) void distill_kernel(const DistillArgs a) {
-    constexpr int E = T::E, NW = NT / 64;
+// NT threads a row.  NV: 16-byte pieces of the row per thread that stay in registers; 0: the row streams
+// through twice.
+template <class T, int NT, int NV, int MODE, bool GRAD>
+__global__ __launch_bounds__(NT, 4) void distill_kernel(const DistillArgs a) {
+    constexpr int E = T::E, NW = NT / 64, UN = 4;
+    constexpr bool MIX = MODE >= 0;   // the cross-entropy term takes part (beta > 0)
+    constexpr float L2E = 1.4426950408889634f;
     typedef typename T::S S;
-    extern __shared__ __attribute__((aligned(16))) char smem[];   // K entries: index, then weight
+    // the row's entries 0 .. K - 1, and its label as entry K: index, (t - max) / tau, e^that, logit
+    extern __shared__ __attribute__((aligned(16))) char smem[];
     __shared__ float red[NW][3];
-    __shared__ float tred[4];
+    __shared__ float tred[3];
     __shared__ int cnt[2];
     int* sidx = (int*)smem;
-    float* sq = (float*)(sidx + a.K);
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    float* su = (float*)(sidx + a.K + 1);
+    float* se = su + a.K + 1;
+    float* sz = se + a.K + 1;
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const float gs = a.gscale != nullptr ? *a.gscale : 1.f;
     if (a.written && gs == 1.f) return;   // the forward wrote this gradient already
-    if (tid < 64) {   // the counts of the whole batch
+    if (w == 0) {   // the counts of the whole batch
         int nt = 0, nl = 0;
         for (int g = lane; g < a.G; g += 64) {
             nt += a.counts[2 * g];
@@ -188,6 +222,8 @@ __global__ __launch_bounds__(NT, NV <= 8 ? 8 : 4) void distill_kernel(const Dist
             cnt[1] = nl;
         }
     }
+    const Soft<T, MODE> soft{L2E / a.tau};
+    const float it = 1.f / a.tau;
     for (int row = blockIdx.x; row < a.M; row += gridDim.x) {
         const S* z = (const S*)a.logits + (int64_t)row * a.ld;
         // whole 16-byte pieces from the first boundary on; the elements before and behind them (less
@@ -195,12 +231,12 @@ __global__ __launch_bounds__(NT, NV <= 8 ? 8 : 4) void distill_kernel(const Dist
         const int skew = (int)(((uintptr_t)z & 15) / sizeof(S));
         const int a0 = min(skew ? E - skew : 0, a.V), np = (a.V - a0) / E, a1 = a0 + np * E;
         const int e0 = tid == 0 ? 0 : a1, e1 = tid == 0 ? a0 : tid == 1 ? a.V : a1;   // this thread's edge elements
-        auto load = [&](int p) { return *(const u32x4*)(z + a0 + (int64_t)p * E); };
+        const u32x4* zp = (const u32x4*)(z + a0);
         u32x4 q[NV > 0 ? NV : 1], qe;
 #pragma unroll
         for (int t = 0; t < NV; ++t) {
             const int p = tid + t * NT;
-            if (p < np) q[t] = load(p);
+            if (p < np) q[t] = zp[p];
         }
         {
             float f[E];
@@ -208,84 +244,118 @@ __global__ __launch_bounds__(NT, NV <= 8 ? 8 : 4) void distill_kernel(const Dist
             for (int i = 0; i < E; ++i) f[i] = e0 + i < e1 ? T::get(z[e0 + i]) : -INFINITY;
             qe = T::pack(f);   // exact: the values come from this type
         }
-        // ---- the last wave takes the teacher's entries: sum of e^(t - max), weights to LDS
-        const int label = MIX ? label_of(a, row) : -1;
+        // ---- the last wave takes the teacher's entries
         if (w == NW - 1) {
-            float tm = -INFINITY;
+            float tm = -INFINITY, nan = 0.f, any = 0.f;
             for (int k = lane; k < a.K; k += 64) {
                 const int64_t at = (int64_t)row * a.K + k;
                 const int i = entry_at(a, at);
                 const float t = i >= 0 ? teacher_at(a, at) : -INFINITY;
                 sidx[k] = i;
-                sq[k] = t;
-                tm = t == t ? fmaxf(tm, t) : t;
+                su[k] = t;
+                sz[k] = i >= 0 ? T::get(z[i]) : 0.f;   // (before the row is overwritten: grad may be the logits)
+                tm = fmaxf(tm, t);
+                nan += t == t ? 0.f : 1.f;
+                any += i >= 0 ? 1.f : 0.f;
             }
-            float any = 0.f, nan = tm == tm ? 0.f : 1.f;
-#pragma unroll
-            for (int o = 32; o > 0; o >>= 1) {
-                nan += __shfl_xor(nan, o, 64);
-                tm = fmaxf(tm, __shfl_xor(tm, o, 64));
-            }
+            tm = wave_max(tm);
             float ts = 0.f;
-            const float c = 1.f / a.tau;
             for (int k = lane; k < a.K; k += 64) {
-                const float e = sq[k] == -INFINITY ? 0.f : __expf((sq[k] - tm) * c);
-                any += sidx[k] >= 0 ? 1.f : 0.f;
+                const float u = (su[k] - tm) * it, e = su[k] == -INFINITY ? 0.f : __expf(u);
+                su[k] = u;
+                se[k] = e;
                 ts += e;
             }
             ts = wave_sum(ts);
+            nan = wave_sum(nan);
             any = wave_sum(any);
             if (lane == 0) {
-                tred[0] = tm;
-                tred[1] = nan > 0.f ? __uint_as_float(0x7fc00000u) : ts;
-                tred[2] = any;
+                const int l = MIX ? label_of(a, row) : -1;
+                sidx[a.K] = l;
+                se[a.K] = 0.f;
+                sz[a.K] = l >= 0 ? T::get(z[l]) : 0.f;
+                tred[0] = nan > 0.f ? __uint_as_float(0x7fc00000u) : ts;
+                tred[1] = any;
             }
         }
-        // ---- the row's maximum and sums of 2^((z - max) log2(e) / tau) and 2^((z - max) log2(e)); each wave
-        // with its own maximum, joined through LDS
-        const float L2E = 1.4426950408889634f;
-        const float ct = L2E / a.tau;
-        float m = -INFINITY;
+        // ---- the row's maximum and sums, each wave with its own maximum, joined through LDS
+        float m = -INFINITY, st = 0.f, s1 = 0.f;
         auto top = [&](const u32x4& u) {
             float f[E];
             T::unpack(u, f);
+            float t = f[0];
 #pragma unroll
-            for (int i = 0; i < E; ++i) m = fmaxf(m, f[i]);
+            for (int i = 1; i < E; ++i) t = fmaxf(t, f[i]);
+            return t;
         };
-        top(qe);
-        if constexpr (NV > 0) {
-#pragma unroll
-            for (int t = 0; t < NV; ++t) {
-                if (tid + t * NT < np) top(q[t]);
-                one_at_a_time();
-            }
-            keep_packed(q);
-        } else {
-            for (int p = tid; p < np; p += NT) top(load(p));
-        }
-        m = wave_max(m);
-        const float mz = m == -INFINITY ? 0.f : m;
-        float st = 0.f, s1 = 0.f;
-        auto sums = [&](const u32x4& u) {
-            float f[E];
+        auto sums = [&](const u32x4& u, float mz) {
+            float f[E], at = 0.f, a1_ = 0.f;
             T::unpack(u, f);
 #pragma unroll
             for (int i = 0; i < E; ++i) {
-                const float d = f[i] - mz;
-                st += exp2_(d * ct);
-                if (MIX) s1 += exp2_(d * L2E);
+                float t, o = 0.f;
+                soft(f[i], mz, t, o);
+                at += t;
+                a1_ += o;
             }
+            st += at;
+            if (MIX) s1 += a1_;
+            asm volatile("" : "+v"(st), "+v"(s1));   // a piece is added before the next one's values are made
         };
-        if (e0 < e1) sums(qe);
+        auto rescale = [&](float d) {   // the sums, taken against a maximum, against one higher by -d
+            st *= exp2_(d * soft.ct);
+            if (MIX) s1 *= exp2_(d * L2E);
+        };
         if constexpr (NV > 0) {
+            m = top(qe);
 #pragma unroll
             for (int t = 0; t < NV; ++t) {
-                if (tid + t * NT < np) sums(q[t]);
-                one_at_a_time();
+                if (tid + t * NT < np) m = fmaxf(m, top(q[t]));
+                __builtin_amdgcn_sched_barrier(0);
             }
             keep_packed(q);
+            m = wave_max(m);
+            const float mz = zero_if_none(m);
+            if (e0 < e1) sums(qe, mz);
+#pragma unroll
+            for (int t = 0; t < NV; ++t)
+                if (tid + t * NT < np) sums(q[t], mz);
+            keep_packed(q);
         } else {
-            for (int p = tid; p < np; p += NT) sums(load(p));
+            // running maximum of the wave; the sums are rescaled where it rises (seldom after the first
+            // pieces).  UN loads of a thread in flight: the row streams through few registers
+            auto take = [&](u32x4 (&u)[UN], int n) {
+                float t = m;
+#pragma unroll
+                for (int x = 0; x < UN; ++x)
+                    if (x < n) t = fmaxf(t, top(u[x]));
+                if (__any(t > m)) {
+                    t = wave_max(t);
+                    rescale(zero_if_none(m) - zero_if_none(t));
+                    m = t;
+                }
+                const float mz = zero_if_none(m);
+                keep_packed(u);
+#pragma unroll
+                for (int x = 0; x < UN; ++x)
+                    if (x < n) sums(u[x], mz);
+            };
+            u32x4 u[UN];
+            int p = tid;
+            for (; p + (UN - 1) * NT < np; p += UN * NT) {
+#pragma unroll
+                for (int x = 0; x < UN; ++x) u[x] = zp[p + x * NT];
+                take(u, UN);
+            }
+            for (; p < np; p += NT) {
+                u[0] = zp[p];
+                take(u, 1);
+            }
+            u[0] = qe;
+            if (e0 < e1) take(u, 1);
+            const float mw = wave_max(m);   // (lanes that left a loop early missed the last rises)
+            rescale(zero_if_none(m) - zero_if_none(mw));
+            m = mw;
         }
         st = wave_sum(st);
         if (MIX) s1 = wave_sum(s1);
@@ -301,130 +371,138 @@ __global__ __launch_bounds__(NT, NV <= 8 ? 8 : 4) void distill_kernel(const Dist
 #pragma unroll
         for (int o = NW / 2; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
         const float dw = mw == -INFINITY ? 0.f : mw - M;
-        float S_t = red[lane % NW][1] * exp2_(dw * ct), S_1 = MIX ? red[lane % NW][2] * exp2_(dw * L2E) : 0.f;
+        float S_t = red[lane % NW][1] * exp2_(dw * soft.ct), S_1 = MIX ? red[lane % NW][2] * exp2_(dw * L2E) : 0.f;
 #pragma unroll
         for (int o = NW / 2; o > 0; o >>= 1) {
             S_t += __shfl_xor(S_t, o, 64);
             if (MIX) S_1 += __shfl_xor(S_1, o, 64);
         }
-        const bool has = tred[2] > 0.f, lab = MIX && label >= 0;
-        const float tm = tred[0], ts = tred[1];
-        const float n_t = (float)max(cnt[0], 1), n_l = (float)max(cnt[1], 1);
-        const float lt = logf(S_t), l1 = MIX ? logf(S_1) : 0.f;   // log sums above the maximum M
-        const float qt = has && ts != 0.f ? 1.f / ts : 0.f;       // (no finite entry: nothing to learn from)
-        const float live = has && ts != 0.f && a.alpha > 0.f ? 1.f : 0.f;
-        const float gt = live * a.alpha * a.tau / n_t * gs, g1 = lab ? a.beta / n_l * gs : 0.f;
-        const float it = 1.f / a.tau;
+        M = uniform(M);
+        S_t = uniform(S_t);
+        S_1 = uniform(S_1);
+        const float ts = uniform(tred[0]);
+        // (no finite entry: nothing to learn from; NaN counts as one)
+        const bool live = uniform(tred[1]) > 0.f && ts != 0.f && a.alpha > 0.f;
+        const int label = MIX ? __builtin_amdgcn_readfirstlane(sidx[a.K]) : -1;
+        const float n_t = uniform((float)max(cnt[0], 1)), n_l = uniform((float)max(cnt[1], 1));
+        const float qt = live ? 1.f / ts : 0.f;
+        const float gt = live ? a.alpha * a.tau / n_t * gs : 0.f, g1 = label >= 0 ? a.beta / n_l * gs : 0.f;
         // ---- loss share: the wave that holds the entries
         if (a.rows != nullptr && w == NW - 1) {
             float kd = 0.f;
-            for (int k = lane; k < a.K && live != 0.f; k += 64) {
-                const int i = sidx[k];
-                if (i < 0 || sq[k] == -INFINITY) continue;
-                const float u = (sq[k] - tm) * it;
-                const float wq = __expf(u) * qt;
-                const float lp = (T::get(z[i]) - M) * it - lt;
-                if (wq != 0.f) kd += wq * ((u - logf(ts)) - lp);   // 0 log 0 = 0
+            if (live) {
+                const float base = logf(S_t) - logf(ts);   // u - log sum e^u - (d / tau - log S_t)
+                for (int k = lane; k < a.K; k += 64) {
+                    const float e = se[k];
+                    if (e != 0.f) kd += e * qt * (su[k] - (sz[k] - M) * it + base);   // 0 log 0 = 0
+                }
+                kd = wave_sum(kd);
             }
-            kd = wave_sum(kd);
             if (lane == 0) {
-                float v = live != 0.f ? a.alpha * a.tau * a.tau * kd / n_t : 0.f;
-                if (lab) v += a.beta / n_l * (l1 - (T::get(z[label]) - M));
+                float v = live ? a.alpha * a.tau * a.tau * kd / n_t : 0.f;
+                if (label >= 0) v += a.beta / n_l * (logf(S_1) - (sz[a.K] - M));
                 a.rows[row] = v;
             }
         }
         if constexpr (GRAD) {
-            // p as 2^((z - M) c - log2 S): the factors 1 / S and the means' weights multiply outside
             const float wt = gt / S_t, w1 = MIX ? g1 / S_1 : 0.f;
-            const bool do_t = gt != 0.f || gt != gt, do_1 = MIX && g1 != 0.f;
-            auto dz = [&](float v) {
-                const float d = v - M;
-                float g = do_t ? wt * exp2_(d * ct) : 0.f;
-                if (MIX && do_1) g += w1 * exp2_(d * L2E);
-                return g;
+            const bool no_t = gt == 0.f, no_1 = g1 == 0.f;   // a row without the term: exactly none of it
+            auto dz = [&](const float (&f)[E], float (&g)[E]) {
+#pragma unroll
+                for (int i = 0; i < E; ++i) {
+                    float t, o;
+                    soft(f[i], M, t, o);
+                    g[i] = no_t ? 0.f : wt * t;
+                    if (MIX) g[i] = no_1 ? g[i] : fmaf(w1, o, g[i]);
+                }
             };
-            // this thread's special columns (entries tid, tid + NT, ...; the label as entry K): read before
-            // the row is overwritten (grad may be the logits)
-            constexpr int NE = (MAX_K + 1 + NT - 1) / NT;
-            float zs[NE];
-#pragma unroll
-            for (int e = 0; e < NE; ++e) {
-                const int k = tid + e * NT;
-                const int i = k < a.K ? sidx[k] : k == a.K ? label : -1;
-                zs[e] = i >= 0 ? T::get(z[i]) : 0.f;
-            }
-            __syncthreads();
             S* g = (S*)a.grad + (int64_t)row * a.gld;
+            u32x4* gp = (u32x4*)(g + a0);   // (the host gives the gradient's rows the logits' alignment)
             auto store = [&](int p, const u32x4& u) {
-                float f[E];
+                float f[E], d[E];
                 T::unpack(u, f);
-#pragma unroll
-                for (int i = 0; i < E; ++i) f[i] = dz(f[i]);
-                *(u32x4*)(g + a0 + (int64_t)p * E) = T::pack(f);   // (the host gives grad rows the logits' alignment)
+                dz(f, d);
+                __builtin_nontemporal_store(T::pack(d), gp + p);
+                __builtin_amdgcn_sched_barrier(0);
             };
             if constexpr (NV > 0) {
 #pragma unroll
-                for (int t = 0; t < NV; ++t) {
+                for (int t = 0; t < NV; ++t)
                     if (tid + t * NT < np) store(tid + t * NT, q[t]);
-                    one_at_a_time();
-                }
             } else {
-                for (int p = tid; p < np; p += NT) store(p, load(p));
+                u32x4 u[UN];
+                int p = tid;
+                for (; p + (UN - 1) * NT < np; p += UN * NT) {
+#pragma unroll
+                    for (int x = 0; x < UN; ++x) u[x] = zp[p + x * NT];
+#pragma unroll
+                    for (int x = 0; x < UN; ++x) store(p + x * NT, u[x]);
+                }
+                for (; p < np; p += NT) store(p, zp[p]);
             }
             if (e0 < e1) {
-                float f[E];
+                float f[E], d[E];
                 T::unpack(qe, f);
+                dz(f, d);
 #pragma unroll
                 for (int i = 0; i < E; ++i)
-                    if (e0 + i < e1) g[e0 + i] = T::put(dz(f[i]));
+                    if (e0 + i < e1) g[e0 + i] = T::put(d[i]);
             }
             for (int j = a.V + tid; j < a.W; j += NT) g[j] = T::put(0.f);
             __syncthreads();   // the special columns are written after the row
-#pragma unroll
-            for (int e = 0; e < NE; ++e) {
-                const int k = tid + e * NT;
-                const int i = k < a.K ? sidx[k] : k == a.K ? label : -1;
-                if (i < 0) continue;
+            for (int k = tid; k <= a.K; k += NT) {
+                const int i = sidx[k];
+                if (i < 0 || (k == a.K && !MIX)) continue;
                 float wq = 0.f;
                 bool first = true;
                 for (int x = 0; x < a.K; ++x) {
                     const bool same = sidx[x] == i;
                     if (same && x < k) first = false;
-                    if (same && sq[x] != -INFINITY) wq += __expf((sq[x] - tm) * it);
+                    if (same) wq += se[x];
                 }
                 if (!first) continue;
-                g[i] = T::put(dz(zs[e]) - gt * (wq * qt) - (i == label ? g1 : 0.f));
+                float f[E], d[E];
+                f[0] = sz[k];
+#pragma unroll
+                for (int y = 1; y < E; ++y) f[y] = 0.f;
+                dz(f, d);
+                g[i] = T::put(d[0] - (no_t ? 0.f : gt * (wq * qt)) - (i == label ? g1 : 0.f));
             }
         }
         __syncthreads();   // the next row's entries and sums replace this one's in LDS
     }
 }
 
-template <class T, int NT, int NV>
-int launch(const DistillArgs& a, hipStream_t s) {
-    const size_t lds = (size_t)a.K * 8;
-    const bool mix = a.beta > 0.f;
+template <class T, int NT, int NV, int MODE>
+int launch_mode(const DistillArgs& a, hipStream_t s) {
+    const size_t lds = (size_t)(a.K + 1) * 16;
     // one workgroup a row; the pass that most often has nothing to do (written) as few as fill the chip
     const int grid = a.written && a.M > 1024 ? 1024 : a.M;
-    if (a.grad != nullptr) {
-        if (mix) distill_kernel<T, NT, NV, true, true><<<grid, NT, lds, s>>>(a);
-        else distill_kernel<T, NT, NV, false, true><<<grid, NT, lds, s>>>(a);
-    } else {
-        if (mix) distill_kernel<T, NT, NV, true, false><<<grid, NT, lds, s>>>(a);
-        else distill_kernel<T, NT, NV, false, false><<<grid, NT, lds, s>>>(a);
-    }
+    if (a.grad != nullptr) distill_kernel<T, NT, NV, MODE, true><<<grid, NT, lds, s>>>(a);
+    else distill_kernel<T, NT, NV, MODE, false><<<grid, NT, lds, s>>>(a);
     return (int)hipGetLastError();
+}
+
+template <class T, int NT, int NV>
+int launch(const DistillArgs& a, hipStream_t s) {
+    if (!(a.beta > 0.f)) return launch_mode<T, NT, NV, -1>(a, s);
+    if (a.tau == 1.f) return launch_mode<T, NT, NV, 1>(a, s);
+    if (a.tau == 2.f) return launch_mode<T, NT, NV, 2>(a, s);
+    if (a.tau == 4.f) return launch_mode<T, NT, NV, 4>(a, s);
+    return launch_mode<T, NT, NV, 0>(a, s);
 }
 
 template <class T>
 int by_length(const DistillArgs& a, hipStream_t s) {
     const int np = a.V / T::E;   // whole pieces, at most
-    if (np <= 256) return launch<T, 256, 1>(a, s);
+    if (np <= 256) return launch<T, 64, 4>(a, s);
     if (np <= 1024) return launch<T, 256, 4>(a, s);
-    if (np <= 4096) return launch<T, 1024, 4>(a, s);
-    if (np <= 8192) return launch<T, 1024, 8>(a, s);
-    if (np <= 16384) return launch<T, 1024, 16>(a, s);
-    return launch<T, 1024, 0>(a, s);
+    // long rows: where there are rows for every CU twice over, workgroups of 4 waves that stream, 5 rows in
+    // flight a CU, mix their loads, sums and stores best (16384 x 50304 bf16: 806 us; 1024 threads with
+    // the row in registers, one row in flight: 1260 us); fewer rows want the whole workgroup on one
+    // row (24 rows: 12.6 against 15.1 us)
+    if (np <= 8192 && a.M < 512) return launch<T, 1024, 8>(a, s);
+    return launch<T, 256, 0>(a, s);
 }
 
 }  // namespace
