@@ -111,11 +111,24 @@ __device__ __forceinline__ short4v tr_read(const bf16_t* p) {
 }
 // operand of 32 columns x 16 rows, columns on the lanes: rows r .. r + 3 and r + 8 .. r + 11 of the
 // lane's half, the order in which an accumulator holds its rows
-template <class T, int DP>
-__device__ __forceinline__ typename T::vec tr_pair(const bf16_t* img, int row, int col) {
-    const short4v a = tr_read(img + elem_at<DP>(row, col)), b = tr_read(img + elem_at<DP>(row + 8, col));
+template <class T>
+__device__ __forceinline__ typename T::vec tr_pair(const bf16_t* lo, const bf16_t* hi) {
+    const short4v a = tr_read(lo), b = tr_read(hi);
     const short8v c = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
     return __builtin_bit_cast(typename T::vec, c);
+}
+template <class T, int DP>
+__device__ __forceinline__ typename T::vec tr_pair(const bf16_t* img, int row, int col) {
+    return tr_pair<T>(img + elem_at<DP>(row, col), img + elem_at<DP>(row + 8, col));
+}
+
+// f(0), f(1), .. f(N - 1) with compile-time indices
+template <int N, int I = 0, class F>
+__device__ __forceinline__ void unrolled(F&& f) {
+    if constexpr (I < N) {
+        f(std::integral_constant<int, I>{});
+        unrolled<N, I + 1>(f);
+    }
 }
 
 // whether one of 8 values is an infinity or NaN (integer test on the exponent field)
@@ -269,10 +282,10 @@ struct Tile {
         }
     }
 };
-// the rows of a flagged tile of 64: bit r set where a chunk of row r was not finite
+// the flagged rows of a tile: bit l set where a chunk of row `row` of lane l was not finite
 template <int DP>
-__device__ __forceinline__ uint64_t flagged_rows(const uint8_t* flags, int lane) {
-    const uint2* p = (const uint2*)(flags + lane * (DP / 8));
+__device__ __forceinline__ uint64_t flagged_rows(const uint8_t* flags, int row) {
+    const uint2* p = (const uint2*)(flags + row * (DP / 8));
     uint32_t any = p[0].x | p[0].y;
     if (DP == 128) any |= p[1].x | p[1].y;
     return __ballot(any != 0);

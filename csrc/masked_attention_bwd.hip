@@ -126,8 +126,9 @@ __global__ __launch_bounds__(64 * NW, DP == 64 ? 8 / NW : 1) void mattn_dq_kerne
                     e = exp2_fast(fmaf(s[i], sc.mul, -lse2));
                 } else if constexpr (CAP) {
                     const float q4 = sc.sat(s[i]);
-                    e = exp2_fast(sc.biased(sc.capped(q4), d0 + (float)kk) - lse2);
-                    x *= fmaf(-4.f * q4, q4, 4.f * q4);   // 1 - tanh^2
+                    if constexpr (ALIBI) e = exp2_fast(sc.biased(sc.capped(q4), d0 + (float)kk) - lse2);
+                    else e = exp2_fast(fmaf(-2.f * sc.capl, q4, sc.capl - lse2));
+                    x *= fmaf(-q4, q4, q4);   // (1 - tanh^2) / 4
                 } else {
                     e = exp2_fast(sc(s[i], d0 + (float)kk) - lse2);
                 }
@@ -157,6 +158,7 @@ __global__ __launch_bounds__(64 * NW, DP == 64 ? 8 / NW : 1) void mattn_dq_kerne
         if (next) sstore(kb + 1, buf ^ 1);
         __syncthreads();
     }
+    const float gscale = CAP ? 4.f * a.scale : a.scale;   // (with the 4 of the cap's derivative)
     if (qi < a.Tq) {
         bf16_t* out = (bf16_t*)a.dq + at.b * a.dqs[0] + at.h * a.dqs[2] + (int64_t)qi * a.dqs[1];
 #pragma unroll
@@ -165,8 +167,8 @@ __global__ __launch_bounds__(64 * NW, DP == 64 ? 8 / NW : 1) void mattn_dq_kerne
             for (int g = 0; g < 4; ++g) {
                 const int d = 32 * i + 8 * g + 4 * h;
                 uint2 u;
-                u.x = T::pack(dq[i][4 * g] * a.scale, dq[i][4 * g + 1] * a.scale);
-                u.y = T::pack(dq[i][4 * g + 2] * a.scale, dq[i][4 * g + 3] * a.scale);
+                u.x = T::pack(dq[i][4 * g] * gscale, dq[i][4 * g + 1] * gscale);
+                u.y = T::pack(dq[i][4 * g + 2] * gscale, dq[i][4 * g + 3] * gscale);
                 if (poison) u.x = u.y = T::NANBITS | T::NANBITS << 16;
                 if (d < a.D) *(uint2*)(out + d) = u;
             }
@@ -175,17 +177,25 @@ __global__ __launch_bounds__(64 * NW, DP == 64 ? 8 / NW : 1) void mattn_dq_kerne
 
 // ============================================================================ dK, dV
 // Workgroup = 128 keys of one KV head (a wave owns 32, key on the lane, K and V fragments resident);
-// walks the 32-query tiles that see the block, head after head of the group, with the next tile's
-// Q / dO rows and row constants loaded into registers during the current one (one barrier per tile).
+// walks the 32-query tiles that see the block, head after head of the group.  One wave's work on tile t
+// is three stages: A(t) the products S and dP, B(t) the 16 scores a lane holds (vector ALU alone), C(t)
+// the products dV and dK.  Run one after the other the matrix unit idles through B and the ALU through A
+// and C, and the registers (accumulators of 2 x DP x 32, fragments of K and V) leave only one or two
+// waves per SIMD to fill in for it.  So the loop is pipelined in the wave: an iteration
+// interleaves C(t - 1), B(t) and A(t + 1), two scores between every few products, each product's LDS
+// fragment read two products ahead.  Four tiles of Q / dO are in LDS (t - 1 .. t + 1, and t + 2
+// arriving), two more in registers on their way there; one barrier per tile.
 template <class T, int DP, bool CAP, bool ALIBI>
 __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void mattn_dkdv_kernel(const Args a) {
-    constexpr int NS = DP / 16, NO = DP / 32;
+    constexpr int NS = DP / 16, NO = DP / 32, RING = 4;
+    constexpr int NA = 2 * NS, NC = 4 * NO, STEPS = 8, AS = NA / STEPS, CS = NC / STEPS, AHEAD = 2;
     typedef Tile<T, DP, QT, 256> TL;
-    __shared__ __attribute__((aligned(16))) bf16_t Qs[2][QT * DP];
-    __shared__ __attribute__((aligned(16))) bf16_t Ds[2][QT * DP];
-    // per query row: lse log2(e), -delta, lo, hi; then the tile's qtab entry
-    __shared__ __attribute__((aligned(16))) uint32_t rowc[2][4 * QT + 4];
-    __shared__ __attribute__((aligned(16))) uint8_t qflag[2][64 * (DP / 8)], dflag[2][64 * (DP / 8)];
+    typedef typename T::vec vec;
+    constexpr int IMG = QT * DP;
+    __shared__ __attribute__((aligned(16))) bf16_t tiles[RING][2 * IMG];   // Q, then dO
+    // per query row: lse log2(e), -delta, lo, hi
+    __shared__ __attribute__((aligned(16))) uint32_t rowc[RING][4 * QT];
+    __shared__ __attribute__((aligned(16))) uint8_t qflag[RING][QT * (DP / 8)], dflag[RING][QT * (DP / 8)];
     const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, r = lane & 31;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int nkv = a.B * a.Hk, G = a.H / a.Hk;
@@ -193,10 +203,9 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void mattn_dkdv_kernel(const
     const int nq = (a.Tq + QT - 1) / QT, nk = (a.Tk + KT - 1) / KT;
     const int k0 = kbi * KT + 32 * w, kj = k0 + r, kc = min(kj, a.Tk - 1);
     const int2 range = a.ktab[(int64_t)b * nk + kbi];
-    const int nt = range.y - range.x, total = nt * G;
-    for (int i = tid; i < 2 * 64 * (DP / 8); i += 256) (&qflag[0][0])[i] = (&dflag[0][0])[i] = 0;   // rows 32 .. 63 stay clear
+    const int total = (range.y - range.x) * G;
 
-    typename T::vec kf[NS], vf[NS];
+    vec kf[NS], vf[NS];
     {
         const bf16_t* krow = (const bf16_t*)a.k + b * a.ks[0] + hk * a.ks[2] + (int64_t)kc * a.ks[1];
         const bf16_t* vrow = (const bf16_t*)a.v + b * a.vs[0] + hk * a.vs[2] + (int64_t)kc * a.vs[1];
@@ -220,78 +229,102 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void mattn_dkdv_kernel(const
     const bf16_t* qbase = (const bf16_t*)a.q + b * a.qs[0] + (int64_t)hk * G * a.qs[2];
     const bf16_t* dbase = (const bf16_t*)a.dout + b * a.dos[0] + (int64_t)hk * G * a.dos[2];
     const int64_t srow = ((int64_t)b * a.H + hk * G) * a.Tq;
-    u32x4 qr[TL::N], dr[TL::N];
-    uint32_t rc;   // this thread's row constant of the staged tile
-    int ng = 0, ntile = range.x;   // the tile that gload takes next: head of the group, query tile
-    auto gload = [&]() {
-        TL::load(qr, qbase + ng * a.qs[2], a.qs[1], ntile * QT, a.Tq - 1, a.D, tid);
-        TL::load(dr, dbase + ng * a.dos[2], a.dos[1], ntile * QT, a.Tq - 1, a.D, tid);
-        const int kind = tid >> 5, q = min(ntile * QT + (tid & 31), a.Tq - 1);
-        const uint32_t* p = kind == 0   ? (const uint32_t*)a.lse + srow + (int64_t)ng * a.Tq + q
-                            : kind == 1 ? (const uint32_t*)a.delta + srow + (int64_t)ng * a.Tq + q
-                            : kind == 2 ? (const uint32_t*)a.lo + (int64_t)b * a.Tq + q
-                            : kind == 3 ? (const uint32_t*)a.hi + (int64_t)b * a.Tq + q
-                                        : (const uint32_t*)(a.qtab + (int64_t)b * nq + ntile) + (tid & 3);
-        rc = *p;
+    // a place in the walk: head of the group and query tile
+    struct At {
+        int g, t;
     };
-    int cg = 0, ct = range.x;   // the tile in registers, then in LDS
-    auto sstore = [&](int buf) {
-        const int4 e = a.qtab[(int64_t)b * nq + ct];
-        const bool whole = e.z <= kbi * KT && e.w >= (kbi + 1) * KT;
-        if (whole && a.D == DP) {
-            TL::put(Qs[buf], qr, tid);
-            TL::put(Ds[buf], dr, tid);
+    auto advance = [&](At& x) {
+        if (++x.t == range.y) {
+            x.t = range.x;
+            ++x.g;
+        }
+    };
+    // a tile on its way: this thread's pieces of Q and dO, its row constant (threads 0 .. 127: one of the
+    // four kinds of one row) and its word of the tile's qtab entry
+    struct Coming {
+        u32x4 q[TL::N], d[TL::N];
+        uint32_t rc, tab;
+    };
+    const int kind = (tid >> 5) & 3, rrow = tid & 31;
+    const uint32_t* rbase = kind == 0   ? (const uint32_t*)a.lse + srow
+                            : kind == 1 ? (const uint32_t*)a.delta + srow
+                            : kind == 2 ? (const uint32_t*)a.lo + (int64_t)b * a.Tq
+                                        : (const uint32_t*)a.hi + (int64_t)b * a.Tq;
+    const int64_t rhead = kind < 2 ? a.Tq : 0;
+    const uint32_t* tbase = (const uint32_t*)(a.qtab + (int64_t)b * nq) + (tid & 3);
+    auto gload = [&](const At& x, Coming& c) __attribute__((always_inline)) {
+        TL::load(c.q, qbase + x.g * a.qs[2], a.qs[1], x.t * QT, a.Tq - 1, a.D, tid);
+        TL::load(c.d, dbase + x.g * a.dos[2], a.dos[1], x.t * QT, a.Tq - 1, a.D, tid);
+        c.rc = rbase[x.g * rhead + min(x.t * QT + rrow, a.Tq - 1)];
+        c.tab = tbase[4 * x.t];
+    };
+    // the qtab entry of a tile, in scalar registers (lanes 0 .. 3 hold its words)
+    struct Bounds {
+        int lo, hi, full_lo, full_hi;   // some row sees [lo, hi), every row sees [full_lo, full_hi)
+    };
+    auto sstore = [&](const At& x, const Coming& c, int buf) __attribute__((always_inline)) {
+        const Bounds e{__builtin_amdgcn_readlane((int)c.tab, 0), __builtin_amdgcn_readlane((int)c.tab, 1),
+                       __builtin_amdgcn_readlane((int)c.tab, 2), __builtin_amdgcn_readlane((int)c.tab, 3)};
+        if (e.full_lo <= kbi * KT && e.full_hi >= (kbi + 1) * KT && a.D == DP) {   // every key of the block is seen by every row
+            TL::put(tiles[buf], c.q, tid);
+            TL::put(tiles[buf] + IMG, c.d, tid);
         } else {
-            TL::put_masked(Qs[buf], qr, tid, 0, a.Tq - ct * QT, a.D, qflag[buf]);   // (as K in dQ)
-            TL::put_masked(Ds[buf], dr, tid, 0, a.Tq - ct * QT, a.D, dflag[buf]);
+            TL::put_masked(tiles[buf], c.q, tid, 0, a.Tq - x.t * QT, a.D, qflag[buf]);   // (as K in dQ)
+            TL::put_masked(tiles[buf] + IMG, c.d, tid, 0, a.Tq - x.t * QT, a.D, dflag[buf]);
         }
-        const int kind = tid >> 5;
-        uint32_t v = rc;
-        if (kind == 0) v = __float_as_uint(__uint_as_float(rc) * LOG2E);
-        if (kind == 1) v = __float_as_uint(-__uint_as_float(rc));
-        if ((kind == 2 || kind == 3) && ct * QT + (tid & 31) >= a.Tq) v = 0;   // no such query: sees nothing
-        if (tid < 4 * QT + 4) rowc[buf][tid] = v;
+        uint32_t v = c.rc;
+        if (kind == 0) v = __float_as_uint(__uint_as_float(v) * LOG2E);
+        if (kind == 1) v ^= 0x80000000u;
+        if (kind >= 2 && x.t * QT + rrow >= a.Tq) v = 0;   // no such query: sees nothing
+        if (tid < 4 * QT) rowc[buf][tid] = v;
+        return e;
     };
-    auto compute = [&](int qt, int buf) {
+    auto active = [&](const Bounds& e) { return e.lo < k0 + 32 && e.hi > k0; };   // some row sees a key of the wave
+
+    // where the lane's fragments stand in a tile's image: chunks 2 d + h of its row; rows 4 h + tq (and
+    // 8 further) of the columns 32 i + tcol (16 rows on, a chunk's place in its row is the same)
+    int rowat[NS], colat[NO][2];
+#pragma unroll
+    for (int d = 0; d < NS; ++d) rowat[d] = chunk_at<DP>(r, 2 * d + h);
+#pragma unroll
+    for (int i = 0; i < NO; ++i) {
+        colat[i][0] = elem_at<DP>(4 * h + tq, 32 * i + tcol);
+        colat[i][1] = elem_at<DP>(4 * h + tq + 8, 32 * i + tcol);
+    }
+    struct Scores {
+        f32x16 s, p;          // S, then P; dP - delta, then dX
+    };
+    vec pb[2], db[2];         // tile t - 1: P and dX, rounded
+    float d0;
+    auto init_b = [&](const At& x) {
+        if (ALIBI) {
+            sc.slope = a.slopes[hk * G + x.g] * LOG2E;
+            d0 = (float)(x.t * QT + 4 * h) - kpos;
+        }
+    };
+    auto score = [&](Scores& y, auto xc, float ls) __attribute__((always_inline)) {
+        constexpr int i = decltype(xc)::value, qq = (i & 3) + 8 * (i >> 2);
+        float e, x = y.p[i];
+        if constexpr (Score<CAP, ALIBI>::PLAIN) {
+            e = exp2_fast(fmaf(y.s[i], sc.mul, -ls));
+        } else if constexpr (CAP) {
+            const float q4 = sc.sat(y.s[i]);
+            if constexpr (ALIBI) e = exp2_fast(sc.biased(sc.capped(q4), d0 + (float)qq) - ls);
+            else e = exp2_fast(fmaf(-2.f * sc.capl, q4, sc.capl - ls));
+            x *= fmaf(-q4, q4, q4);
+        } else {
+            e = exp2_fast(sc(y.s[i], d0 + (float)qq) - ls);
+        }
+        x *= e;
+        asm volatile("" : "+v"(e), "+v"(x));   // here, between the products, and not sunk behind them
+        y.s[i] = e;
+        y.p[i] = x;
+    };
+    // masks of tile t, and the operands of C(t)
+    auto finish_b = [&](const At& x, const Bounds& bnd, Scores& y, int buf) __attribute__((always_inline)) {
+        f32x16 &s = y.s, &p = y.p;
+        const bool part = bnd.full_lo > k0 || bnd.full_hi < k0 + 32;
         const uint32_t* rw = rowc[buf];
-        const int el = __builtin_amdgcn_readfirstlane((int)rw[4 * QT]), eh = __builtin_amdgcn_readfirstlane((int)rw[4 * QT + 1]);
-        const int efl = __builtin_amdgcn_readfirstlane((int)rw[4 * QT + 2]), efh = __builtin_amdgcn_readfirstlane((int)rw[4 * QT + 3]);
-        if (el >= k0 + 32 || eh <= k0) return;
-        const bool part = efl > k0 || efh < k0 + 32;
-        const bf16_t* Q_ = Qs[buf];
-        const bf16_t* D_ = Ds[buf];
-        f32x16 s = {}, p;
-        float ls[16];
-#pragma unroll
-        for (int g4 = 0; g4 < 4; ++g4) {
-            const float4 c = *(const float4*)((const float*)rw + QT + 8 * g4 + 4 * h);
-            const float4 e = *(const float4*)((const float*)rw + 8 * g4 + 4 * h);
-            p[4 * g4] = c.x, p[4 * g4 + 1] = c.y, p[4 * g4 + 2] = c.z, p[4 * g4 + 3] = c.w;
-            ls[4 * g4] = e.x, ls[4 * g4 + 1] = e.y, ls[4 * g4 + 2] = e.z, ls[4 * g4 + 3] = e.w;
-        }
-#pragma unroll
-        for (int d = 0; d < NS; ++d) {
-            const int at_ = chunk_at<DP>(r, 2 * d + h);
-            s = T::mfma(as_vec<T>(*(const u32x4*)(Q_ + at_)), kf[d], s);
-            p = T::mfma(as_vec<T>(*(const u32x4*)(D_ + at_)), vf[d], p);
-        }
-        const float d0 = ALIBI ? (float)(qt * QT + 4 * h) - kpos : 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int qq = (i & 3) + 8 * (i >> 2);
-            float e, x = p[i];
-            if constexpr (Score<CAP, ALIBI>::PLAIN) {
-                e = exp2_fast(fmaf(s[i], sc.mul, -ls[i]));
-            } else if constexpr (CAP) {
-                const float q4 = sc.sat(s[i]);
-                e = exp2_fast(sc.biased(sc.capped(q4), d0 + (float)qq) - ls[i]);
-                x *= fmaf(-4.f * q4, q4, 4.f * q4);
-            } else {
-                e = exp2_fast(sc(s[i], d0 + (float)qq) - ls[i]);
-            }
-            s[i] = e;
-            p[i] = e * x;
-        }
         if (part) {
 #pragma unroll
             for (int g4 = 0; g4 < 4; ++g4) {
@@ -307,57 +340,136 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void mattn_dkdv_kernel(const
             }
         }
         if (part || a.D != DP) {   // a query that is not finite: NaN for the keys it sees
-            uint64_t bad = flagged_rows<DP>(qflag[buf], lane);
+            uint32_t bad = (uint32_t)flagged_rows<DP>(qflag[buf], r);
             while (bad != 0) {
-                const int q = __builtin_ctzll(bad);
+                const int q = __builtin_ctz(bad);
                 bad &= bad - 1;
                 poison |= kj >= (int)rw[2 * QT + q] && kj < (int)rw[3 * QT + q];
             }
-            bad = flagged_rows<DP>(dflag[buf], lane);   // dO: dP, so dK, is NaN by itself
+            bad = (uint32_t)flagged_rows<DP>(dflag[buf], r);   // dO: dP, so dK, is NaN by itself
             while (bad != 0) {
-                const int q = __builtin_ctzll(bad);
+                const int q = __builtin_ctz(bad);
                 bad &= bad - 1;
-                add_not_finite<T>(dv, dbase + cg * a.dos[2] + (int64_t)(qt * QT + q) * a.dos[1], a.D, h,
+                add_not_finite<T>(dv, dbase + x.g * a.dos[2] + (int64_t)(x.t * QT + q) * a.dos[1], a.D, h,
                                   kj >= (int)rw[2 * QT + q] && kj < (int)rw[3 * QT + q]);
             }
         }
 #pragma unroll
-        for (int s2 = 0; s2 < 2; ++s2) {
-            const typename T::vec pb = round8<T>(s, s2), db = round8<T>(p, s2);
-            const int row = 16 * s2 + 4 * h + tq;
+        for (int s2 = 0; s2 < 2; ++s2) pb[s2] = round8<T>(s, s2), db[s2] = round8<T>(p, s2);
+    };
+    // one iteration: C of the tile in LDS slot bc, B of tile x (bounds bnd, scores y) in slot bb, A of slot ba
+    // (scores yn), as far as they are wanted
+    auto run = [&](auto cc, auto bc_, auto ac, const At& x, const Bounds& bnd, Scores& y, Scores& yn, int bc, int bb,
+                   int ba) __attribute__((always_inline)) {
+        constexpr bool C = decltype(cc)::value, B = decltype(bc_)::value, A = decltype(ac)::value;
+        vec fa[NA], fc[NC];
+        auto load_a = [&](auto ic) {
+            constexpr int i = decltype(ic)::value;
+            if constexpr (i < NA) fa[i] = as_vec<T>(*(const u32x4*)(tiles[ba] + rowat[i / 2] + (i & 1 ? IMG : 0)));
+        };
+        auto load_c = [&](auto ic) {
+            constexpr int i = decltype(ic)::value;
+            if constexpr (i < NC)
+                fc[i] = tr_pair<T>(tiles[bc] + colat[i / 2 % NO][0] + (i & 1 ? 0 : IMG) + 16 * DP * (i / (2 * NO)),
+                                   tiles[bc] + colat[i / 2 % NO][1] + (i & 1 ? 0 : IMG) + 16 * DP * (i / (2 * NO)));
+        };
+        if constexpr (A) {
+            yn.s = (f32x16){};
 #pragma unroll
-            for (int i = 0; i < NO; ++i) {
-                dv[i] = T::mfma(tr_pair<T, DP>(D_, row, 32 * i + tcol), pb, dv[i]);
-                dk[i] = T::mfma(tr_pair<T, DP>(Q_, row, 32 * i + tcol), db, dk[i]);
+            for (int g4 = 0; g4 < 4; ++g4) {
+                const float4 c = *(const float4*)((const float*)rowc[ba] + QT + 8 * g4 + 4 * h);
+                yn.p[4 * g4] = c.x, yn.p[4 * g4 + 1] = c.y, yn.p[4 * g4 + 2] = c.z, yn.p[4 * g4 + 3] = c.w;
             }
+            unrolled<AHEAD>(load_a);
+        }
+        if constexpr (C) unrolled<AHEAD>(load_c);
+        if constexpr (B) init_b(x);
+        unrolled<STEPS>([&](auto sc_) {
+            constexpr int st = decltype(sc_)::value;
+            const float2 ls = *(const float2*)((const float*)rowc[bb] + (2 * st & 3) + 8 * (st >> 1) + 4 * h);
+            if constexpr (C)
+                unrolled<CS>([&](auto k) {
+                    constexpr int i = st * CS + decltype(k)::value, s2 = i / (2 * NO), o = i / 2 % NO;
+                    load_c(std::integral_constant<int, i + AHEAD>{});
+                    if constexpr (i & 1) dk[o] = T::mfma(fc[i], db[s2], dk[o]);
+                    else dv[o] = T::mfma(fc[i], pb[s2], dv[o]);
+                });
+            if constexpr (A)
+                unrolled<AS>([&](auto k) {
+                    constexpr int i = st * AS + decltype(k)::value;
+                    load_a(std::integral_constant<int, i + AHEAD>{});
+                    if constexpr (i & 1) yn.p = T::mfma(fa[i], vf[i / 2], yn.p);
+                    else yn.s = T::mfma(fa[i], kf[i / 2], yn.s);
+                });
+            if constexpr (B) {   // scores 2 st, 2 st + 1: neighbouring rows
+                score(y, std::integral_constant<int, 2 * st>{}, ls.x);
+                score(y, std::integral_constant<int, 2 * st + 1>{}, ls.y);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        if constexpr (B) finish_b(x, bnd, y, bb);
+    };
+    constexpr std::true_type Y{};
+    constexpr std::false_type N{};
+
+    At ld{0, range.x}, st{0, range.x}, cur{0, range.x};
+    Coming c0, c1;
+    Scores y0, y1;
+    Bounds e0{0, 0, 0, 0}, e1{0, 0, 0, 0}, e2{0, 0, 0, 0};   // of tiles t, t + 1, t + 2
+    bool acc_ = false;   // tile t - 1 has work for this wave
+#pragma unroll
+    for (int i = 0; i < 2; ++i) pb[i] = db[i] = as_vec<T>((u32x4)(0u));
+    auto load_next = [&](Coming& c) __attribute__((always_inline)) {
+        if (ld.g < G) {
+            gload(ld, c);
+            advance(ld);
         }
     };
-    auto advance = [&](int& g, int& t) {
-        if (++t == range.y) {
-            t = range.x;
-            ++g;
+    auto store_next = [&](const Coming& c, int buf) __attribute__((always_inline)) {
+        Bounds e{0, 0, 0, 0};   // past the last tile: no work
+        if (st.g < G) {
+            e = sstore(st, c, buf);
+            advance(st);
         }
+        return e;
     };
-    __syncthreads();   // the flags are clear
     if (total > 0) {
-        gload();
-        advance(ng, ntile);
-        sstore(0);
+        // slot 3 stands for tile -1: finite values for the weights 0 of the first C
+        for (int i = tid; i < 2 * IMG / 8; i += 256) ((u32x4*)tiles[3])[i] = (u32x4)(0u);
+        load_next(c0);
+        load_next(c1);
+        e0 = store_next(c0, 0);
+        e1 = store_next(c1, 1);
+        load_next(c0);
+        load_next(c1);
         __syncthreads();
+        run(N, N, Y, cur, e0, y1, y0, 0, 0, 0);
     }
-    for (int it = 0; it < total; ++it) {
-        const int buf = it & 1;
-        const bool next = it + 1 < total;
-        if (next) gload();
-        if (ALIBI) sc.slope = a.slopes[hk * G + cg] * LOG2E;
-        compute(ct, buf);
-        advance(cg, ct);
-        if (next) {
-            advance(ng, ntile);
-            sstore(buf ^ 1);
+    // tile t: its scores in y, the next tile's in yn; tile t + 2 arrives from c, tile t + 4 is asked for
+    auto iter = [&](int t, Coming& c, Scores& y, Scores& yn) __attribute__((always_inline)) {
+        e2 = store_next(c, (t + 2) & 3);
+        load_next(c);
+        const bool act = active(e0);
+        // a tile without work inside the pipeline counts with weights 0 (its masks leave nothing); the
+        // products of a tile past the last are not used
+        if (acc_ || act || active(e1)) {
+            run(Y, Y, Y, cur, e0, y, yn, (t - 1) & 3, t & 3, (t + 1) & 3);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) pb[i] = db[i] = as_vec<T>((u32x4)(0u));
         }
+        acc_ = act;
+        e0 = e1;
+        e1 = e2;
+        advance(cur);
         __syncthreads();
+    };
+    for (int t = 0; t < total; t += 2) {
+        iter(t, c0, y0, y1);
+        if (t + 1 < total) iter(t + 1, c1, y1, y0);
     }
+    if (total > 0) run(Y, N, N, cur, e0, y0, y1, (total - 1) & 3, 0, 0);
+    const float gscale = CAP ? 4.f * a.scale : a.scale;
     if (kj < a.Tk) {
         bf16_t* dkr = (bf16_t*)a.dk + b * a.dks[0] + hk * a.dks[2] + (int64_t)kj * a.dks[1];
         bf16_t* dvr = (bf16_t*)a.dv + b * a.dvs[0] + hk * a.dvs[2] + (int64_t)kj * a.dvs[1];
@@ -367,8 +479,8 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void mattn_dkdv_kernel(const
             for (int g = 0; g < 4; ++g) {
                 const int d = 32 * i + 8 * g + 4 * h;
                 uint2 u, v;
-                u.x = T::pack(dk[i][4 * g] * a.scale, dk[i][4 * g + 1] * a.scale);
-                u.y = T::pack(dk[i][4 * g + 2] * a.scale, dk[i][4 * g + 3] * a.scale);
+                u.x = T::pack(dk[i][4 * g] * gscale, dk[i][4 * g + 1] * gscale);
+                u.y = T::pack(dk[i][4 * g + 2] * gscale, dk[i][4 * g + 3] * gscale);
                 v.x = T::pack(dv[i][4 * g], dv[i][4 * g + 1]);
                 v.y = T::pack(dv[i][4 * g + 2], dv[i][4 * g + 3]);
                 if (poison) u.x = u.y = v.x = v.y = T::NANBITS | T::NANBITS << 16;
