@@ -47,6 +47,9 @@ struct Bf16 {
     static __device__ __forceinline__ f32x16 mfma(vec a, vec b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
     }
+    static __device__ __forceinline__ void mfma_acc(f32x16& c, vec a, vec b) {
+        asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+    }
     static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack2(a, b); }
     static __device__ __forceinline__ void unpack(uint32_t w, float& a, float& b) {
         a = __uint_as_float(w << 16);
@@ -58,6 +61,9 @@ struct F16 {
     static constexpr uint32_t INF = 0x7c00, NANBITS = 0x7e00;
     static __device__ __forceinline__ f32x16 mfma(vec a, vec b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ void mfma_acc(f32x16& c, vec a, vec b) {
+        asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
     }
     static __device__ __forceinline__ uint32_t pack(float a, float b) {   // round to nearest even
         typedef _Float16 h2 __attribute__((ext_vector_type(2)));
@@ -71,6 +77,18 @@ struct F16 {
         b = (float)r[1];
     }
 };
+
+// T::mfma_acc: c += a b with c in accumulation registers (AGPRs), for sums that only products touch: the
+// 256 ordinary registers stay free for the scores.  In asm, because the compiler gives a whole kernel's
+// products one form.  The wait states in front cover an operand that the vector ALU has just written.
+// Nothing but mfma_acc may read such a sum until acc_done has run (a product takes 16 passes at most).
+template <int N>
+__device__ __forceinline__ void acc_done(f32x16 (&x)[N], f32x16 (&y)[N]) {
+    asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+a"(x[i]), "+a"(y[i]));
+    __builtin_amdgcn_sched_barrier(0);
+}
 
 template <class T>
 __device__ __forceinline__ typename T::vec as_vec(u32x4 u) {
@@ -152,27 +170,40 @@ __device__ __forceinline__ u32x4 finite_only(u32x4 u) {
     }
     return u;
 }
-// The values that finite_only left out of a row (`row`: where it stands in memory), added to the lane's
-// accumulator where it sees the row: what a product with a weight > 0 makes of an infinity or NaN.
-template <class T, int NO>
-__device__ __forceinline__ void add_not_finite(f32x16 (&o)[NO], const bf16_t* row, int D, int h, bool see) {
+// The values that finite_only left out of the rows a lane sees: what a product with weights > 0 makes of
+// infinities and NaN, as one bit per accumulator element (4 registers, touched hardly ever).
+struct NotFinite {
+    uint64_t up = 0, down = 0;   // + infinity, - infinity; NaN is both
+    // row: where it stands in memory
+    template <class T, int NO>
+    __device__ __forceinline__ void note(const bf16_t* row, int D, int h, bool see) {
 #pragma unroll
-    for (int i = 0; i < NO; ++i)
+        for (int i = 0; i < NO; ++i)
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const int d = 32 * i + 8 * g + 4 * h;
-            const uint2 u = *(const uint2*)(row + (d < D ? d : 0));
-            const uint32_t w[2] = {u.x, u.y};
+            for (int g = 0; g < 4; ++g) {
+                const int d = 32 * i + 8 * g + 4 * h;
+                const uint2 u = *(const uint2*)(row + (d < D ? d : 0));
+                const uint32_t w[2] = {u.x, u.y};
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const uint32_t x = (w[k >> 1] >> (16 * (k & 1))) & 0xffffu;
-                float lo, hi;
-                T::unpack(x, lo, hi);
-                if (see && d < D && (x & 0x7fffu) >= T::INF) o[i][4 * g + k] += lo;
+                for (int k = 0; k < 4; ++k) {
+                    const uint32_t x = (w[k >> 1] >> (16 * (k & 1))) & 0xffffu;
+                    const bool bad = see && d < D && (x & 0x7fffu) >= T::INF, inf = (x & 0x7fffu) == T::INF;
+                    const uint64_t bit = 1ull << (16 * i + 4 * g + k);
+                    if (bad && !(inf && (x & 0x8000u))) up |= bit;
+                    if (bad && !(inf && !(x & 0x8000u))) down |= bit;
+                }
+                __builtin_amdgcn_sched_barrier(0);   // one load at a time: no registers for more
             }
-            __builtin_amdgcn_sched_barrier(0);   // hardly ever run: one load at a time, no registers for more
-        }
-}
+    }
+    __device__ __forceinline__ bool any() const { return (up | down) != 0; }
+    // element e (a constant) of the finished sums
+    __device__ __forceinline__ float operator()(float v, int e) const {
+        const bool u = (up >> e) & 1, d = (down >> e) & 1;
+        float nan = __uint_as_float(0x7fc00000u);
+        asm volatile("" : "+v"(nan));   // (opaque: these files are compiled as if no value were NaN)
+        return u && d ? nan : u ? INFINITY : d ? -INFINITY : v;
+    }
+};
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float max3(float a, float b, float c) { return __builtin_fmaxf(a, __builtin_fmaxf(b, c)); }

@@ -54,7 +54,14 @@ __global__ __launch_bounds__(64 * NW, DP == 64 ? 8 / NW : 1) void mattn_dq_kerne
         }
     }
     delta += __shfl_xor(delta, 32, 64);
-    if (h == 0 && qi < a.Tq) a.delta[stat] = delta;
+    {   // for dK / dV: planes of lse log2(e) and -delta, zeros behind the last row of a head
+        const int tp = (a.Tq + QT - 1) / QT * QT;
+        float* st = a.delta + ((int64_t)at.b * a.H + at.h) * 2 * tp;
+        if (h == 0 && qi < tp) {
+            st[qi] = qi < a.Tq ? lse2 : 0.f;
+            st[tp + qi] = qi < a.Tq ? -delta : 0.f;
+        }
+    }
     Score<CAP, ALIBI> sc;
     sc.init(a.scale, a.cap, ALIBI ? a.slopes[at.h] : 0.f);
     const float qpos = ALIBI ? (float)(a.pos[at.b] + qi) : 0.f;
@@ -221,6 +228,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void mattn_dkdv_kernel(const
 #pragma unroll
     for (int i = 0; i < NO; ++i) dk[i] = dv[i] = (f32x16){};
     bool poison = false;
+    NotFinite odd;
     const int tq = (lane & 15) >> 2, tcol = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
     Score<CAP, ALIBI> sc;
     sc.init(a.scale, a.cap, 0.f);
@@ -228,7 +236,6 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void mattn_dkdv_kernel(const
 
     const bf16_t* qbase = (const bf16_t*)a.q + b * a.qs[0] + (int64_t)hk * G * a.qs[2];
     const bf16_t* dbase = (const bf16_t*)a.dout + b * a.dos[0] + (int64_t)hk * G * a.dos[2];
-    const int64_t srow = ((int64_t)b * a.H + hk * G) * a.Tq;
     // a place in the walk: head of the group and query tile
     struct At {
         int g, t;
@@ -245,17 +252,35 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void mattn_dkdv_kernel(const
         u32x4 q[TL::N], d[TL::N];
         uint32_t rc, tab;
     };
-    const int kind = (tid >> 5) & 3, rrow = tid & 31;
-    const uint32_t* rbase = kind == 0   ? (const uint32_t*)a.lse + srow
-                            : kind == 1 ? (const uint32_t*)a.delta + srow
-                            : kind == 2 ? (const uint32_t*)a.lo + (int64_t)b * a.Tq
-                                        : (const uint32_t*)a.hi + (int64_t)b * a.Tq;
-    const int64_t rhead = kind < 2 ? a.Tq : 0;
+    const int kind = (tid >> 5) & 3, rrow = tid & 31, tp = nq * QT;
+    const uint32_t* rbase = kind < 2 ? (const uint32_t*)a.delta + (((int64_t)b * a.H + hk * G) * 2 + kind) * tp
+                                     : (const uint32_t*)(kind == 2 ? a.lo : a.hi) + (int64_t)b * a.Tq;
+    const int64_t rhead = kind < 2 ? 2 * tp : 0;
+    const int rlast = kind < 2 ? tp - 1 : a.Tq - 1;
     const uint32_t* tbase = (const uint32_t*)(a.qtab + (int64_t)b * nq) + (tid & 3);
+    // a tile's rows through a buffer resource that starts at its first row: the lane's offsets never change,
+    // and rows past the tensor (and columns past D, offset 2^31) read as zeros
+    uint32_t qoff[TL::N], doff[TL::N];
+#pragma unroll
+    for (int i = 0; i < TL::N; ++i) {
+        const bool in = TL::chunk(tid) * 8 < a.D;
+        qoff[i] = in ? (uint32_t)(TL::row(tid, i) * a.qs[1] + TL::chunk(tid) * 8) * 2u : 0x80000000u;
+        doff[i] = in ? (uint32_t)(TL::row(tid, i) * a.dos[1] + TL::chunk(tid) * 8) * 2u : 0x80000000u;
+    }
+    auto rows_of = [&](const bf16_t* base, int64_t ld, int t) __attribute__((always_inline)) {
+        const int left = a.Tq - t * QT;
+        const uint32_t n = left >= QT ? 0x7fffffffu : (uint32_t)((left - 1) * ld + a.D) * 2u;
+        return __builtin_amdgcn_make_buffer_rsrc((void*)(base + (int64_t)t * QT * ld), 0, n, 0x00020000);
+    };
     auto gload = [&](const At& x, Coming& c) __attribute__((always_inline)) {
-        TL::load(c.q, qbase + x.g * a.qs[2], a.qs[1], x.t * QT, a.Tq - 1, a.D, tid);
-        TL::load(c.d, dbase + x.g * a.dos[2], a.dos[1], x.t * QT, a.Tq - 1, a.D, tid);
-        c.rc = rbase[x.g * rhead + min(x.t * QT + rrow, a.Tq - 1)];
+        const __amdgpu_buffer_rsrc_t qb = rows_of(qbase + x.g * a.qs[2], a.qs[1], x.t);
+        const __amdgpu_buffer_rsrc_t db_ = rows_of(dbase + x.g * a.dos[2], a.dos[1], x.t);
+#pragma unroll
+        for (int i = 0; i < TL::N; ++i) {
+            c.q[i] = __builtin_amdgcn_raw_buffer_load_b128(qb, qoff[i], 0, 0);
+            c.d[i] = __builtin_amdgcn_raw_buffer_load_b128(db_, doff[i], 0, 0);
+        }
+        c.rc = rbase[x.g * rhead + min(x.t * QT + rrow, rlast)];
         c.tab = tbase[4 * x.t];
     };
     // the qtab entry of a tile, in scalar registers (lanes 0 .. 3 hold its words)
@@ -272,11 +297,8 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void mattn_dkdv_kernel(const
             TL::put_masked(tiles[buf], c.q, tid, 0, a.Tq - x.t * QT, a.D, qflag[buf]);   // (as K in dQ)
             TL::put_masked(tiles[buf] + IMG, c.d, tid, 0, a.Tq - x.t * QT, a.D, dflag[buf]);
         }
-        uint32_t v = c.rc;
-        if (kind == 0) v = __float_as_uint(__uint_as_float(v) * LOG2E);
-        if (kind == 1) v ^= 0x80000000u;
-        if (kind >= 2 && x.t * QT + rrow >= a.Tq) v = 0;   // no such query: sees nothing
-        if (tid < 4 * QT) rowc[buf][tid] = v;
+        // (a row past the last sees nothing)
+        if (tid < 4 * QT) rowc[buf][tid] = kind >= 2 && x.t * QT + rrow >= a.Tq ? 0 : c.rc;
         return e;
     };
     auto active = [&](const Bounds& e) { return e.lo < k0 + 32 && e.hi > k0; };   // some row sees a key of the wave
@@ -350,12 +372,17 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void mattn_dkdv_kernel(const
             while (bad != 0) {
                 const int q = __builtin_ctz(bad);
                 bad &= bad - 1;
-                add_not_finite<T>(dv, dbase + x.g * a.dos[2] + (int64_t)(x.t * QT + q) * a.dos[1], a.D, h,
-                                  kj >= (int)rw[2 * QT + q] && kj < (int)rw[3 * QT + q]);
+                odd.note<T, NO>(dbase + x.g * a.dos[2] + (int64_t)(x.t * QT + q) * a.dos[1], a.D, h,
+                                kj >= (int)rw[2 * QT + q] && kj < (int)rw[3 * QT + q]);
             }
         }
 #pragma unroll
         for (int s2 = 0; s2 < 2; ++s2) pb[s2] = round8<T>(s, s2), db[s2] = round8<T>(p, s2);
+    };
+    // (DP 128: one wave per SIMD, sums in AGPRs; DP 64: two, all in ordinary registers)
+    auto mul_acc = [&](f32x16& c, const vec& x, const vec& y) __attribute__((always_inline)) {
+        if constexpr (DP == 128) T::mfma_acc(c, x, y);
+        else c = T::mfma(x, y, c);
     };
     // one iteration: C of the tile in LDS slot bc, B of tile x (bounds bnd, scores y) in slot bb, A of slot ba
     // (scores yn), as far as they are wanted
@@ -391,8 +418,8 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void mattn_dkdv_kernel(const
                 unrolled<CS>([&](auto k) {
                     constexpr int i = st * CS + decltype(k)::value, s2 = i / (2 * NO), o = i / 2 % NO;
                     load_c(std::integral_constant<int, i + AHEAD>{});
-                    if constexpr (i & 1) dk[o] = T::mfma(fc[i], db[s2], dk[o]);
-                    else dv[o] = T::mfma(fc[i], pb[s2], dv[o]);
+                    if constexpr (i & 1) mul_acc(dk[o], fc[i], db[s2]);
+                    else mul_acc(dv[o], fc[i], pb[s2]);
                 });
             if constexpr (A)
                 unrolled<AS>([&](auto k) {
@@ -469,10 +496,17 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void mattn_dkdv_kernel(const
         if (t + 1 < total) iter(t + 1, c1, y1, y0);
     }
     if (total > 0) run(Y, N, N, cur, e0, y0, y1, (total - 1) & 3, 0, 0);
+    if constexpr (DP == 128) acc_done(dk, dv);
     const float gscale = CAP ? 4.f * a.scale : a.scale;
     if (kj < a.Tk) {
         bf16_t* dkr = (bf16_t*)a.dk + b * a.dks[0] + hk * a.dks[2] + (int64_t)kj * a.dks[1];
         bf16_t* dvr = (bf16_t*)a.dv + b * a.dvs[0] + hk * a.dvs[2] + (int64_t)kj * a.dvs[1];
+        if (odd.any()) {
+#pragma unroll
+            for (int i = 0; i < NO; ++i)
+#pragma unroll
+                for (int k = 0; k < 16; ++k) dv[i][k] = odd(dv[i][k], 16 * i + k);
+        }
 #pragma unroll
         for (int i = 0; i < NO; ++i)
 #pragma unroll

@@ -157,13 +157,13 @@ TDL_API int tdl_attn_mask(const void* documents, int wide, const int* prefix_row
 }
 
 // ============================================================================ many queries
-// Workgroup = 32 NW queries of one head (a wave owns 32, query on the lane); keys in tiles of 64,
+// Workgroup = 128 queries of one head (a wave owns 32, query on the lane); keys in tiles of 64,
 // double-buffered in LDS with the next tile's loads in registers.  S^T = K Q^T leaves 16 keys of a
 // 32-key tile on each lane, so a row's maximum and sum are lane-local (the two halves of the wave
 // exchange their maximum), and the rounded S^T accumulator IS the B operand of O^T += V^T P^T.
-template <class T, int DP, bool CAP, bool ALIBI, int NW>
-__global__ __launch_bounds__(64 * NW) void mattn_fwd_kernel(const Args a) {
-    constexpr int BM = QT * NW, BN = 64, NS = DP / 16, NO = DP / 32, NTHR = 64 * NW;
+template <class T, int DP, bool CAP, bool ALIBI>
+__global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void mattn_fwd_kernel(const Args a) {
+    constexpr int NW = 4, BM = QT * NW, BN = 64, NS = DP / 16, NO = DP / 32, NTHR = 64 * NW;
     typedef Tile<T, DP, BN, NTHR> TL;
     __shared__ __attribute__((aligned(16))) bf16_t Ks[2][BN * DP];
     __shared__ __attribute__((aligned(16))) bf16_t Vs[2][BN * DP];
@@ -214,6 +214,7 @@ __global__ __launch_bounds__(64 * NW) void mattn_fwd_kernel(const Args a) {
 #pragma unroll
     for (int i = 0; i < NO; ++i) o[i] = (f32x16){};
     float m = -INFINITY, l = 0.f;
+    NotFinite odd;
     const int kb0 = bh > bl ? bl / BN : 0, kb1 = bh > bl ? (bh + BN - 1) / BN : 0;
     const int tq = (lane & 15) >> 2, tcol = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
 
@@ -289,7 +290,7 @@ __global__ __launch_bounds__(64 * NW) void mattn_fwd_kernel(const Args a) {
             while (bad != 0) {
                 const int k = kb * BN + __builtin_ctzll(bad);
                 bad &= bad - 1;
-                add_not_finite<T>(o, vbase + (int64_t)k * a.vs[1], a.D, h, k >= lo && k < hi);
+                odd.note<T, NO>(vbase + (int64_t)k * a.vs[1], a.D, h, k >= lo && k < hi);
             }
         }
 #pragma unroll
@@ -323,6 +324,12 @@ __global__ __launch_bounds__(64 * NW) void mattn_fwd_kernel(const Args a) {
     if (qi < a.Tq) {
         const float inv = l == 0.f ? 0.f : 1.f / l;   // nothing visible: 0
         bf16_t* orow = (bf16_t*)a.o + at.b * a.os[0] + at.h * a.os[2] + (int64_t)qi * a.os[1];
+        if (odd.any()) {
+#pragma unroll
+            for (int i = 0; i < NO; ++i)
+#pragma unroll
+                for (int k = 0; k < 16; ++k) o[i][k] = odd(o[i][k], 16 * i + k);
+        }
 #pragma unroll
         for (int i = 0; i < NO; ++i)
 #pragma unroll
@@ -381,6 +388,7 @@ __global__ __launch_bounds__(256, 2) void mattn_few_kernel(const Args a) {
 #pragma unroll
     for (int i = 0; i < NO; ++i) o[i] = (f32x16){};
     float m = -INFINITY, l = 0.f;
+    NotFinite odd;
     // this split's 32-key pieces u0 .. u1, dealt over the waves
     const int p0 = bh > bl ? bl / 32 : 0, np = bh > bl ? (bh + 31) / 32 - p0 : 0;
     const int per = (np + a.nsplit - 1) / a.nsplit;
@@ -447,7 +455,7 @@ __global__ __launch_bounds__(256, 2) void mattn_few_kernel(const Args a) {
             while (bad != 0) {
                 const int k = kb + __builtin_ctz(bad);
                 bad &= bad - 1;
-                add_not_finite<T>(o, vbase + (int64_t)k * a.vs[1], a.D, h, k >= lo && k < hi);
+                odd.note<T, NO>(vbase + (int64_t)k * a.vs[1], a.D, h, k >= lo && k < hi);
             }
         }
 #pragma unroll
@@ -466,6 +474,12 @@ __global__ __launch_bounds__(256, 2) void mattn_few_kernel(const Args a) {
     __syncthreads();
     float* od = (float*)smem;
     if (r < nr) {
+        if (odd.any()) {
+#pragma unroll
+            for (int i = 0; i < NO; ++i)
+#pragma unroll
+                for (int k = 0; k < 16; ++k) o[i][k] = odd(o[i][k], 16 * i + k);
+        }
 #pragma unroll
         for (int i = 0; i < NO; ++i)
 #pragma unroll
@@ -572,10 +586,9 @@ static int fwd_launch(const Args& a, hipStream_t s) {
         }
         TDL_LAUNCH_CHECK();
     }
-    const int64_t g4 = (int64_t)a.B * a.H * ((a.Tq + 127) / 128), g8 = (int64_t)a.B * a.H * ((a.Tq + 255) / 256);
-    if (g4 > 0x7fffffff) return (int)hipErrorInvalidValue;
-    if (g8 >= 512) mattn_fwd_kernel<T, DP, CAP, ALIBI, 8><<<(int)g8, 512, 0, s>>>(a);
-    else mattn_fwd_kernel<T, DP, CAP, ALIBI, 4><<<(int)g4, 256, 0, s>>>(a);
+    const int64_t grid = (int64_t)a.B * a.H * ((a.Tq + 127) / 128);
+    if (grid > 0x7fffffff) return (int)hipErrorInvalidValue;
+    mattn_fwd_kernel<T, DP, CAP, ALIBI><<<(int)grid, 256, 0, s>>>(a);
     TDL_LAUNCH_CHECK();
 }
 

@@ -190,8 +190,10 @@ def _strides(t: torch.Tensor):
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
-    """``t`` [B, T, heads, D] with unit column stride and 16-byte rows: as it is, or a contiguous copy."""
-    if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(t.stride(i) % 8 == 0 for i in range(3) if t.shape[i] > 1):
+    """``t`` [B, T, heads, D] with unit column stride and 16-byte rows (32 of which span less than 2 GiB):
+    as it is, or a contiguous copy."""
+    if (t.stride(3) == 1 and t.data_ptr() % 16 == 0 and t.stride(1) < 1 << 25
+            and all(t.stride(i) % 8 == 0 for i in range(3) if t.shape[i] > 1)):
         return t
     return t.contiguous()
 
@@ -247,7 +249,8 @@ def _backward(q, k, v, out, lse, dout, mask, scale, cap, slopes, dq, dk, dv):
                 g.zero_()
         return
     a = _args(q, k, v, mask, scale, cap, slopes)
-    delta = torch.empty_like(lse)
+    # the rows' statistics, padded to whole tiles: lse log2(e) and -rowsum(dout out)
+    delta = torch.empty(q.shape[0] * q.shape[2] * 2 * (-(-q.shape[1] // _Q_TILE) * _Q_TILE), dtype=torch.float32, device=q.device)
     a.o, a.os, a.lse, a.delta = out.data_ptr(), _strides(out), lse.data_ptr(), delta.data_ptr()
     a.dout, a.dos = dout.data_ptr(), _strides(dout)
     a.dq, a.dqs = dq.data_ptr(), _strides(dq)
