@@ -32,6 +32,7 @@ struct Args {
     const void *q, *k, *v, *dout;
     void *o, *dq, *dk, *dv;
     float *lse, *delta, *ws;
+    uint32_t* rest;      // what the rounding of o left out (e5m2 of Rest::SCALE times it), [B][Tq][H][D] bytes; null: not kept
     const float* slopes;
     const int *lo, *hi, *pos;
     const int4* qtab;    // [B][ceil(Tq / 32)]: lowest lo, highest hi (rows that see something), highest lo, lowest hi (all rows)
@@ -148,6 +149,32 @@ __device__ __forceinline__ void unrolled(F&& f) {
         unrolled<N, I + 1>(f);
     }
 }
+
+// The backward pass takes delta_i = dO_i . o_i.  From the rounded o it would carry o's rounding error
+// (2^-9 of |o| |dO|) into P (dP - delta), where peaked rows cancel: dQ and dK came out 1.8 times as far
+// from the exact ones as their own rounding.  So a forward pass that will be differentiated keeps the
+// remainder in 8 bits beside o: e5m2, 3 more bits of o, scaled into that type's range.
+template <class T>
+struct Rest {
+    static constexpr float SCALE = T::INF == 0x7f80 ? 512.f : 4096.f, MAX = 57344.f;
+    static __device__ __forceinline__ float clip(float x) { return __builtin_amdgcn_fmed3f(x * SCALE, -MAX, MAX); }
+    // of four values and their two packed roundings
+    static __device__ __forceinline__ uint32_t of(const float (&v)[4], uint2 r) {
+        float a, b, c, d;
+        T::unpack(r.x, a, b);
+        T::unpack(r.y, c, d);
+        int w = __builtin_amdgcn_cvt_pk_bf8_f32(clip(v[0] - a), clip(v[1] - b), 0, false);
+        w = __builtin_amdgcn_cvt_pk_bf8_f32(clip(v[2] - c), clip(v[3] - d), w, true);
+        return (uint32_t)w;
+    }
+    static __device__ __forceinline__ void back(uint32_t w, float (&v)[4]) {
+        const auto lo = __builtin_amdgcn_cvt_pk_f32_bf8((int)w, false), hi = __builtin_amdgcn_cvt_pk_f32_bf8((int)w, true);
+        v[0] = lo[0] * (1.f / SCALE);
+        v[1] = lo[1] * (1.f / SCALE);
+        v[2] = hi[0] * (1.f / SCALE);
+        v[3] = hi[1] * (1.f / SCALE);
+    }
+};
 
 // whether one of 8 values is an infinity or NaN (integer test on the exponent field)
 template <class T>

@@ -31,7 +31,8 @@ __global__ __launch_bounds__(64 * NW, DP == 64 ? 8 / NW : 1) void mattn_dq_kerne
     int lo = a.lo[(int64_t)at.b * a.Tq + qc], hi = a.hi[(int64_t)at.b * a.Tq + qc];
     if (qi >= a.Tq) lo = hi = 0;
     const float lse2 = a.lse[stat] * LOG2E;
-    // delta: both factors as the forward left them; the halves of the wave hold the halves of each row
+    // delta = dO . (o + what its rounding left out); the halves of the wave hold the halves of each row
+    const uint32_t* rest = a.rest + (((int64_t)at.b * a.Tq + qc) * a.H + at.h) * a.D / 4;
     typename T::vec qf[NS], df[NS];
     float delta = 0.f;
 #pragma unroll
@@ -42,14 +43,17 @@ __global__ __launch_bounds__(64 * NW, DP == 64 ? 8 / NW : 1) void mattn_dq_kerne
         qf[s] = as_vec<T>(c < a.D ? qu : z);
         df[s] = as_vec<T>(c < a.D ? du : z);
         if (c < a.D) {
-            const uint32_t dw[4] = {du.x, du.y, du.z, du.w}, ow[4] = {ou.x, ou.y, ou.z, ou.w};
+            const uint2 rw = *(const uint2*)(rest + cc / 4);
+            float rv[8];
+            Rest<T>::back(rw.x, *(float(*)[4])rv);
+            Rest<T>::back(rw.y, *(float(*)[4])(rv + 4));
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 float d0, d1, o0, o1;
-                T::unpack(dw[k], d0, d1);
-                T::unpack(ow[k], o0, o1);
-                delta = fmaf(d0, o0, delta);
-                delta = fmaf(d1, o1, delta);
+                T::unpack(du[k], d0, d1);
+                T::unpack(ou[k], o0, o1);
+                delta = fmaf(d0, o0 + rv[2 * k], delta);
+                delta = fmaf(d1, o1 + rv[2 * k + 1], delta);
             }
         }
     }

@@ -335,10 +335,14 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void mattn_fwd_kernel(const 
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const int d = 32 * i + 8 * g + 4 * h;
+                const float v[4] = {o[i][4 * g] * inv, o[i][4 * g + 1] * inv, o[i][4 * g + 2] * inv, o[i][4 * g + 3] * inv};
                 uint2 u;
-                u.x = T::pack(o[i][4 * g] * inv, o[i][4 * g + 1] * inv);
-                u.y = T::pack(o[i][4 * g + 2] * inv, o[i][4 * g + 3] * inv);
-                if (d < a.D) *(uint2*)(orow + d) = u;
+                u.x = T::pack(v[0], v[1]);
+                u.y = T::pack(v[2], v[3]);
+                if (d < a.D) {
+                    *(uint2*)(orow + d) = u;
+                    if (a.rest != nullptr) a.rest[((((int64_t)at.b * a.Tq + qi) * a.H + at.h) * a.D + d) / 4] = Rest<T>::of(v, u);
+                }
             }
         if (h == 0 && a.lse != nullptr)
             a.lse[((int64_t)at.b * a.H + at.h) * a.Tq + qi] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
@@ -346,6 +350,18 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void mattn_fwd_kernel(const 
 }
 
 // ============================================================================ few queries
+// four finished values of a row
+template <class T>
+__device__ __forceinline__ void put_out(const Args& a, const float (&acc)[4], float inv, int b, int h, int i, int d) {
+    if (d >= a.D) return;
+    const float v[4] = {acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv};
+    uint2 u;
+    u.x = T::pack(v[0], v[1]);
+    u.y = T::pack(v[2], v[3]);
+    *(uint2*)((bf16_t*)a.o + b * a.os[0] + h * a.os[2] + (int64_t)i * a.os[1] + d) = u;
+    if (a.rest != nullptr) a.rest[((((int64_t)b * a.Tq + i) * a.H + h) * a.D + d) / 4] = Rest<T>::of(v, u);
+}
+
 // Single tokens (or a few) against a long cache: bound by reading K and V once.  The rows of a tile are
 // the queries of ALL heads that share a KV head (row = g Tq + i), so the cache is read once per KV head;
 // the keys are split over `nsplit` workgroups and, within one, over 4 waves that never wait for each
@@ -515,10 +531,7 @@ __global__ __launch_bounds__(256, 2) void mattn_few_kernel(const Args a) {
             if (d == 0) *(float2*)ml = make_float2(M, L);
         } else {
             const float inv = L == 0.f ? 0.f : 1.f / L;
-            uint2 u2;
-            u2.x = T::pack(acc[0] * inv, acc[1] * inv);
-            u2.y = T::pack(acc[2] * inv, acc[3] * inv);
-            if (d < a.D) *(uint2*)((bf16_t*)a.o + b * a.os[0] + hh * a.os[2] + (int64_t)ii * a.os[1] + d) = u2;
+            put_out<T>(a, acc, inv, b, hh, ii, d);
             if (d == 0 && a.lse != nullptr) a.lse[out] = L == 0.f ? -INFINITY : (M + log2f(L)) * LN2;
         }
     }
@@ -551,10 +564,7 @@ __global__ __launch_bounds__(256) void mattn_join_kernel(const Args a) {
     const float inv = L == 0.f ? 0.f : 1.f / L;
     const int64_t bh = out / a.Tq;
     const int ii = (int)(out - bh * a.Tq), b = (int)(bh / a.H), hh = (int)(bh - (int64_t)b * a.H);
-    uint2 u;
-    u.x = T::pack(acc[0] * inv, acc[1] * inv);
-    u.y = T::pack(acc[2] * inv, acc[3] * inv);
-    if (d < a.D) *(uint2*)((bf16_t*)a.o + b * a.os[0] + hh * a.os[2] + (int64_t)ii * a.os[1] + d) = u;
+    put_out<T>(a, acc, inv, b, hh, ii, d);
     if (d == 0 && a.lse != nullptr) a.lse[out] = L == 0.f ? -INFINITY : (M + log2f(L)) * LN2;
 }
 

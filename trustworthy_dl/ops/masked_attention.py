@@ -177,7 +177,7 @@ def _mask_reference(B, Tq, Tk, causal, documents, rows, marks, lengths, q_start,
 # ============================================================== launches
 class _Args(ctypes.Structure):
     """csrc/masked_attention.h mattn::Args"""
-    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v", "dout", "o", "dq", "dk", "dv", "lse", "delta", "ws", "slopes",
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v", "dout", "o", "dq", "dk", "dv", "lse", "delta", "ws", "rest", "slopes",
                                                 "lo", "hi", "pos", "qtab", "ktab")]
                 + [(n, ctypes.c_int64 * 3) for n in ("qs", "ks", "vs", "os", "dos", "dqs", "dks", "dvs")]
                 + [(n, ctypes.c_int) for n in ("B", "Tq", "Tk", "H", "Hk", "D", "dtype", "nsplit")]
@@ -221,16 +221,19 @@ def _args(q, k, v, mask: AttentionMask, scale: float, cap: float, slopes) -> _Ar
     return a
 
 
-def _forward(q, k, v, mask, scale, cap, slopes, want_lse: bool):
+def _forward(q, k, v, mask, scale, cap, slopes, want_lse: bool, want_rest: bool):
+    """(out, lse or None, out's rounding remainder for the backward pass or None)"""
     B, Tq, H, D = q.shape
     Tk, Hk = k.shape[1], k.shape[2]
     out = torch.empty(B, Tq, H, D, dtype=q.dtype, device=q.device)
     lse = torch.empty(B, H, Tq, dtype=torch.float32, device=q.device) if want_lse else None
+    rest = torch.empty(B, Tq, H, D, dtype=torch.uint8, device=q.device) if want_rest else None
     if out.numel() == 0:
-        return out, lse
+        return out, lse, rest
     a = _args(q, k, v, mask, scale, cap, slopes)
     a.o, a.os = out.data_ptr(), _strides(out)
     a.lse = 0 if lse is None else lse.data_ptr()
+    a.rest = 0 if rest is None else rest.data_ptr()
     a.nsplit = few_queries(B, Hk, H // Hk, Tq, Tk)
     ws = None
     if a.nsplit > 1:
@@ -238,10 +241,10 @@ def _forward(q, k, v, mask, scale, cap, slopes, want_lse: bool):
         a.ws = ws.data_ptr()
     with _on_device(q.device):
         _lib.call("tdl_masked_attn_fwd", ctypes.addressof(a), stream_ptr(q.device))
-    return out, lse
+    return out, lse, rest
 
 
-def _backward(q, k, v, out, lse, dout, mask, scale, cap, slopes, dq, dk, dv):
+def _backward(q, k, v, out, lse, rest, dout, mask, scale, cap, slopes, dq, dk, dv):
     """Writes dq and, unless both are None, dk and dv."""
     if q.numel() == 0:
         for g in (dk, dv):
@@ -252,6 +255,7 @@ def _backward(q, k, v, out, lse, dout, mask, scale, cap, slopes, dq, dk, dv):
     # the rows' statistics, padded to whole tiles: lse log2(e) and -rowsum(dout out)
     delta = torch.empty(q.shape[0] * q.shape[2] * 2 * (-(-q.shape[1] // _Q_TILE) * _Q_TILE), dtype=torch.float32, device=q.device)
     a.o, a.os, a.lse, a.delta = out.data_ptr(), _strides(out), lse.data_ptr(), delta.data_ptr()
+    a.rest = rest.data_ptr()
     a.dout, a.dos = dout.data_ptr(), _strides(dout)
     a.dq, a.dqs = dq.data_ptr(), _strides(dq)
     if dk is not None:
@@ -264,8 +268,9 @@ class _MaskedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, mask, scale, cap, slopes, want_lse):
         q, k, v = _aligned(q), _aligned(k), _aligned(v)
-        out, lse = _forward(q, k, v, mask, scale, cap, slopes, want_lse or any(ctx.needs_input_grad[:3]))
-        ctx.save_for_backward(q, k, v, out, lse, slopes)
+        grad = any(ctx.needs_input_grad[:3])
+        out, lse, rest = _forward(q, k, v, mask, scale, cap, slopes, want_lse or grad, grad)
+        ctx.save_for_backward(q, k, v, out, lse, rest, slopes)
         ctx.mask, ctx.scale, ctx.cap = mask, scale, cap
         if lse is not None:
             ctx.mark_non_differentiable(lse)
@@ -274,12 +279,12 @@ class _MaskedAttention(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dout, _dlse):
-        q, k, v, out, lse, slopes = ctx.saved_tensors
+        q, k, v, out, lse, rest, slopes = ctx.saved_tensors
         keys = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
         dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         dk = torch.empty(k.shape, dtype=k.dtype, device=k.device) if keys else None
         dv = torch.empty(v.shape, dtype=v.dtype, device=v.device) if keys else None
-        _backward(q, k, v, out, lse, _aligned(dout), ctx.mask, ctx.scale, ctx.cap, slopes, dq, dk, dv)
+        _backward(q, k, v, out, lse, rest, _aligned(dout), ctx.mask, ctx.scale, ctx.cap, slopes, dq, dk, dv)
         return dq, dk, dv, None, None, None, None, None
 
 
@@ -290,17 +295,17 @@ class _MaskedAttentionPacked(torch.autograd.Function):
     def forward(ctx, qkv, n_head, n_kv_head, mask, scale, cap, slopes):
         qkv = _aligned(qkv)
         q, k, v = qkv.split((n_head, n_kv_head, n_kv_head), dim=2)
-        out, lse = _forward(q, k, v, mask, scale, cap, slopes, ctx.needs_input_grad[0])
-        ctx.save_for_backward(qkv, out, lse, slopes)
+        out, lse, rest = _forward(q, k, v, mask, scale, cap, slopes, ctx.needs_input_grad[0], ctx.needs_input_grad[0])
+        ctx.save_for_backward(qkv, out, lse, rest, slopes)
         ctx.mask, ctx.scale, ctx.cap, ctx.heads = mask, scale, cap, (n_head, n_kv_head, n_kv_head)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        qkv, out, lse, slopes = ctx.saved_tensors
+        qkv, out, lse, rest, slopes = ctx.saved_tensors
         dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
-        _backward(*qkv.split(ctx.heads, dim=2), out, lse, _aligned(dout), ctx.mask, ctx.scale, ctx.cap, slopes,
+        _backward(*qkv.split(ctx.heads, dim=2), out, lse, rest, _aligned(dout), ctx.mask, ctx.scale, ctx.cap, slopes,
                   *dqkv.split(ctx.heads, dim=2))
         return dqkv, None, None, None, None, None, None
 
