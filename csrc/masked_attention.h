@@ -204,23 +204,20 @@ struct NotFinite {
     // row: where it stands in memory
     template <class T, int NO>
     __device__ __forceinline__ void note(const bf16_t* row, int D, int h, bool see) {
+#pragma unroll 1
+        for (int c = 0; c < 4 * NO; ++c) {   // (rolled: few registers and little code beside the hot loops)
+            const int d = 8 * c + 4 * h;
+            const uint2 u = *(const uint2*)(row + (d < D ? d : 0));
+            const uint32_t w[2] = {u.x, u.y};
 #pragma unroll
-        for (int i = 0; i < NO; ++i)
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const int d = 32 * i + 8 * g + 4 * h;
-                const uint2 u = *(const uint2*)(row + (d < D ? d : 0));
-                const uint32_t w[2] = {u.x, u.y};
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const uint32_t x = (w[k >> 1] >> (16 * (k & 1))) & 0xffffu;
-                    const bool bad = see && d < D && (x & 0x7fffu) >= T::INF, inf = (x & 0x7fffu) == T::INF;
-                    const uint64_t bit = 1ull << (16 * i + 4 * g + k);
-                    if (bad && !(inf && (x & 0x8000u))) up |= bit;
-                    if (bad && !(inf && !(x & 0x8000u))) down |= bit;
-                }
-                __builtin_amdgcn_sched_barrier(0);   // one load at a time: no registers for more
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t x = (w[k >> 1] >> (16 * (k & 1))) & 0xffffu;
+                const bool bad = see && d < D && (x & 0x7fffu) >= T::INF, inf = (x & 0x7fffu) == T::INF;
+                const uint64_t bit = 1ull << (4 * c + k);
+                if (bad && !(inf && (x & 0x8000u))) up |= bit;
+                if (bad && !(inf && !(x & 0x8000u))) down |= bit;
             }
+        }
     }
     __device__ __forceinline__ bool any() const { return (up | down) != 0; }
     // element e (a constant) of the finished sums

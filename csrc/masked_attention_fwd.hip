@@ -372,7 +372,7 @@ template <class T, int DP, bool CAP, bool ALIBI>
 __global__ __launch_bounds__(256, 2) void mattn_few_kernel(const Args a) {
     constexpr int NS = DP / 16, NO = DP / 32, NW = 4, NCH = DP / 8;
     typedef Tile<T, DP, 32, 64> TL;   // one wave's V tile
-    extern __shared__ __attribute__((aligned(16))) char smem[];
+    __shared__ __attribute__((aligned(16))) char smem[NW * 32 * DP * 2];   // V tiles; then halves of O, [wave][row][DP / 2] floats
     __shared__ float mls[NW][2][32];
     __shared__ __attribute__((aligned(16))) uint8_t vflag[NW][64 * NCH];
     const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, r = lane & 31;
@@ -411,15 +411,23 @@ __global__ __launch_bounds__(256, 2) void mattn_few_kernel(const Args a) {
     const int u0 = p0 + min(split * per, np), u1 = p0 + min((split + 1) * per, np);
     const int tq = (lane & 15) >> 2, tcol = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
     u32x4 kr[NS], vr[TL::N];
+    // 32 rows through a buffer resource that starts at the first: the lane's offsets never change (nor is
+    // a 64-bit address held per load), keys past the tensor and columns past D (offset 2^31) read as zeros
+    auto rows_of = [&](const bf16_t* base, int64_t ld, int u) {
+        const int left = min(a.Tk - u * 32, 32);
+        return __builtin_amdgcn_make_buffer_rsrc((void*)(base + (int64_t)u * 32 * ld), 0, (uint32_t)((left - 1) * ld + a.D) * 2u,
+                                                 0x00020000);
+    };
+    const uint32_t koff = (uint32_t)(r * a.ks[1] + 8 * h) * 2u;
+    const uint32_t voff = TL::chunk(lane) * 8 < a.D ? (uint32_t)(TL::row(lane, 0) * a.vs[1] + TL::chunk(lane) * 8) * 2u : 0x80000000u;
+    const uint32_t vstep = (uint32_t)(TL::RPP * a.vs[1]) * 2u;   // (31 rows span less than 2 GiB: 2^31 + 31 rows stay out of range)
     auto gload = [&](int u) {
-        const int kk = min(u * 32 + r, a.Tk - 1);
-        const bf16_t* kp = kbase + (int64_t)kk * a.ks[1];
+        const __amdgpu_buffer_rsrc_t kb_ = rows_of(kbase, a.ks[1], u), vb_ = rows_of(vbase, a.vs[1], u);
 #pragma unroll
-        for (int s = 0; s < NS; ++s) {
-            const int c = 16 * s + 8 * h;
-            kr[s] = *(const u32x4*)(kp + (c < a.D ? c : 0));
-        }
-        TL::load(vr, vbase, a.vs[1], u * 32, a.Tk - 1, a.D, lane);
+        for (int s = 0; s < NS; ++s)
+            kr[s] = __builtin_amdgcn_raw_buffer_load_b128(kb_, 16 * s + 8 * h < a.D ? koff + 32 * s : 0x80000000u, 0, 0);
+#pragma unroll
+        for (int j = 0; j < TL::N; ++j) vr[j] = __builtin_amdgcn_raw_buffer_load_b128(vb_, voff + j * vstep, 0, 0);
     };
     int u = u0 + w;
     if (u < u1) gload(u);
@@ -482,31 +490,37 @@ __global__ __launch_bounds__(256, 2) void mattn_few_kernel(const Args a) {
         }
     }
     l += __shfl_xor(l, 32, 64);
-    // join the waves: weights 2^(m_w - M), O through LDS ([wave][row][DP] floats, the V tiles are done)
+    // join the waves: weights 2^(m_w - M), O through LDS
     if (h == 0) {
         mls[w][0][r] = m;
         mls[w][1][r] = l;
     }
     __syncthreads();
+    // (half of the columns at a time: no more LDS than the V tiles had)
     float* od = (float*)smem;
-    if (r < nr) {
-        if (odd.any()) {
-#pragma unroll
-            for (int i = 0; i < NO; ++i)
-#pragma unroll
-                for (int k = 0; k < 16; ++k) o[i][k] = odd(o[i][k], 16 * i + k);
-        }
+    constexpr int DH = DP / 2;
+    if (odd.any()) {
 #pragma unroll
         for (int i = 0; i < NO; ++i)
 #pragma unroll
+            for (int k = 0; k < 16; ++k) o[i][k] = odd(o[i][k], 16 * i + k);
+    }
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+    if (half) __syncthreads();   // the first half has been read
+    if (r < nr) {
+#pragma unroll
+        for (int i = 0; i < NO / 2; ++i)
+#pragma unroll
             for (int q4 = 0; q4 < 4; ++q4) {
-                const float4 f = make_float4(o[i][4 * q4], o[i][4 * q4 + 1], o[i][4 * q4 + 2], o[i][4 * q4 + 3]);
-                *(float4*)(od + ((w * nr + r) * DP + 32 * i + 8 * q4 + 4 * h)) = f;
+                const f32x16& f = o[half * (NO / 2) + i];
+                *(float4*)(od + ((w * nr + r) * DH + 32 * i + 8 * q4 + 4 * h)) =
+                    make_float4(f[4 * q4], f[4 * q4 + 1], f[4 * q4 + 2], f[4 * q4 + 3]);
             }
     }
     __syncthreads();
-    for (int e = tid; e < nr * (DP / 4); e += 256) {
-        const int rr = e / (DP / 4), d = (e - rr * (DP / 4)) * 4;
+    for (int e = tid; e < nr * (DH / 4); e += 256) {
+        const int rr = e / (DH / 4), dh = (e - rr * (DH / 4)) * 4, d = half * DH + dh;
         float M = mls[0][0][rr];
 #pragma unroll
         for (int x = 1; x < NW; ++x) M = fmaxf(M, mls[x][0][rr]);
@@ -515,7 +529,7 @@ __global__ __launch_bounds__(256, 2) void mattn_few_kernel(const Args a) {
 #pragma unroll
         for (int x = 0; x < NW; ++x) {
             const float wt = exp2_fast(mls[x][0][rr] - Ms);
-            const float4 f = *(const float4*)(od + ((x * nr + rr) * DP + d));
+            const float4 f = *(const float4*)(od + ((x * nr + rr) * DH + dh));
             L += wt * mls[x][1][rr];
             acc[0] += wt * f.x;
             acc[1] += wt * f.y;
@@ -534,6 +548,7 @@ __global__ __launch_bounds__(256, 2) void mattn_few_kernel(const Args a) {
             put_out<T>(a, acc, inv, b, hh, ii, d);
             if (d == 0 && a.lse != nullptr) a.lse[out] = L == 0.f ? -INFINITY : (M + log2f(L)) * LN2;
         }
+    }
     }
 }
 
@@ -577,17 +592,10 @@ static bool bad_args(const Args& a) {
 template <class T, int DP, bool CAP, bool ALIBI>
 static int fwd_launch(const Args& a, hipStream_t s) {
     if (a.nsplit > 0) {
-        const int R = (a.H / a.Hk) * a.Tq, rt = (R + 31) / 32, nr = R < 32 ? R : 32;   // rows, tiles of 32, rows of a tile
-        const size_t join = (size_t)4 * nr * DP * 4, tiles = (size_t)4 * 32 * DP * 2;
+        const int R = (a.H / a.Hk) * a.Tq, rt = (R + 31) / 32;   // rows, tiles of 32
         const int64_t grid = (int64_t)a.B * a.Hk * a.nsplit * rt;
         if (grid > 0x7fffffff) return (int)hipErrorInvalidValue;
-        const size_t lds = join > tiles ? join : tiles;
-        if (lds > 32768) {   // past the default limit of 64 KiB with the kernel's static part
-            const int rc = (int)hipFuncSetAttribute((const void*)mattn_few_kernel<T, DP, CAP, ALIBI>,
-                                                    hipFuncAttributeMaxDynamicSharedMemorySize, 65536);
-            if (rc) return rc;
-        }
-        mattn_few_kernel<T, DP, CAP, ALIBI><<<(int)grid, 256, lds, s>>>(a);
+        mattn_few_kernel<T, DP, CAP, ALIBI><<<(int)grid, 256, 0, s>>>(a);
         if (a.nsplit > 1) {
             const int rc = (int)hipGetLastError();
             if (rc) return rc;

@@ -219,4 +219,15 @@ def call(name: str, *args):
             raise RuntimeError(f"native kernel {name} faulted: {e}") from e
 
 
+def call_on(device: torch.device, name: str, *args):
+    """``call`` on ``device``, whichever device is current, with its current stream as the last argument.
+    (Small calls are bound by the host: the stream's handle is read directly, without a Stream object.)"""
+    index = device.index
+    if index is None or index == torch.cuda.current_device():
+        call(name, *args, torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index))
+    else:
+        with torch.cuda.device(index):
+            call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+
+
 DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}

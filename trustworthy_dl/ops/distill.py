@@ -19,8 +19,6 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import stream_ptr
-from .masked_attention import _on_device
 
 MAX_ENTRIES = 1024   # csrc/distill.hip MAX_K
 
@@ -43,18 +41,13 @@ def _grad_like(z: torch.Tensor) -> torch.Tensor:
 
 
 def _launch(z, index, teacher, labels, V, tau, alpha, counts, grad=None, rows=None, loss=None, gscale=None, written=False):
-    a = _Args()
     M, W = z.shape
-    a.logits, a.index, a.teacher, a.counts = z.data_ptr(), index.data_ptr(), teacher.data_ptr(), counts.data_ptr()
-    for name, t in (("grad", grad), ("labels", labels), ("gscale", gscale), ("rows", rows), ("loss", loss)):
-        setattr(a, name, 0 if t is None else t.data_ptr())
-    a.ld, a.gld = z.stride(0), grad.stride(0) if grad is not None else 0
-    a.M, a.V, a.W, a.K, a.G = M, V, W, index.shape[1], counts.shape[0]
-    a.dtype, a.teacher_dtype = _lib.DTYPE_CODE[z.dtype], _lib.DTYPE_CODE[teacher.dtype]
-    a.index64, a.written = int(index.dtype == torch.int64), int(written)
-    a.tau, a.alpha, a.beta = tau, alpha, 1.0 - alpha
-    with _on_device(z.device):
-        _lib.call("tdl_distill", ctypes.addressof(a), stream_ptr(z.device))
+    gptr, gld = (0, 0) if grad is None else (grad.data_ptr(), grad.stride(0))
+    a = _Args(z.data_ptr(), gptr, index.data_ptr(), teacher.data_ptr(), 0 if labels is None else labels.data_ptr(),
+              0 if gscale is None else gscale.data_ptr(), 0 if rows is None else rows.data_ptr(), counts.data_ptr(),
+              0 if loss is None else loss.data_ptr(), z.stride(0), gld, M, V, W, index.shape[1], counts.shape[0],
+              _lib.DTYPE_CODE[z.dtype], index.dtype is torch.int64, _lib.DTYPE_CODE[teacher.dtype], written, tau, alpha, 1.0 - alpha)
+    _lib.call_on(z.device, "tdl_distill", ctypes.addressof(a))
 
 
 class _Distill(torch.autograd.Function):
@@ -83,7 +76,7 @@ class _Distill(torch.autograd.Function):
         written = grad is not None   # else a second backward through the same node: its own buffer
         if not written:
             grad = _grad_like(z)
-        _launch(z, index, teacher, labels, *ctx.how, counts, grad=grad, gscale=g.to(torch.float32).contiguous(), written=written)
+        _launch(z, index, teacher, labels, *ctx.how, counts, grad=grad, gscale=g, written=written)
         return (grad,) + (None,) * 6
 
 
@@ -156,8 +149,9 @@ def distillation_loss(logits: torch.Tensor, teacher_index: torch.Tensor, teacher
     for name, t in (("teacher_index", teacher_index), ("teacher_logits", teacher_logits), ("labels", labels)):
         if t is not None and t.device != logits.device:
             raise ValueError(f"distillation_loss: {name} is on {t.device}, the logits on {logits.device}")
-    z = logits.reshape(-1, W)
-    index, teacher = teacher_index.reshape(-1, K), teacher_logits.reshape(-1, K)
+    z, index, teacher = logits, teacher_index, teacher_logits
+    if z.dim() != 2:
+        z, index, teacher = z.reshape(-1, W), index.reshape(-1, K), teacher.reshape(-1, K)
     labels = None if labels is None else labels.reshape(-1).long()
     if z.shape[0] == 0:
         return z.float().sum()   # no rows: zero, with a gradient of no rows

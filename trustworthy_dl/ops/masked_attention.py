@@ -22,26 +22,10 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import ptr, stream_ptr
+from ._lib import ptr
 
 _Q_TILE, _K_TILE = 32, 128     # csrc/masked_attention.h QT, KT
 MAX_SOFTCAP = 1000.0
-
-
-class _on_device:
-    """Launch on the tensors' device, whichever device is current."""
-
-    def __init__(self, device: torch.device):
-        self.guard = None if device.index in (None, torch.cuda.current_device()) else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-        return False
 
 
 # ============================================================== the mask
@@ -135,10 +119,9 @@ def attention_mask(batch: int, q_len: int, k_len: Optional[int] = None, *, causa
     if batch == 0 or q_len == 0:
         return m
     ws = ints(batch * 3 * k_len) if documents is not None or marks is not None else None
-    with _on_device(device):
-        _lib.call("tdl_attn_mask", ptr(documents), int(documents is not None and documents.dtype == torch.int64), ptr(rows),
-                  ptr(marks), ptr(lengths), ptr(q_start), batch, q_len, k_len, int(causal), ptr(ws), ptr(m.lo), ptr(m.hi),
-                  ptr(m.pos), ptr(m.q_table), ptr(m.k_table), stream_ptr(device))
+    _lib.call_on(device, "tdl_attn_mask", ptr(documents), int(documents is not None and documents.dtype == torch.int64), ptr(rows),
+                 ptr(marks), ptr(lengths), ptr(q_start), batch, q_len, k_len, int(causal), ptr(ws), ptr(m.lo), ptr(m.hi),
+                 ptr(m.pos), ptr(m.q_table), ptr(m.k_table))
     return m
 
 
@@ -176,25 +159,30 @@ def _mask_reference(B, Tq, Tk, causal, documents, rows, marks, lengths, q_start,
 
 # ============================================================== launches
 class _Args(ctypes.Structure):
-    """csrc/masked_attention.h mattn::Args"""
+    """csrc/masked_attention.h mattn::Args (strides: batch, token, head of each tensor)"""
     _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v", "dout", "o", "dq", "dk", "dv", "lse", "delta", "ws", "rest", "slopes",
                                                 "lo", "hi", "pos", "qtab", "ktab")]
-                + [(n, ctypes.c_int64 * 3) for n in ("qs", "ks", "vs", "os", "dos", "dqs", "dks", "dvs")]
+                + [(n + i, ctypes.c_int64) for n in ("qs", "ks", "vs", "os", "dos", "dqs", "dks", "dvs") for i in "012"]
                 + [(n, ctypes.c_int) for n in ("B", "Tq", "Tk", "H", "Hk", "D", "dtype", "nsplit")]
                 + [("scale", ctypes.c_float), ("cap", ctypes.c_float)])
 
 
+_UNUSED = (0, 0, 0)
+
+
 def _strides(t: torch.Tensor):
     # a dimension of one element is never stepped over
-    return (ctypes.c_int64 * 3)(*[t.stride(i) if t.shape[i] > 1 else 0 for i in range(3)])
+    (b, n, h, _), (sb, sn, sh, _) = t.shape, t.stride()
+    return sb if b > 1 else 0, sn if n > 1 else 0, sh if h > 1 else 0
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
     """``t`` [B, T, heads, D] with unit column stride and 16-byte rows (32 of which span less than 2 GiB):
     as it is, or a contiguous copy."""
-    if (t.stride(3) == 1 and t.data_ptr() % 16 == 0 and t.stride(1) < 1 << 25
-            and all(t.stride(i) % 8 == 0 for i in range(3) if t.shape[i] > 1)):
-        return t
+    s = t.stride()
+    if s[3] == 1 and t.data_ptr() % 16 == 0 and s[1] < 1 << 25:
+        if not (s[0] | s[1] | s[2]) % 8 or all(s[i] % 8 == 0 for i in range(3) if t.shape[i] > 1):
+            return t
     return t.contiguous()
 
 
@@ -204,43 +192,29 @@ def few_queries(batch: int, kv_heads: int, group: int, q_len: int, k_len: int) -
     if q_len > 16:
         return 0
     tiles = batch * kv_heads * -(-(group * q_len) // 32)
-    return max(1, min(1024 // tiles, -(-k_len // 128), 64))
-
-
-def _args(q, k, v, mask: AttentionMask, scale: float, cap: float, slopes) -> _Args:
-    a = _Args()
-    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    a.qs, a.ks, a.vs = _strides(q), _strides(k), _strides(v)
-    a.B, a.Tq, a.H, a.D = q.shape
-    a.Tk, a.Hk = k.shape[1], k.shape[2]
-    a.dtype = _lib.DTYPE_CODE[q.dtype]
-    a.scale, a.cap = scale, cap
-    a.slopes = 0 if slopes is None else slopes.data_ptr()
-    a.lo, a.hi, a.pos = mask.lo.data_ptr(), mask.hi.data_ptr(), mask.pos.data_ptr()
-    a.qtab, a.ktab = mask.q_table.data_ptr(), mask.k_table.data_ptr()
-    return a
+    return max(1, min(max(-(-512 // tiles), 4), k_len // 512, 64))
 
 
 def _forward(q, k, v, mask, scale, cap, slopes, want_lse: bool, want_rest: bool):
     """(out, lse or None, out's rounding remainder for the backward pass or None)"""
     B, Tq, H, D = q.shape
     Tk, Hk = k.shape[1], k.shape[2]
-    out = torch.empty(B, Tq, H, D, dtype=q.dtype, device=q.device)
-    lse = torch.empty(B, H, Tq, dtype=torch.float32, device=q.device) if want_lse else None
-    rest = torch.empty(B, Tq, H, D, dtype=torch.uint8, device=q.device) if want_rest else None
+    dev = q.device
+    out = torch.empty(B, Tq, H, D, dtype=q.dtype, device=dev)
+    lse = torch.empty(B, H, Tq, dtype=torch.float32, device=dev) if want_lse else None
+    rest = torch.empty(B, Tq, H, D, dtype=torch.uint8, device=dev) if want_rest else None
     if out.numel() == 0:
         return out, lse, rest
-    a = _args(q, k, v, mask, scale, cap, slopes)
-    a.o, a.os = out.data_ptr(), _strides(out)
-    a.lse = 0 if lse is None else lse.data_ptr()
-    a.rest = 0 if rest is None else rest.data_ptr()
-    a.nsplit = few_queries(B, Hk, H // Hk, Tq, Tk)
+    nsplit = few_queries(B, Hk, H // Hk, Tq, Tk)
     ws = None
-    if a.nsplit > 1:
-        ws = torch.empty(B * H * Tq * a.nsplit * ((64 if D <= 64 else 128) + 2), dtype=torch.float32, device=q.device)
-        a.ws = ws.data_ptr()
-    with _on_device(q.device):
-        _lib.call("tdl_masked_attn_fwd", ctypes.addressof(a), stream_ptr(q.device))
+    if nsplit > 1:
+        ws = torch.empty(B * H * Tq * nsplit * ((64 if D <= 64 else 128) + 2), dtype=torch.float32, device=dev)
+    a = _Args(q.data_ptr(), k.data_ptr(), v.data_ptr(), 0, out.data_ptr(), 0, 0, 0, 0 if lse is None else lse.data_ptr(), 0,
+              0 if ws is None else ws.data_ptr(), 0 if rest is None else rest.data_ptr(), 0 if slopes is None else slopes.data_ptr(),
+              mask.lo.data_ptr(), mask.hi.data_ptr(), mask.pos.data_ptr(), mask.q_table.data_ptr(), mask.k_table.data_ptr(),
+              *_strides(q), *_strides(k), *_strides(v), *_strides(out), *_UNUSED, *_UNUSED, *_UNUSED, *_UNUSED,
+              B, Tq, Tk, H, Hk, D, _lib.DTYPE_CODE[q.dtype], nsplit, scale, cap)
+    _lib.call_on(dev, "tdl_masked_attn_fwd", ctypes.addressof(a))
     return out, lse, rest
 
 
@@ -251,17 +225,17 @@ def _backward(q, k, v, out, lse, rest, dout, mask, scale, cap, slopes, dq, dk, d
             if g is not None:
                 g.zero_()
         return
-    a = _args(q, k, v, mask, scale, cap, slopes)
+    B, Tq, H, D = q.shape
     # the rows' statistics, padded to whole tiles: lse log2(e) and -rowsum(dout out)
-    delta = torch.empty(q.shape[0] * q.shape[2] * 2 * (-(-q.shape[1] // _Q_TILE) * _Q_TILE), dtype=torch.float32, device=q.device)
-    a.o, a.os, a.lse, a.delta = out.data_ptr(), _strides(out), lse.data_ptr(), delta.data_ptr()
-    a.rest = rest.data_ptr()
-    a.dout, a.dos = dout.data_ptr(), _strides(dout)
-    a.dq, a.dqs = dq.data_ptr(), _strides(dq)
-    if dk is not None:
-        a.dk, a.dv, a.dks, a.dvs = dk.data_ptr(), dv.data_ptr(), _strides(dk), _strides(dv)
-    with _on_device(q.device):
-        _lib.call("tdl_masked_attn_bwd", ctypes.addressof(a), stream_ptr(q.device))
+    delta = torch.empty(B * H * 2 * (-(-Tq // _Q_TILE) * _Q_TILE), dtype=torch.float32, device=q.device)
+    keys = dk is not None
+    a = _Args(q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(), out.data_ptr(), dq.data_ptr(), dk.data_ptr() if keys else 0,
+              dv.data_ptr() if keys else 0, lse.data_ptr(), delta.data_ptr(), 0, rest.data_ptr(),
+              0 if slopes is None else slopes.data_ptr(), mask.lo.data_ptr(), mask.hi.data_ptr(), mask.pos.data_ptr(),
+              mask.q_table.data_ptr(), mask.k_table.data_ptr(), *_strides(q), *_strides(k), *_strides(v), *_strides(out),
+              *_strides(dout), *_strides(dq), *(_strides(dk) if keys else _UNUSED), *(_strides(dv) if keys else _UNUSED),
+              B, Tq, k.shape[1], H, k.shape[2], D, _lib.DTYPE_CODE[q.dtype], 0, scale, cap)
+    _lib.call_on(q.device, "tdl_masked_attn_bwd", ctypes.addressof(a))
 
 
 class _MaskedAttention(torch.autograd.Function):
@@ -272,6 +246,7 @@ class _MaskedAttention(torch.autograd.Function):
         out, lse, rest = _forward(q, k, v, mask, scale, cap, slopes, want_lse or grad, grad)
         ctx.save_for_backward(q, k, v, out, lse, rest, slopes)
         ctx.mask, ctx.scale, ctx.cap = mask, scale, cap
+        ctx.set_materialize_grads(False)   # (no zeros for the statistics)
         if lse is not None:
             ctx.mark_non_differentiable(lse)
         return out, lse
@@ -279,6 +254,8 @@ class _MaskedAttention(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dout, _dlse):
+        if dout is None:
+            return (None,) * 8
         q, k, v, out, lse, rest, slopes = ctx.saved_tensors
         keys = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
         dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
@@ -390,8 +367,10 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: At
     ``return_lse`` also the fp32 log-sum-exp of each query's scores [B, H, Tq] (-inf where it sees
     nothing; not differentiable)."""
     scale, cap, slopes = _check("masked_attention", q, k, v, mask, scale, softcap, slopes)
-    if q.is_cuda:
+    if q.is_cuda and torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         out, lse = _MaskedAttention.apply(q, k, v, mask, scale, cap, slopes, return_lse)
+    elif q.is_cuda:   # (a single token's call is bound by the host: no autograd node)
+        out, lse, _ = _forward(_aligned(q), _aligned(k), _aligned(v), mask, scale, cap, slopes, return_lse, False)
     else:
         out, lse = _reference(q, k, v, mask, scale, cap, slopes)
     return (out, lse) if return_lse else out
