@@ -251,17 +251,21 @@ struct Score {
     float mul;      // scale log2(e)
     float c2;       // 2 log2(e) scale / cap
     float capl;     // cap log2(e)
+    float c1;       // -1 / (2 capl)
     float slope;    // slope log2(e)
     __device__ __forceinline__ void init(float scale, float cap, float sl) {
         mul = scale * LOG2E;
         if (CAP) {
             c2 = 2.f * LOG2E * scale / cap;
             capl = cap * LOG2E;
+            c1 = -0.5f / capl;
         }
         slope = ALIBI ? sl * LOG2E : 0.f;
     }
     // 1 / (1 + e^(2 u)), u = x / cap: tanh u = 1 - 2 r, its derivative 4 r (1 - r)
     __device__ __forceinline__ float sat(float dot) const { return __builtin_amdgcn_rcpf(1.f + exp2_fast(dot * c2)); }
+    // capped score less its bound, -2 capl / (1 + e^(2 u)): the factor rides in the sum's fma
+    __device__ __forceinline__ float below(float dot) const { return __builtin_amdgcn_rcpf(fmaf(exp2_fast(dot * c2), c1, c1)); }
     __device__ __forceinline__ float capped(float r) const { return fmaf(-2.f * capl, r, capl); }
     __device__ __forceinline__ float biased(float y, float dist) const {
         return ALIBI ? fmaf(-slope, fabsf(dist), y) : y;

@@ -213,7 +213,12 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void mattn_fwd_kernel(const 
     f32x16 o[NO];
 #pragma unroll
     for (int i = 0; i < NO; ++i) o[i] = (f32x16){};
-    float m = -INFINITY, l = 0.f;
+    // Capped scores without a bias are taken less their bound, the cap (Score::below): in [-2 cap, 0].  Up
+    // to a cap of 32 a bf16 softmax needs no running maximum then: its smallest weight is e^-64, well in
+    // bf16's range (not in fp16's).  1 x 8 x 2048 x 25 heads: FIXED us against RUNNING us.
+    constexpr bool SAT = CAP && !ALIBI;
+    const bool fixed = SAT && T::INF == 0x7f80 && a.cap <= 32.f;
+    float m = fixed ? 0.f : -INFINITY, l = 0.f;
     NotFinite odd;
     const int kb0 = bh > bl ? bl / BN : 0, kb1 = bh > bl ? (bh + BN - 1) / BN : 0;
     const int tq = (lane & 15) >> 2, tcol = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
@@ -245,7 +250,12 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void mattn_fwd_kernel(const 
             s[0] = T::mfma(a0, qf[d], s[0]);
             s[1] = T::mfma(a1, qf[d], s[1]);
         }
-        if constexpr (!Score<CAP, ALIBI>::PLAIN) {
+        if constexpr (SAT) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[t][i] = sc.below(s[t][i]);
+        } else if constexpr (!Score<CAP, ALIBI>::PLAIN) {
             const float d0 = (float)(kb * BN + 4 * h) - qpos;
 #pragma unroll
             for (int t = 0; t < 2; ++t)
@@ -261,27 +271,30 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void mattn_fwd_kernel(const 
                 for (int i = 0; i < 16; ++i)
                     s[t][i] = (uint32_t)(k0 + 32 * t + (i & 3) + 8 * (i >> 2)) < n ? s[t][i] : -INFINITY;
         }
-        float mx = max3(s[0][0], s[1][0], s[0][1]);
+        float ms = m;
+        if (!fixed) {
+            float mx = max3(s[0][0], s[1][0], s[0][1]);
 #pragma unroll
-        for (int i = 1; i < 16; ++i) mx = max3(mx, s[1][i], i + 1 < 16 ? s[0][i + 1] : s[1][i]);
-        const float ot = __shfl_xor(mx, 32, 64);
-        mx = max3(mx, ot, ot);
-        if constexpr (Score<CAP, ALIBI>::PLAIN) mx *= sc.mul;   // scale > 0: the maximum commutes with it
-        const float mn = fmaxf(m, mx);
-        const float ms = mn == -INFINITY ? 0.f : mn;   // nothing visible yet: 2^(-inf - 0) = 0
-        if (__any(mn > m)) {   // the old sums keep their scale where no row's maximum rose
-            const float alpha = exp2_fast(m - ms);
-            l *= alpha;
+            for (int i = 1; i < 16; ++i) mx = max3(mx, s[1][i], i + 1 < 16 ? s[0][i + 1] : s[1][i]);
+            const float ot = __shfl_xor(mx, 32, 64);
+            mx = max3(mx, ot, ot);
+            if constexpr (Score<CAP, ALIBI>::PLAIN) mx *= sc.mul;   // scale > 0: the maximum commutes with it
+            const float mn = fmaxf(m, mx);
+            ms = mn == -INFINITY ? 0.f : mn;   // nothing visible yet: 2^(-inf - 0) = 0
+            if (__any(mn > m)) {   // the old sums keep their scale where no row's maximum rose
+                const float alpha = exp2_fast(m - ms);
+                l *= alpha;
 #pragma unroll
-            for (int i = 0; i < NO; ++i) o[i] *= alpha;
+                for (int i = 0; i < NO; ++i) o[i] *= alpha;
+            }
+            m = mn;
         }
-        m = mn;
         float rs = 0.f;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                s[t][i] = exp2_fast(Score<CAP, ALIBI>::PLAIN ? fmaf(s[t][i], sc.mul, -ms) : s[t][i] - ms);
+                s[t][i] = exp2_fast(Score<CAP, ALIBI>::PLAIN ? fmaf(s[t][i], sc.mul, -ms) : fixed ? s[t][i] : s[t][i] - ms);
                 rs += s[t][i];
             }
         l += rs;   // this half's keys; the halves are added at the end
@@ -345,7 +358,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void mattn_fwd_kernel(const 
                 }
             }
         if (h == 0 && a.lse != nullptr)
-            a.lse[((int64_t)at.b * a.H + at.h) * a.Tq + qi] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
+            a.lse[((int64_t)at.b * a.H + at.h) * a.Tq + qi] = l == 0.f ? -INFINITY : (m + (SAT ? sc.capl : 0.f) + log2f(l)) * LN2;
     }
 }
 
