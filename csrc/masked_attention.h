@@ -341,6 +341,66 @@ struct Tile {
         }
     }
 };
+// The same tile copied from memory straight into LDS: a wave's 64 copies land side by side, so the swizzle
+// is on the memory side (thread t copies the chunk that belongs at place t of the image).  Nothing passes
+// through registers, and a copy is waited for only where its tile is about to be read (landed()).
+template <class T, int DP, int ROWS, int NTHR>
+struct Copy {
+    static constexpr int NCH = DP / 8, RPP = NTHR / NCH, N = ROWS / RPP;
+    static_assert(ROWS % RPP == 0 && RPP % 16 == 0, "whole passes that keep the swizzle");
+    static __device__ __forceinline__ int row(int tid, int j) { return tid / NCH + j * RPP; }
+    static __device__ __forceinline__ int chunk(int tid) { return (tid % NCH) ^ swz_key<DP>(tid / NCH); }
+    uint32_t off, step;
+    __device__ __forceinline__ void init(int64_t ld, int D, int tid) {
+        off = (uint32_t)(row(tid, 0) * ld + (chunk(tid) * 8 < D ? chunk(tid) * 8 : 0)) * 2u;   // (fix zeroes the columns past D)
+        step = (uint32_t)(RPP * ld) * 2u;
+    }
+    // rows r0 .. of `base`, which has `rows`: the lane's offsets are relative to row r0, rows past the
+    // last are out of the resource's range
+    __device__ __forceinline__ void start(bf16_t* img, const bf16_t* base, int64_t ld, int r0, int rows, int D, int w) const {
+        const int left = min(rows - r0, ROWS);
+        const __amdgpu_buffer_rsrc_t b = __builtin_amdgcn_make_buffer_rsrc(
+            (void*)(base + (int64_t)r0 * ld), 0, (uint32_t)((left - 1) * ld + D) * 2u, 0x00020000);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            // (from asm: before a transposed LDS read the compiler waits for every copy it knows of, it cannot
+            // tell the two buffers apart)
+            const uint32_t at = __builtin_amdgcn_readfirstlane(
+                (uint32_t)(size_t)(__attribute__((address_space(3))) bf16_t*)(img + (j * NTHR + w * 64) * 8));
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(off + j * step),
+                         "s"(b) : "memory", "m0");
+        }
+    }
+    // the columns past D, in whose place column 0 was copied
+    static __device__ __forceinline__ void trim(bf16_t* img, int tid, int D) {
+        if (chunk(tid) * 8 >= D)
+#pragma unroll
+            for (int j = 0; j < N; ++j) *(u32x4*)(img + (j * NTHR + tid) * 8) = (u32x4)(0u);
+    }
+    // put_masked of a tile that has landed: each thread mends what it copied
+    static __device__ __forceinline__ void fix(bf16_t* img, int tid, int keep0, int keep1, int D, uint8_t* flags) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int r = row(tid, j), c = chunk(tid);
+            u32x4* p = (u32x4*)(img + (j * NTHR + tid) * 8);
+            u32x4 u = *p;
+            const bool in = r >= keep0 && r < keep1 && c * 8 < D;
+            const bool bad = in && not_finite8<T>(u);
+            if (bad) u = finite_only<T>(u);
+            if (!in) u = (u32x4)(0u);
+            if (bad || !in) *p = u;
+            flags[r * NCH + c] = bad ? 1 : 0;
+        }
+    }
+};
+// all but the newest N of the wave's loads, copies and stores are done
+template <int N>
+__device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(%c0)" ::"n"(N) : "memory"); }
+// barrier that leaves copies in flight (__syncthreads waits for them); LDS reads and writes are done
+__device__ __forceinline__ void barrier_lds() {
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
 // the flagged rows of a tile: bit l set where a chunk of row `row` of lane l was not finite
 template <int DP>
 __device__ __forceinline__ uint64_t flagged_rows(const uint8_t* flags, int row) {

@@ -10,9 +10,9 @@ using namespace mattn;
 
 // ============================================================================ dQ
 template <class T, int DP, bool CAP, bool ALIBI, int NW>
-__global__ __launch_bounds__(64 * NW, DP == 64 ? 8 / NW : 1) void mattn_dq_kernel(const Args a) {
+__global__ __launch_bounds__(64 * NW, 2) void mattn_dq_kernel(const Args a) {
     constexpr int BM = QT * NW, BN = 64, NS = DP / 16, NO = DP / 32, NTHR = 64 * NW;
-    typedef Tile<T, DP, BN, NTHR> TL;
+    typedef Copy<T, DP, BN, NTHR> CP;
     __shared__ __attribute__((aligned(16))) bf16_t Ks[2][BN * DP];
     __shared__ __attribute__((aligned(16))) bf16_t Vs[2][BN * DP];
     __shared__ __attribute__((aligned(16))) uint8_t kflag[2][BN * (DP / 8)];
@@ -93,18 +93,21 @@ __global__ __launch_bounds__(64 * NW, DP == 64 ? 8 / NW : 1) void mattn_dq_kerne
     bool poison = false;
     const int kb0 = bh > bl ? bl / BN : 0, kb1 = bh > bl ? (bh + BN - 1) / BN : 0;
     const int tq = (lane & 15) >> 2, tcol = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-    u32x4 kr[TL::N], vr[TL::N];
-    auto gload = [&](int kb) {
-        TL::load(kr, kbase, a.ks[1], kb * BN, a.Tk - 1, a.D, tid);
-        TL::load(vr, vbase, a.vs[1], kb * BN, a.Tk - 1, a.D, tid);
+    CP kc, vc;
+    kc.init(a.ks[1], a.D, tid);
+    vc.init(a.vs[1], a.D, tid);
+    auto fetch = [&](int kb, int buf) {
+        kc.start(Ks[buf], kbase, a.ks[1], kb * BN, a.Tk, a.D, w);
+        vc.start(Vs[buf], vbase, a.vs[1], kb * BN, a.Tk, a.D, w);
     };
     auto whole = [&](int kb) { return kb * BN >= bfl && (kb + 1) * BN <= bfh && a.D == DP; };
-    auto sstore = [&](int kb, int buf) {
+    auto mend = [&](int kb, int buf) {
         // K meets masked zeros of dX in the last product: a masked key that is not finite is stored as
         // zeros, a visible one makes the row NaN through its flag
-        if (whole(kb)) TL::put(Ks[buf], kr, tid);
-        else TL::put_masked(Ks[buf], kr, tid, bl - kb * BN, bh - kb * BN, a.D, kflag[buf]);
-        TL::put(Vs[buf], vr, tid);
+        landed<0>();
+        if (whole(kb)) return;
+        if (a.D != DP) CP::trim(Vs[buf], tid, a.D);
+        CP::fix(Ks[buf], tid, bl - kb * BN, bh - kb * BN, a.D, kflag[buf]);
     };
     auto compute = [&](int kb, int buf) {
         if (kb * BN >= wh || (kb + 1) * BN <= wl) return;
@@ -157,17 +160,15 @@ __global__ __launch_bounds__(64 * NW, DP == 64 ? 8 / NW : 1) void mattn_dq_kerne
         }
     };
     if (kb0 < kb1) {
-        gload(kb0);
-        sstore(kb0, 0);
-        __syncthreads();
+        fetch(kb0, 0);
+        mend(kb0, 0);
     }
     for (int kb = kb0; kb < kb1; ++kb) {
         const int buf = (kb - kb0) & 1;
-        const bool next = kb + 1 < kb1;
-        if (next) gload(kb + 1);
+        barrier_lds();   // tile kb is complete, the other buffer has been read
+        if (kb + 1 < kb1) fetch(kb + 1, buf ^ 1);
         compute(kb, buf);
-        if (next) sstore(kb + 1, buf ^ 1);
-        __syncthreads();
+        if (kb + 1 < kb1) mend(kb + 1, buf ^ 1);
     }
     const float gscale = CAP ? 4.f * a.scale : a.scale;   // (with the 4 of the cap's derivative)
     if (qi < a.Tq) {

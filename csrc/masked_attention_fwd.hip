@@ -164,7 +164,7 @@ TDL_API int tdl_attn_mask(const void* documents, int wide, const int* prefix_row
 template <class T, int DP, bool CAP, bool ALIBI>
 __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void mattn_fwd_kernel(const Args a) {
     constexpr int NW = 4, BM = QT * NW, BN = 64, NS = DP / 16, NO = DP / 32, NTHR = 64 * NW;
-    typedef Tile<T, DP, BN, NTHR> TL;
+    typedef Copy<T, DP, BN, NTHR> CP;
     __shared__ __attribute__((aligned(16))) bf16_t Ks[2][BN * DP];
     __shared__ __attribute__((aligned(16))) bf16_t Vs[2][BN * DP];
     __shared__ __attribute__((aligned(16))) uint8_t vflag[2][BN * (DP / 8)];
@@ -223,20 +223,19 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void mattn_fwd_kernel(const 
     const int kb0 = bh > bl ? bl / BN : 0, kb1 = bh > bl ? (bh + BN - 1) / BN : 0;
     const int tq = (lane & 15) >> 2, tcol = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
 
-    u32x4 kr[TL::N], vr[TL::N];
-    auto gload = [&](int kb) {
-        TL::load(kr, kbase, a.ks[1], kb * BN, a.Tk - 1, a.D, tid);
-        TL::load(vr, vbase, a.vs[1], kb * BN, a.Tk - 1, a.D, tid);
+    CP kc, vc;
+    kc.init(a.ks[1], a.D, tid);
+    vc.init(a.vs[1], a.D, tid);
+    auto fetch = [&](int kb, int buf) {
+        kc.start(Ks[buf], kbase, a.ks[1], kb * BN, a.Tk, a.D, w);
+        vc.start(Vs[buf], vbase, a.vs[1], kb * BN, a.Tk, a.D, w);
     };
-    auto whole = [&](int kb) { return kb * BN >= bfl && (kb + 1) * BN <= bfh; };   // seen by every row
-    auto sstore = [&](int kb, int buf) {
-        if (whole(kb) && a.D == DP) {
-            TL::put(Ks[buf], kr, tid);
-            TL::put(Vs[buf], vr, tid);
-        } else {
-            TL::put(Ks[buf], kr, tid);   // a masked key's score is replaced, whatever it was
-            TL::put_masked(Vs[buf], vr, tid, bl - kb * BN, bh - kb * BN, a.D, vflag[buf]);
-        }
+    auto whole = [&](int kb) { return kb * BN >= bfl && (kb + 1) * BN <= bfh && a.D == DP; };   // seen by every row
+    auto mend = [&](int kb, int buf) {   // (a masked key's score is replaced, whatever it was; columns past D are not)
+        landed<0>();
+        if (whole(kb)) return;
+        if (a.D != DP) CP::trim(Ks[buf], tid, a.D);
+        CP::fix(Vs[buf], tid, bl - kb * BN, bh - kb * BN, a.D, vflag[buf]);
     };
     auto compute = [&](int kb, int buf) {
         if (kb * BN >= wh || (kb + 1) * BN <= wl) return;
@@ -298,7 +297,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void mattn_fwd_kernel(const 
                 rs += s[t][i];
             }
         l += rs;   // this half's keys; the halves are added at the end
-        if (!whole(kb) || a.D != DP) {
+        if (!whole(kb)) {
             uint64_t bad = flagged_rows<DP>(vflag[buf], lane);
             while (bad != 0) {
                 const int k = kb * BN + __builtin_ctzll(bad);
@@ -317,21 +316,15 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void mattn_fwd_kernel(const 
             }
     };
     if (kb0 < kb1) {
-        gload(kb0);
-        sstore(kb0, 0);
-        __syncthreads();
+        fetch(kb0, 0);
+        mend(kb0, 0);
     }
-    // the Q fragments land before the loop (else their loads sink into its first tile, and a wait for
-    // them drains the K / V prefetch)
-#pragma unroll
-    for (int s = 0; s < NS; ++s) asm volatile("" ::"v"(qf[s]));
     for (int kb = kb0; kb < kb1; ++kb) {
         const int buf = (kb - kb0) & 1;
-        const bool next = kb + 1 < kb1;
-        if (next) gload(kb + 1);
+        barrier_lds();   // tile kb is complete, the other buffer has been read
+        if (kb + 1 < kb1) fetch(kb + 1, buf ^ 1);
         compute(kb, buf);
-        if (next) sstore(kb + 1, buf ^ 1);
-        __syncthreads();
+        if (kb + 1 < kb1) mend(kb + 1, buf ^ 1);
     }
     l += __shfl_xor(l, 32, 64);
     if (qi < a.Tq) {
