@@ -341,6 +341,9 @@ struct Tile {
         }
     }
 };
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+    return __builtin_amdgcn_readfirstlane((uint32_t)(size_t)(const __attribute__((address_space(3))) char*)p);
+}
 // The same tile copied from memory straight into LDS: a wave's 64 copies land side by side, so the swizzle
 // is on the memory side (thread t copies the chunk that belongs at place t of the image).  Nothing passes
 // through registers, and a copy is waited for only where its tile is about to be read (landed()).
@@ -355,18 +358,16 @@ struct Copy {
         off = (uint32_t)(row(tid, 0) * ld + (chunk(tid) * 8 < D ? chunk(tid) * 8 : 0)) * 2u;   // (fix zeroes the columns past D)
         step = (uint32_t)(RPP * ld) * 2u;
     }
-    // rows r0 .. of `base`, which has `rows`: the lane's offsets are relative to row r0, rows past the
-    // last are out of the resource's range
-    __device__ __forceinline__ void start(bf16_t* img, const bf16_t* base, int64_t ld, int r0, int rows, int D, int w) const {
-        const int left = min(rows - r0, ROWS);
+    // ROWS rows from `first`, of which `left` exist (those past the last are out of the resource's range), to
+    // LDS address img; w: the wave's number
+    __device__ __forceinline__ void start(uint32_t img, const bf16_t* first, int64_t ld, int left, int D, int w) const {
         const __amdgpu_buffer_rsrc_t b = __builtin_amdgcn_make_buffer_rsrc(
-            (void*)(base + (int64_t)r0 * ld), 0, (uint32_t)((left - 1) * ld + D) * 2u, 0x00020000);
+            (void*)first, 0, (uint32_t)((min(left, ROWS) - 1) * (uint32_t)ld + D) * 2u, 0x00020000);
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             // (from asm: before a transposed LDS read the compiler waits for every copy it knows of, it cannot
             // tell the two buffers apart)
-            const uint32_t at = __builtin_amdgcn_readfirstlane(
-                (uint32_t)(size_t)(__attribute__((address_space(3))) bf16_t*)(img + (j * NTHR + w * 64) * 8));
+            const uint32_t at = __builtin_amdgcn_readfirstlane(img + (j * NTHR + w * 64) * 16);
             asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(off + j * step),
                          "s"(b) : "memory", "m0");
         }

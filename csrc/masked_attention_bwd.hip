@@ -96,9 +96,14 @@ __global__ __launch_bounds__(64 * NW, 2) void mattn_dq_kernel(const Args a) {
     CP kc, vc;
     kc.init(a.ks[1], a.D, tid);
     vc.init(a.vs[1], a.D, tid);
-    auto fetch = [&](int kb, int buf) {
-        kc.start(Ks[buf], kbase, a.ks[1], kb * BN, a.Tk, a.D, w);
-        vc.start(Vs[buf], vbase, a.vs[1], kb * BN, a.Tk, a.D, w);
+    const uint32_t kat = lds_address(Ks), vat = lds_address(Vs);
+    const bf16_t *kp = kbase + (int64_t)kb0 * BN * a.ks[1], *vp = vbase + (int64_t)kb0 * BN * a.vs[1];   // next to copy
+    const int64_t kstep = BN * a.ks[1], vstep = BN * a.vs[1];
+    auto fetch = [&](int kb, int buf) {   // kb0, then one after the other
+        kc.start(kat + buf * (BN * DP * 2), kp, a.ks[1], a.Tk - kb * BN, a.D, w);
+        vc.start(vat + buf * (BN * DP * 2), vp, a.vs[1], a.Tk - kb * BN, a.D, w);
+        kp += kstep;
+        vp += vstep;
     };
     auto whole = [&](int kb) { return kb * BN >= bfl && (kb + 1) * BN <= bfh && a.D == DP; };
     auto mend = [&](int kb, int buf) {
@@ -130,8 +135,6 @@ __global__ __launch_bounds__(64 * NW, 2) void mattn_dq_kernel(const Args a) {
                 p = T::mfma(as_vec<T>(*(const u32x4*)(V_ + at_)), df[d], p);
             }
             const float d0 = ALIBI ? (float)(kb * BN + 32 * t + 4 * h) - qpos : 0.f;
-            const int k0 = kb * BN + 32 * t + 4 * h - lo;
-            const uint32_t n = (uint32_t)(hi - lo);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int kk = (i & 3) + 8 * (i >> 2);
@@ -146,9 +149,14 @@ __global__ __launch_bounds__(64 * NW, 2) void mattn_dq_kernel(const Args a) {
                 } else {
                     e = exp2_fast(sc(s[i], d0 + (float)kk) - lse2);
                 }
-                e *= x;
-                if (part) e = (uint32_t)(k0 + kk) < n ? e : 0.f;
-                s[i] = e;
+                s[i] = e * x;
+            }
+            if (part) {
+                asm volatile("" : "+v"(s));   // (a branch, and not 3 instructions a score in every tile)
+                const int k0 = kb * BN + 32 * t + 4 * h - lo;
+                const uint32_t n = (uint32_t)(hi - lo);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[i] = (uint32_t)(k0 + (i & 3) + 8 * (i >> 2)) < n ? s[i] : 0.f;
             }
 #pragma unroll
             for (int s2 = 0; s2 < 2; ++s2) {
@@ -195,13 +203,13 @@ __global__ __launch_bounds__(64 * NW, 2) void mattn_dq_kernel(const Args a) {
 // and C, and the registers (accumulators of 2 x DP x 32, fragments of K and V) leave only one or two
 // waves per SIMD to fill in for it.  So the loop is pipelined in the wave: an iteration
 // interleaves C(t - 1), B(t) and A(t + 1), two scores between every few products, each product's LDS
-// fragment read two products ahead.  Four tiles of Q / dO are in LDS (t - 1 .. t + 1, and t + 2
-// arriving), two more in registers on their way there; one barrier per tile.
+// fragment read two products ahead.  Eight places for tiles of Q / dO are in LDS: t - 1 .. t + 1 are
+// read, t + 2 .. t + 4 are on their way (copies straight from memory); one barrier per tile.
 template <class T, int DP, bool CAP, bool ALIBI>
 __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void mattn_dkdv_kernel(const Args a) {
-    constexpr int NS = DP / 16, NO = DP / 32, RING = 4;
+    constexpr int NS = DP / 16, NO = DP / 32, RING = 8;
     constexpr int NA = 2 * NS, NC = 4 * NO, STEPS = 8, AS = NA / STEPS, CS = NC / STEPS, AHEAD = 2;
-    typedef Tile<T, DP, QT, 256> TL;
+    typedef Copy<T, DP, QT, 256> CP;
     typedef typename T::vec vec;
     constexpr int IMG = QT * DP;
     __shared__ __attribute__((aligned(16))) bf16_t tiles[RING][2 * IMG];   // Q, then dO
@@ -251,60 +259,67 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void mattn_dkdv_kernel(const
             ++x.g;
         }
     };
-    // a tile on its way: this thread's pieces of Q and dO, its row constant (threads 0 .. 127: one of the
-    // four kinds of one row) and its word of the tile's qtab entry
-    struct Coming {
-        u32x4 q[TL::N], d[TL::N];
-        uint32_t rc, tab;
-    };
-    const int kind = (tid >> 5) & 3, rrow = tid & 31, tp = nq * QT;
+    // this lane's word of a tile's row constants (waves 2 and 3 copy what 0 and 1 do: every wave has the
+    // same number of copies in flight)
+    const int kind = 2 * (w & 1) + h, tp = nq * QT;
     const uint32_t* rbase = kind < 2 ? (const uint32_t*)a.delta + (((int64_t)b * a.H + hk * G) * 2 + kind) * tp
                                      : (const uint32_t*)(kind == 2 ? a.lo : a.hi) + (int64_t)b * a.Tq;
-    const int64_t rhead = kind < 2 ? 2 * tp : 0;
-    const int rlast = kind < 2 ? tp - 1 : a.Tq - 1;
-    const uint32_t* tbase = (const uint32_t*)(a.qtab + (int64_t)b * nq) + (tid & 3);
-    // a tile's rows through a buffer resource that starts at its first row: the lane's offsets never change,
-    // and rows past the tensor (and columns past D, offset 2^31) read as zeros
-    uint32_t qoff[TL::N], doff[TL::N];
-#pragma unroll
-    for (int i = 0; i < TL::N; ++i) {
-        const bool in = TL::chunk(tid) * 8 < a.D;
-        qoff[i] = in ? (uint32_t)(TL::row(tid, i) * a.qs[1] + TL::chunk(tid) * 8) * 2u : 0x80000000u;
-        doff[i] = in ? (uint32_t)(TL::row(tid, i) * a.dos[1] + TL::chunk(tid) * 8) * 2u : 0x80000000u;
-    }
-    auto rows_of = [&](const bf16_t* base, int64_t ld, int t) __attribute__((always_inline)) {
-        const int left = a.Tq - t * QT;
-        const uint32_t n = left >= QT ? 0x7fffffffu : (uint32_t)((left - 1) * ld + a.D) * 2u;
-        return __builtin_amdgcn_make_buffer_rsrc((void*)(base + (int64_t)t * QT * ld), 0, n, 0x00020000);
-    };
-    auto gload = [&](const At& x, Coming& c) __attribute__((always_inline)) {
-        const __amdgpu_buffer_rsrc_t qb = rows_of(qbase + x.g * a.qs[2], a.qs[1], x.t);
-        const __amdgpu_buffer_rsrc_t db_ = rows_of(dbase + x.g * a.dos[2], a.dos[1], x.t);
-#pragma unroll
-        for (int i = 0; i < TL::N; ++i) {
-            c.q[i] = __builtin_amdgcn_raw_buffer_load_b128(qb, qoff[i], 0, 0);
-            c.d[i] = __builtin_amdgcn_raw_buffer_load_b128(db_, doff[i], 0, 0);
+    const int rhead = kind < 2 ? 2 * tp : 0, rlast = kind < 2 ? tp - 1 : a.Tq - 1;
+    CP qc, dc;
+    qc.init(a.qs[1], a.D, tid);
+    dc.init(a.dos[1], a.D, tid);
+    constexpr int COPIES = 2 * CP::N + 1;   // a tile's, per wave
+    const uint32_t tat = lds_address(tiles), rat = lds_address(rowc) + 256 * (w & 1);
+    // the next tile to copy: the first rows, and how far to the next tile and from a head's last to the next head
+    const bf16_t *qp = qbase + (int64_t)range.x * QT * a.qs[1], *dp = dbase + (int64_t)range.x * QT * a.dos[1];
+    const uint32_t* rp = rbase;
+    const int64_t qstep = QT * a.qs[1], dstep = QT * a.dos[1];
+    const int64_t qhead = a.qs[2] - (range.y - range.x) * qstep, dhead = a.dos[2] - (range.y - range.x) * dstep;
+    auto fetch = [&](At& x, int buf) __attribute__((always_inline)) {
+        const int left = a.Tq - x.t * QT;
+        qc.start(tat + buf * (4 * IMG), qp, a.qs[1], left, a.D, w);
+        dc.start(tat + buf * (4 * IMG) + 2 * IMG, dp, a.dos[1], left, a.D, w);
+        const uint32_t* p = rp + min(x.t * QT + r, rlast);
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(rat + buf * (16 * QT)), "v"(p) : "memory", "m0");
+        qp += qstep;
+        dp += dstep;
+        if (++x.t == range.y) {
+            x.t = range.x;
+            ++x.g;
+            qp += qhead;
+            dp += dhead;
+            rp += rhead;
         }
-        c.rc = rbase[x.g * rhead + min(x.t * QT + rrow, rlast)];
-        c.tab = tbase[4 * x.t];
     };
-    // the qtab entry of a tile, in scalar registers (lanes 0 .. 3 hold its words)
     struct Bounds {
         int lo, hi, full_lo, full_hi;   // some row sees [lo, hi), every row sees [full_lo, full_hi)
     };
-    auto sstore = [&](const At& x, const Coming& c, int buf) __attribute__((always_inline)) {
-        const Bounds e{__builtin_amdgcn_readlane((int)c.tab, 0), __builtin_amdgcn_readlane((int)c.tab, 1),
-                       __builtin_amdgcn_readlane((int)c.tab, 2), __builtin_amdgcn_readlane((int)c.tab, 3)};
-        if (e.full_lo <= kbi * KT && e.full_hi >= (kbi + 1) * KT && a.D == DP) {   // every key of the block is seen by every row
-            TL::put(tiles[buf], c.q, tid);
-            TL::put(tiles[buf] + IMG, c.d, tid);
-        } else {
-            TL::put_masked(tiles[buf], c.q, tid, 0, a.Tq - x.t * QT, a.D, qflag[buf]);   // (as K in dQ)
-            TL::put_masked(tiles[buf] + IMG, c.d, tid, 0, a.Tq - x.t * QT, a.D, dflag[buf]);
+    // 64 entries of the table at a time stand in the wave's lanes (a scalar load in the loop would be waited
+    // for by the next LDS read)
+    int part_of_tab = -1;
+    int4 tab;
+    auto bounds = [&](const At& x) __attribute__((always_inline)) {
+        const int i = x.t - range.x;
+        if (i >> 6 != part_of_tab) {
+            part_of_tab = i >> 6;
+            tab = a.qtab[(int64_t)b * nq + min(x.t - (i & 63) + lane, nq - 1)];
+            // (waited for here: a load that might be pending at the loop's head would be waited for there in
+            // every iteration, and with it every copy in flight)
+            asm volatile("" : "+v"(tab.x), "+v"(tab.y), "+v"(tab.z), "+v"(tab.w));
         }
-        // (a row past the last sees nothing)
-        if (tid < 4 * QT) rowc[buf][tid] = kind >= 2 && x.t * QT + rrow >= a.Tq ? 0 : c.rc;
-        return e;
+        return Bounds{__builtin_amdgcn_readlane(tab.x, i & 63), __builtin_amdgcn_readlane(tab.y, i & 63),
+                      __builtin_amdgcn_readlane(tab.z, i & 63), __builtin_amdgcn_readlane(tab.w, i & 63)};
+    };
+    // every key of the block is seen by every row of a tile
+    auto whole = [&](const At& x, const Bounds& e) {
+        return e.full_lo <= kbi * KT && e.full_hi >= (kbi + 1) * KT && a.D == DP && (x.t + 1) * QT <= a.Tq;
+    };
+    // of a tile that has landed: the rows past the last are zeros, so whatever their constants say they
+    // add nothing (lse log2(e) is padded with zeros)
+    auto mend = [&](const At& x, const Bounds& e, int buf) __attribute__((always_inline)) {
+        if (whole(x, e)) return;
+        CP::fix(tiles[buf], tid, 0, a.Tq - x.t * QT, a.D, qflag[buf]);   // (as K in dQ)
+        CP::fix(tiles[buf] + IMG, tid, 0, a.Tq - x.t * QT, a.D, dflag[buf]);
     };
     auto active = [&](const Bounds& e) { return e.lo < k0 + 32 && e.hi > k0; };   // some row sees a key of the wave
 
@@ -366,7 +381,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void mattn_dkdv_kernel(const
                 }
             }
         }
-        if (part || a.D != DP) {   // a query that is not finite: NaN for the keys it sees
+        if (!whole(x, bnd)) {   // a query that is not finite: NaN for the keys it sees
             uint32_t bad = (uint32_t)flagged_rows<DP>(qflag[buf], r);
             while (bad != 0) {
                 const int q = __builtin_ctz(bad);
@@ -444,63 +459,68 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void mattn_dkdv_kernel(const
     constexpr std::true_type Y{};
     constexpr std::false_type N{};
 
-    At ld{0, range.x}, st{0, range.x}, cur{0, range.x};
-    Coming c0, c1;
+    At ld{0, range.x}, tb{0, range.x}, st{0, range.x}, cur{0, range.x};   // next to copy, to look up, to mend; tile t
     Scores y0, y1;
     Bounds e0{0, 0, 0, 0}, e1{0, 0, 0, 0}, e2{0, 0, 0, 0};   // of tiles t, t + 1, t + 2
     bool acc_ = false;   // tile t - 1 has work for this wave
 #pragma unroll
     for (int i = 0; i < 2; ++i) pb[i] = db[i] = as_vec<T>((u32x4)(0u));
-    auto load_next = [&](Coming& c) __attribute__((always_inline)) {
-        if (ld.g < G) {
-            gload(ld, c);
-            advance(ld);
-        }
-    };
-    auto store_next = [&](const Coming& c, int buf) __attribute__((always_inline)) {
-        Bounds e{0, 0, 0, 0};   // past the last tile: no work
-        if (st.g < G) {
-            e = sstore(st, c, buf);
-            advance(st);
-        }
+    auto look_up = [&]() __attribute__((always_inline)) {   // past the last tile: no work
+        Bounds e{0, 0, 0, 0};
+        if (tb.g < G) e = bounds(tb);
+        advance(tb);
         return e;
     };
+    auto copy_next = [&](int t) __attribute__((always_inline)) {
+        if (t < total) fetch(ld, t & (RING - 1));
+    };
+    // tile t is complete but for the barrier; tiles up to t + 2 may be on their way
+    auto await = [&](int t, const Bounds& e) __attribute__((always_inline)) {
+        if (t >= total) return;
+        if (t + 2 < total) landed<2 * COPIES>();
+        else landed<0>();
+        mend(st, e, t & (RING - 1));
+        advance(st);
+    };
     if (total > 0) {
-        // slot 3 stands for tile -1: finite values for the weights 0 of the first C
-        for (int i = tid; i < 2 * IMG / 8; i += 256) ((u32x4*)tiles[3])[i] = (u32x4)(0u);
-        load_next(c0);
-        load_next(c1);
-        e0 = store_next(c0, 0);
-        e1 = store_next(c1, 1);
-        load_next(c0);
-        load_next(c1);
-        __syncthreads();
+        // the last place stands for tile -1: finite values for the weights 0 of the first C
+        for (int i = tid; i < 2 * IMG / 8; i += 256) ((u32x4*)tiles[RING - 1])[i] = (u32x4)(0u);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) copy_next(i);
+        e0 = look_up();
+        e1 = look_up();
+        e2 = look_up();
+        await(0, e0);
+        await(1, e1);
+        barrier_lds();
         run(N, N, Y, cur, e0, y1, y0, 0, 0, 0);
     }
-    // tile t: its scores in y, the next tile's in yn; tile t + 2 arrives from c, tile t + 4 is asked for
-    auto iter = [&](int t, Coming& c, Scores& y, Scores& yn) __attribute__((always_inline)) {
-        e2 = store_next(c, (t + 2) & 3);
-        load_next(c);
+    // tile t: its scores in y, the next tile's in yn
+    auto iter = [&](int t, Scores& y, Scores& yn) __attribute__((always_inline)) {
+        copy_next(t + 4);
+        const Bounds e3 = look_up();
         const bool act = active(e0);
         // a tile without work inside the pipeline counts with weights 0 (its masks leave nothing); the
         // products of a tile past the last are not used
         if (acc_ || act || active(e1)) {
-            run(Y, Y, Y, cur, e0, y, yn, (t - 1) & 3, t & 3, (t + 1) & 3);
+            run(Y, Y, Y, cur, e0, y, yn, (t - 1) & (RING - 1), t & (RING - 1), (t + 1) & (RING - 1));
         } else {
 #pragma unroll
             for (int i = 0; i < 2; ++i) pb[i] = db[i] = as_vec<T>((u32x4)(0u));
         }
+        await(t + 2, e2);
         acc_ = act;
         e0 = e1;
         e1 = e2;
+        e2 = e3;
         advance(cur);
-        __syncthreads();
+        barrier_lds();
     };
     for (int t = 0; t < total; t += 2) {
-        iter(t, c0, y0, y1);
-        if (t + 1 < total) iter(t + 1, c1, y1, y0);
+        iter(t, y0, y1);
+        if (t + 1 < total) iter(t + 1, y1, y0);
     }
-    if (total > 0) run(Y, N, N, cur, e0, y0, y1, (total - 1) & 3, 0, 0);
+    if (total > 0) run(Y, N, N, cur, e0, y0, y1, (total - 1) & (RING - 1), 0, 0);
     if constexpr (DP == 128) acc_done(dk, dv);
     const float gscale = CAP ? 4.f * a.scale : a.scale;
     if (kj < a.Tk) {

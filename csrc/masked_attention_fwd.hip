@@ -226,9 +226,14 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void mattn_fwd_kernel(const 
     CP kc, vc;
     kc.init(a.ks[1], a.D, tid);
     vc.init(a.vs[1], a.D, tid);
-    auto fetch = [&](int kb, int buf) {
-        kc.start(Ks[buf], kbase, a.ks[1], kb * BN, a.Tk, a.D, w);
-        vc.start(Vs[buf], vbase, a.vs[1], kb * BN, a.Tk, a.D, w);
+    const uint32_t kat = lds_address(Ks), vat = lds_address(Vs);
+    const bf16_t *kp = kbase + (int64_t)kb0 * BN * a.ks[1], *vp = vbase + (int64_t)kb0 * BN * a.vs[1];   // next to copy
+    const int64_t kstep = BN * a.ks[1], vstep = BN * a.vs[1];
+    auto fetch = [&](int kb, int buf) {   // kb0, then one after the other
+        kc.start(kat + buf * (BN * DP * 2), kp, a.ks[1], a.Tk - kb * BN, a.D, w);
+        vc.start(vat + buf * (BN * DP * 2), vp, a.vs[1], a.Tk - kb * BN, a.D, w);
+        kp += kstep;
+        vp += vstep;
     };
     auto whole = [&](int kb) { return kb * BN >= bfl && (kb + 1) * BN <= bfh && a.D == DP; };   // seen by every row
     auto mend = [&](int kb, int buf) {   // (a masked key's score is replaced, whatever it was; columns past D are not)
