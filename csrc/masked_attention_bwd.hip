@@ -35,26 +35,32 @@ __global__ __launch_bounds__(64 * NW, 2) void mattn_dq_kernel(const Args a) {
     const uint32_t* rest = a.rest + (((int64_t)at.b * a.Tq + qc) * a.H + at.h) * a.D / 4;
     typename T::vec qf[NS], df[NS];
     float delta = 0.f;
+    u32x4 du[NS], ou[NS];
+    uint2 rw[NS];
 #pragma unroll
-    for (int s = 0; s < NS; ++s) {
+    for (int s = 0; s < NS; ++s) {   // every load on its way before the first is waited for
         const int c = 16 * s + 8 * h, cc = c < a.D ? c : 0;
-        const u32x4 z = (u32x4)(0u);
-        const u32x4 qu = *(const u32x4*)(qrow + cc), du = *(const u32x4*)(drow + cc), ou = *(const u32x4*)(orow + cc);
+        const u32x4 z = (u32x4)(0u), qu = *(const u32x4*)(qrow + cc);
+        du[s] = *(const u32x4*)(drow + cc);
+        ou[s] = *(const u32x4*)(orow + cc);
+        rw[s] = *(const uint2*)(rest + cc / 4);
         qf[s] = as_vec<T>(c < a.D ? qu : z);
-        df[s] = as_vec<T>(c < a.D ? du : z);
-        if (c < a.D) {
-            const uint2 rw = *(const uint2*)(rest + cc / 4);
-            float rv[8];
-            Rest<T>::back(rw.x, *(float(*)[4])rv);
-            Rest<T>::back(rw.y, *(float(*)[4])(rv + 4));
+        du[s] = c < a.D ? du[s] : z;
+        ou[s] = c < a.D ? ou[s] : z;
+        df[s] = as_vec<T>(du[s]);
+    }
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                float d0, d1, o0, o1;
-                T::unpack(du[k], d0, d1);
-                T::unpack(ou[k], o0, o1);
-                delta = fmaf(d0, o0 + rv[2 * k], delta);
-                delta = fmaf(d1, o1 + rv[2 * k + 1], delta);
-            }
+    for (int s = 0; s < NS; ++s) {   // (past D: 0 times 0 plus a finite remainder)
+        float rv[8];
+        Rest<T>::back(rw[s].x, *(float(*)[4])rv);
+        Rest<T>::back(rw[s].y, *(float(*)[4])(rv + 4));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            float d0, d1, o0, o1;
+            T::unpack(du[s][k], d0, d1);
+            T::unpack(ou[s][k], o0, o1);
+            delta = fmaf(d0, o0 + rv[2 * k], delta);
+            delta = fmaf(d1, o1 + rv[2 * k + 1], delta);
         }
     }
     delta += __shfl_xor(delta, 32, 64);
