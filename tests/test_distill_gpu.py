@@ -5,6 +5,7 @@ distance d from the row's maximum (inputs here: d < 2^5 in units of log 2), of t
 at most 2^5 additions a thread) and a few roundings: 2^-17 relative covers them with a factor to spare.
 dz is rounded once to the logits' type, u = eps / 2.  The loss is a mean of such terms: 2^-17 of the mean of
 their magnitudes."""
+import contextlib
 import math
 
 import pytest
@@ -169,6 +170,31 @@ def test_second_backward_and_shared_logits():
         z2.add_(1)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("upstream", [1.0, 3.0])
+def test_tensors_saved_elsewhere(dtype, upstream):
+    """Saved-tensor hooks bring the logits back with other strides than the forward saw: the same gradient."""
+    from trustworthy_dl import ops
+    M, W, K = 37, 1003, 9
+    base = torch.randn(M, W + 6, generator=torch.Generator(device=DEV).manual_seed(5), device=DEV).to(dtype)
+    index = torch.randint(0, W, (M, K), generator=torch.Generator(device=DEV).manual_seed(6), device=DEV)
+    teacher = torch.randn(M, K, generator=torch.Generator(device=DEV).manual_seed(7), device=DEV)
+    labels = torch.randint(0, W, (M,), generator=torch.Generator(device=DEV).manual_seed(8), device=DEV)
+
+    def grad(hooks):
+        z = base.clone().requires_grad_(True)
+        part = z[:, 3:3 + W]
+        with hooks:
+            loss = ops.distillation_loss(part, index, teacher, labels, temperature=2.0, alpha=0.4)
+        return torch.autograd.grad(loss, z, torch.tensor(upstream, device=DEV))[0]
+    want = grad(contextlib.nullcontext())
+    got = grad(torch.autograd.graph.save_on_cpu())
+    # pieces of a row start elsewhere, so sums over a row are taken in another order: both are within the
+    # rounding u of one value and 2^-20 of the row's sums (V terms of 2^-24) apart
+    u = torch.finfo(dtype).eps / 2
+    assert ((want.double() - got.double()).abs() <= 2 * u * want.double().abs() + 2.0 ** -20 * want.double().abs().max()).all()
 
 
 def test_no_gradient_wanted():

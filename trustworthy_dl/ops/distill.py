@@ -37,7 +37,14 @@ def _grad_like(z: torch.Tensor) -> torch.Tensor:
     per = 16 // z.element_size()
     ld = W + (z.stride(0) - W) % per if M > 1 else W
     skew = z.data_ptr() % 16 // z.element_size()
+    if skew == 0:
+        return torch.empty_strided((M, W), (ld, 1), dtype=z.dtype, device=z.device)
     return torch.empty(M * ld + skew, dtype=z.dtype, device=z.device)[skew:].as_strided((M, W), (ld, 1), skew)
+
+
+def _alike(z: torch.Tensor, grad: torch.Tensor) -> bool:
+    """``grad`` stands to the logits as _grad_like makes it."""
+    return (z.data_ptr() - grad.data_ptr()) % 16 == 0 and (z.stride(0) - grad.stride(0)) * z.element_size() % 16 == 0
 
 
 def _launch(z, index, teacher, labels, V, tau, alpha, counts, grad=None, rows=None, loss=None, gscale=None, written=False):
@@ -73,7 +80,9 @@ class _Distill(torch.autograd.Function):
     def backward(ctx, g):
         z, index, teacher, labels, counts = ctx.saved_tensors
         grad, ctx.grad = ctx.grad, None
-        written = grad is not None   # else a second backward through the same node: its own buffer
+        # a second backward through the same node gets its own buffer, and so do logits that saved-tensor
+        # hooks brought back with other rows
+        written = grad is not None and _alike(z, grad)
         if not written:
             grad = _grad_like(z)
         _launch(z, index, teacher, labels, *ctx.how, counts, grad=grad, gscale=g, written=written)
