@@ -243,8 +243,8 @@ __device__ __forceinline__ int wave_max_i(int v) {
 }
 
 // Scores in units of log 2 (the softmax is taken with 2^x).  tanh u = 1 - 2 / (1 + e^(2 u)): exact to
-// 2^-23 of 1 from v_exp and v_rcp, so of a capped score to cap x 2^-23 (the op takes cap <= 1000:
-// 2^-13, below the rounding of a 16-bit probability), and it saturates without overflow.
+// 2^-22 of 1 from v_exp and v_rcp, so of a capped score to cap x 2^-21 (the op takes cap <= 1000:
+// 2^-11, the rounding of an fp16 probability), and it saturates without overflow.
 template <bool CAP, bool ALIBI>
 struct Score {
     static constexpr bool PLAIN = !CAP && !ALIBI;

@@ -5,9 +5,13 @@ is done in 32 bits (scores of magnitude < 2^7 in units of log 2: their products,
 the exponential, the sums over keys: each a few 2^-24 of the magnitudes, times that magnitude).
   out   P is rounded once (u) before its product, the result once:  (2 u + 2 d) sum_j P |v|
   dV    likewise                                                   (2 u + 2 d) sum_i P |dO|
-  delta from the rounded out:  e_i = sum_c |dO| (2 u + 2 d) sum_j P |v|
+  delta from out (the bound allows it the error of the rounded one):  e_i = sum_c |dO| (2 u + 2 d) sum_j P |v|
   dS    rounded once: |error| <= (u + d) |dS| + P (e_i + d (sum_c |dO| |v| + |delta|)), so
   dQ    scale sum_j error |k| + (u + d) |dQ|;   dK   scale sum_i error |q| + (u + d) |dK|
+fp16 also has a smallest step, 2^-24: a P below 2^-14 is off by up to 2^-25 however small it is (forward: of
+a row whose largest is 1 and whose sum is at least 1), which adds 2^-25 sum |v| to out over the visible keys
+and 2^-25 sum |dO| to dV.  dS is rounded times 2^n with 2^n max|dO| in [2^4, 2^5), with a cap as a quarter (the derivative r (1 - r) without its 4):
+an absolute error of 2^-25 max|dO| / 16 (x 4 with a cap) per visible pair.
 With a cap, dS carries the factor 1 - tanh^2 = 4 r (1 - r), exact to a few 2^-24: within d.
 """
 import math
@@ -65,24 +69,27 @@ def run(q, k, v, seen, first, scale, cap=0.0, slopes=None, dout=None):
     P = torch.where(seen, torch.exp(s - lse[..., None]), 0.0)
     out = P @ V
     A = P @ V.abs()
-    res = {"out": (out.transpose(1, 2), ((2 * u + 2 * d) * A).transpose(1, 2)), "lse": lse}
+    step = 2.0 ** -25 if q.dtype == torch.float16 else 0.0
+    tiny = step * (seen.double() @ V.abs())
+    res = {"out": (out.transpose(1, 2), ((2 * u + 2 * d) * A + tiny).transpose(1, 2)), "lse": lse}
     if dout is None:
         return res
     dO = dout.detach().double().transpose(1, 2)
     delta = (dO * out).sum(-1, keepdim=True)
     dP = dO @ V.transpose(-1, -2)
     dS = P * (dP - delta)
-    e = (dO.abs() * A).sum(-1, keepdim=True) * (2 * u + 2 * d)
+    e = (dO.abs() * ((2 * u + 2 * d) * A + tiny)).sum(-1, keepdim=True)
     err = (u + d) * dS.abs() + P * (e + d * (dO.abs() @ V.abs().transpose(-1, -2) + delta.abs()))
     if cap:
         dS, err = dS * (1 - t * t), err * (1 - t * t) + d * dS.abs() * 2.0 ** -6
+    err = err + seen * (step / 16 * (4 if cap else 1) * float(dO.abs().max()))
 
     def heads(t):   # sum over the query heads of a group
         return t.view(B, Hk, G, Tk, D).sum(2).transpose(1, 2)
     dq, dk, dv = dS @ K * scale, heads(dS.transpose(-1, -2) @ Q * scale), heads(P.transpose(-1, -2) @ dO)
     res["dq"] = (dq.transpose(1, 2), (err @ K.abs() * scale + (u + d) * dq.abs()).transpose(1, 2))
     res["dk"] = (dk, heads(err.transpose(-1, -2) @ Q.abs() * scale) + (u + d) * dk.abs())
-    res["dv"] = (dv, (2 * u + 2 * d) * heads(P.transpose(-1, -2) @ dO.abs()))
+    res["dv"] = (dv, heads(((2 * u + 2 * d) * P + step * seen).transpose(-1, -2) @ dO.abs()))
     return res
 
 

@@ -1,4 +1,5 @@
 """Masked attention on the GPU against the 64-bit definition, with the bounds of masked_attention_oracle."""
+import contextlib
 import math
 
 import pytest
@@ -249,6 +250,77 @@ def test_unseen_garbage_has_no_effect(T, D):
     assert torch.isposinf(got[3][:, cut:j + 1, :, 1]).all()
     rest = [c for c in range(D) if c != 1]
     assert torch.equal(got[3][..., rest], clean[3][..., rest])
+
+
+@pytest.mark.parametrize("D", [64, 128, 40])
+@pytest.mark.parametrize("what", ["dout", "query"])
+def test_not_finite_queries_and_gradients_reach_what_they_see(D, what):
+    """One row's infinity and NaN: every key that the row sees, in blocks that the row's tile sees whole or
+    in part, and nothing else."""
+    from trustworthy_dl import ops
+    B, T, H, Hk, i = 2, 300, 4, 2, 200
+    mask = ops.attention_mask(B, T, device=DEV)
+    q, k, v, do = (_rand(n, B, T, h, D) for n, h in enumerate((H, Hk, Hk, H)))
+
+    def run():
+        ins = [t.clone().requires_grad_(True) for t in (q, k, v)]
+        return torch.autograd.grad(ops.masked_attention(*ins, mask), ins, do)
+    clean = run()
+    t = do if what == "dout" else q
+    t[:, i, :, 3] = float("nan")
+    t[:, i, :, 5] = float("inf")
+    dq, dk, dv = run()
+    others = [r for r in range(T) if r != i]
+    assert torch.equal(dq[:, others], clean[0][:, others]) and torch.isnan(dq[:, i]).all()
+    for g, c in ((dk, clean[1]), (dv, clean[2])):
+        assert torch.equal(g[:, i + 1:], c[:, i + 1:])
+    assert torch.isnan(dk[:, :i + 1]).all()
+    if what == "query":
+        assert torch.isnan(dv[:, :i + 1]).all()
+    else:      # dV: the gradient's own columns
+        assert torch.isnan(dv[:, :i + 1, :, 3]).all() and torch.isposinf(dv[:, :i + 1, :, 5]).all()
+        rest = [c for c in range(D) if c not in (3, 5)]
+        assert torch.equal(dv[..., rest], clean[2][..., rest])
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("cap", [30.0, 32.0, 33.0, 1000.0])
+def test_capped_scores_at_their_bounds(dtype, cap):
+    """Scores that saturate the cap on both sides (weights of e^(-2 cap)), and rows all of whose scores do."""
+    from trustworthy_dl import ops
+    if cap < 2 ** 7 / 1.4427:    # (the oracle's bound is for scores below 2^7)
+        _check(2, 161, 161, 3, 3, 64, dtype, "documents", cap=cap, mul=20.0)
+    v = _rand(5, 1, 70, 2, 64, dtype=dtype)
+    mask = ops.attention_mask(1, 70, causal=False, device=DEV)
+    for sign in (1.0, -1.0):
+        # every score is the same number near the bound: the mean of the values
+        q = torch.full((1, 70, 2, 64), 16.0, dtype=dtype, device=DEV)
+        k = torch.full((1, 70, 2, 64), 16.0 * sign, dtype=dtype, device=DEV)
+        out, lse = ops.masked_attention(q, k, v, mask, softcap=cap, return_lse=True)
+        want = oracle.run(q, k, v, mask.dense(), mask.pos.long(), 0.125, cap)
+        oracle.check(out, want["out"], "out")
+        # the score less its bound, up to 2 cap: a constant, a sum and a reciprocal of 2^-24, 2^-24 and 2^-23;
+        # the bound, its sum and the change of units: 2^-24 of cap each.  Together below cap 2^-20
+        assert ((lse.double() - want["lse"]).abs() <= 2.0 ** -13 + cap * 2.0 ** -20).all()
+
+
+def test_tensors_saved_elsewhere():
+    """Saved-tensor hooks bring the operands back contiguous: the same gradients, bit for bit."""
+    from trustworthy_dl import ops
+    x = _rand(11, 2, 150, (4 + 2 + 2) * 64)
+    mask = ops.attention_mask(2, 150, device=DEV)
+    do = _rand(12, 2, 150, 4 * 64)
+
+    def grad(packed, hooks):
+        z = x.clone().requires_grad_(True)
+        with hooks:
+            if packed:
+                out = ops.masked_attention_packed(z, 4, mask, n_kv_head=2)
+            else:
+                out = ops.masked_attention(*z.view(2, 150, 8, 64).split((4, 2, 2), 2), mask).reshape(2, 150, -1)
+        return torch.autograd.grad(out, z, do)[0]
+    for packed in (True, False):
+        assert torch.equal(grad(packed, contextlib.nullcontext()), grad(packed, torch.autograd.graph.save_on_cpu()))
 
 
 @pytest.mark.parametrize("Tk", [100, 1500])

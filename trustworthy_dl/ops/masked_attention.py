@@ -25,7 +25,7 @@ from . import _lib
 from ._lib import ptr
 
 _Q_TILE, _K_TILE = 32, 128     # csrc/masked_attention.h QT, KT
-MAX_SOFTCAP = 1000.0
+MIN_SOFTCAP, MAX_SOFTCAP = 1e-6, 1000.0
 
 
 # ============================================================== the mask
@@ -226,11 +226,11 @@ def _backward(q, k, v, out, lse, rest, dout, mask, scale, cap, slopes, dq, dk, d
                 g.zero_()
         return
     B, Tq, H, D = q.shape
-    # the rows' statistics, padded to whole tiles: lse log2(e) and -rowsum(dout out)
-    delta = torch.empty(B * H * 2 * (-(-Tq // _Q_TILE) * _Q_TILE), dtype=torch.float32, device=q.device)
+    # 256 words of scratch, then the rows' statistics, padded to whole tiles: lse log2(e) and -rowsum(dout out)
+    ws = torch.empty(256 + B * H * 2 * (-(-Tq // _Q_TILE) * _Q_TILE), dtype=torch.float32, device=q.device)
     keys = dk is not None
     a = _Args(q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(), out.data_ptr(), dq.data_ptr(), dk.data_ptr() if keys else 0,
-              dv.data_ptr() if keys else 0, lse.data_ptr(), delta.data_ptr(), 0, rest.data_ptr(),
+              dv.data_ptr() if keys else 0, lse.data_ptr(), ws.data_ptr() + 1024, ws.data_ptr(), rest.data_ptr(),
               0 if slopes is None else slopes.data_ptr(), mask.lo.data_ptr(), mask.hi.data_ptr(), mask.pos.data_ptr(),
               mask.q_table.data_ptr(), mask.k_table.data_ptr(), *_strides(q), *_strides(k), *_strides(v), *_strides(out),
               *_strides(dout), *_strides(dq), *(_strides(dk) if keys else _UNUSED), *(_strides(dv) if keys else _UNUSED),
@@ -343,9 +343,10 @@ def _check(name: str, q, k, v, mask, scale, softcap, slopes):
     if not (scale > 0 and math.isfinite(scale)):
         raise ValueError(f"{name}: scale must be positive, got {scale}")
     cap = 0.0 if softcap is None else float(softcap)
-    if softcap is not None and not 0 < cap <= MAX_SOFTCAP:
-        # cap tanh(x / cap) is evaluated to cap x 2^-23: beyond this the cap's own rounding would show
-        raise ValueError(f"{name}: softcap must lie in (0, {MAX_SOFTCAP:g}], got {softcap}")
+    if softcap is not None and not MIN_SOFTCAP <= cap <= MAX_SOFTCAP:
+        # cap tanh(x / cap) is evaluated to cap x 2^-21: beyond this the cap's own rounding would show (and
+        # below it scale / cap would leave fp32's range)
+        raise ValueError(f"{name}: softcap must lie in [{MIN_SOFTCAP:g}, {MAX_SOFTCAP:g}], got {softcap}")
     if slopes is not None:
         if slopes.shape != (H,) or slopes.device != q.device:
             raise ValueError(f"{name}: slopes must be a [{H}] tensor on {q.device}, got {tuple(slopes.shape)} on {slopes.device}")
