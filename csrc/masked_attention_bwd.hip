@@ -12,7 +12,8 @@ using namespace mattn;
 // dX is rounded to the inputs' type for the last product.  In fp16 it would leave the normal range where
 // probabilities (1 / T) and upstream gradients are small (1024 keys, |dO| ~ 1: steps of 6e-8 in values of
 // 1e-5; dQ and dK 1.8 times as far off as their own rounding) and overflow where a loss scale makes them
-// large, so it is scaled by a power of two that puts the largest |dO| into [2^4, 2^5).  The largest
+// large, so it is scaled by a power of two that puts the largest |dO| into [2^6, 2^7): steps below 2^-25 of a
+// unit P |dO|, and no overflow while P |dO . (v - o)| stays below 500 times the largest |dO|.  The largest
 // finite |dO| of the rows that see something, one per workgroup:
 constexpr int NMAX = 256;
 template <class T>
@@ -45,10 +46,14 @@ __device__ __forceinline__ int scale_exponent(const Args& a) {
     const uint32_t m = (uint32_t)wave_max_i((int)max(max(u.x, u.y), max(u.z, u.w)));
     float v, z;
     T::unpack(m, v, z);
-    return m == 0 ? 0 : 4 - (int)(((__float_as_uint(v) >> 23) & 0xffu) - 127u);
+    return m == 0 ? 0 : 6 - (int)(((__float_as_uint(v) >> 23) & 0xffu) - 127u);
 }
 
 // ============================================================================ dQ
+// Workgroup and tiles as in the forward.  Bound by the vector ALU: 500 instructions for 64 keys of a capped
+// score, 48 of them products.  Two waves a SIMD (three, for heads of 64: 88 against 85 us on 16 x 1024).
+// 2 x 8192, 16 heads of 128 on 4, cap 50: 942 us (one wave a SIMD, tiles through registers: 1656 us);
+// 16 x 1024 in documents, 16 heads of 64: 70 us.
 template <class T, int DP, bool CAP, bool ALIBI, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void mattn_dq_kernel(const Args a) {
     constexpr int BM = QT * NW, BN = 64, NS = DP / 16, NO = DP / 32, NTHR = 64 * NW;
@@ -254,6 +259,9 @@ __global__ __launch_bounds__(64 * NW, 2) void mattn_dq_kernel(const Args a) {
 // interleaves C(t - 1), B(t) and A(t + 1), two scores between every few products, each product's LDS
 // fragment read two products ahead.  Eight places for tiles of Q / dO are in LDS: t - 1 .. t + 1 are
 // read, t + 2 .. t + 4 are on their way (copies straight from memory); one barrier per tile.
+// 2 x 8192, 16 heads of 128 on 4, cap 50: 1540 us, 3500 cycles a tile of which 1024 are products (reading
+// fragments 4 or 5 products ahead: 1577 us); 16 x 1024 in documents, 16 heads of 64: 105 us (115 without
+// the pipeline).
 template <class T, int DP, bool CAP, bool ALIBI>
 __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void mattn_dkdv_kernel(const Args a) {
     constexpr int NS = DP / 16, NO = DP / 32, RING = 8;

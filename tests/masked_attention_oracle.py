@@ -10,8 +10,8 @@ the exponential, the sums over keys: each a few 2^-24 of the magnitudes, times t
   dQ    scale sum_j error |k| + (u + d) |dQ|;   dK   scale sum_i error |q| + (u + d) |dK|
 fp16 also has a smallest step, 2^-24: a P below 2^-14 is off by up to 2^-25 however small it is (forward: of
 a row whose largest is 1 and whose sum is at least 1), which adds 2^-25 sum |v| to out over the visible keys
-and 2^-25 sum |dO| to dV.  dS is rounded times 2^n with 2^n max|dO| in [2^4, 2^5), with a cap as a quarter (the derivative r (1 - r) without its 4):
-an absolute error of 2^-25 max|dO| / 16 (x 4 with a cap) per visible pair.
+and 2^-25 sum |dO| to dV.  dS is rounded times 2^n with 2^n max|dO| in [2^6, 2^7), with a cap as a quarter (the derivative r (1 - r) without its 4):
+an absolute error of 2^-25 max|dO| / 64 (x 4 with a cap) per visible pair.
 With a cap, dS carries the factor 1 - tanh^2 = 4 r (1 - r), exact to a few 2^-24: within d.
 """
 import math
@@ -82,7 +82,7 @@ def run(q, k, v, seen, first, scale, cap=0.0, slopes=None, dout=None):
     err = (u + d) * dS.abs() + P * (e + d * (dO.abs() @ V.abs().transpose(-1, -2) + delta.abs()))
     if cap:
         dS, err = dS * (1 - t * t), err * (1 - t * t) + d * dS.abs() * 2.0 ** -6
-    err = err + seen * (step / 16 * (4 if cap else 1) * float(dO.abs().max()))
+    err = err + seen * (step / 64 * (4 if cap else 1) * float(dO.abs().max()))
 
     def heads(t):   # sum over the query heads of a group
         return t.view(B, Hk, G, Tk, D).sum(2).transpose(1, 2)

@@ -188,8 +188,15 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
 
 def few_queries(batch: int, kv_heads: int, group: int, q_len: int, k_len: int) -> int:
     """0: the tiled kernel (32 queries of one head per wave).  Else the number of key ranges of the
-    few-queries kernel, which reads K / V once for the rows (heads of a group x queries) of a tile of 32."""
-    if q_len > 16:
+    few-queries kernel, which reads K / V once for the rows (heads of a group x queries) of a tile of 32.
+
+    Two workgroups a CU where the keys allow it, at least 4 ranges so that ragged caches even out, 512 keys
+    or more in each (a range costs a workgroup's start and its part of the join).  48 x 8 tiles of up to 8191 keys:
+    1 range 370 us, 2 317, 4 293, 8 294, 16 307; 16 tiles of 5003: 4 31 us, 8 23, 10 22, 20 27, 40 39; 12 tiles
+    of 1000: 1 12 us, 4 10 and a second launch.
+    Up to 32 queries it is the faster one (16 x 16 heads of 64, 4096 keys: 16 queries 63 against 96 us, 32 68
+    against 83, 64 125 against 87; 4 x 2 groups of 8 heads of 128, 5003 keys: 32 queries 42 against 148 us)."""
+    if q_len > 32:
         return 0
     tiles = batch * kv_heads * -(-(group * q_len) // 32)
     return max(1, min(max(-(-512 // tiles), 4), k_len // 512, 64))
