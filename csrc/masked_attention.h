@@ -368,8 +368,9 @@ struct Copy {
             // (from asm: before a transposed LDS read the compiler waits for every copy it knows of, it cannot
             // tell the two buffers apart)
             const uint32_t at = __builtin_amdgcn_readfirstlane(img + (j * NTHR + w * 64) * 16);
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(off + j * step),
-                         "s"(b) : "memory", "m0");
+            // (5 wait states before the first: the resource's registers might have been written by the vector ALU)
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop %c3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at),
+                         "v"(off + j * step), "s"(b), "n"(j == 0 ? 4 : 0) : "memory", "m0");
         }
     }
     // the columns past D, in whose place column 0 was copied

@@ -44,7 +44,8 @@ def _grad_like(z: torch.Tensor) -> torch.Tensor:
 
 def _alike(z: torch.Tensor, grad: torch.Tensor) -> bool:
     """``grad`` stands to the logits as _grad_like makes it."""
-    return (z.data_ptr() - grad.data_ptr()) % 16 == 0 and (z.stride(0) - grad.stride(0)) * z.element_size() % 16 == 0
+    return ((z.data_ptr() - grad.data_ptr()) % 16 == 0
+            and (z.shape[0] == 1 or (z.stride(0) - grad.stride(0)) * z.element_size() % 16 == 0))
 
 
 def _launch(z, index, teacher, labels, V, tau, alpha, counts, grad=None, rows=None, loss=None, gscale=None, written=False):
