@@ -323,7 +323,9 @@ __global__ __launch_bounds__(NT, 4) void distill_kernel(const DistillArgs a) {
             keep_packed(q);
         } else {
             // running maximum of the wave; the sums are rescaled where it rises (seldom after the first
-            // pieces).  UN loads of a thread in flight: the row streams through few registers
+            // pieces), except from -infinity, where they are zero still.  The maximum is taken across lanes, so
+            // every lane of a wave makes every trip; one without a piece of its own brings -infinity.  UN
+            // loads of a thread in flight: the row streams through few registers
             auto take = [&](u32x4 (&u)[UN], int n) {
                 float t = m;
 #pragma unroll
@@ -331,7 +333,7 @@ __global__ __launch_bounds__(NT, 4) void distill_kernel(const DistillArgs a) {
                     if (x < n) t = fmaxf(t, top(u[x]));
                 if (__any(t > m)) {
                     t = wave_max(t);
-                    rescale(zero_if_none(m) - zero_if_none(t));
+                    if (m != -INFINITY) rescale(m - t);
                     m = t;
                 }
                 const float mz = zero_if_none(m);
@@ -340,22 +342,26 @@ __global__ __launch_bounds__(NT, 4) void distill_kernel(const DistillArgs a) {
                 for (int x = 0; x < UN; ++x)
                     if (x < n) sums(u[x], mz);
             };
+            float none_[E];
+#pragma unroll
+            for (int i = 0; i < E; ++i) none_[i] = -INFINITY;
+            const u32x4 none = T::pack(none_);
             u32x4 u[UN];
             int p = tid;
-            for (; p + (UN - 1) * NT < np; p += UN * NT) {
+            for (; p - lane + 63 + (UN - 1) * NT < np; p += UN * NT) {
 #pragma unroll
                 for (int x = 0; x < UN; ++x) u[x] = zp[p + x * NT];
                 take(u, UN);
             }
-            for (; p < np; p += NT) {
-                u[0] = zp[p];
+            for (; p - lane < np; p += NT) {
+                u[0] = none;
+                if (p < np) u[0] = zp[p];
                 take(u, 1);
             }
-            u[0] = qe;
-            if (e0 < e1) take(u, 1);
-            const float mw = wave_max(m);   // (lanes that left a loop early missed the last rises)
-            rescale(zero_if_none(m) - zero_if_none(mw));
-            m = mw;
+            if (w == 0) {   // (the edge elements are lanes 0 and 1)
+                u[0] = qe;
+                take(u, 1);
+            }
         }
         st = wave_sum(st);
         if (MIX) s1 = wave_sum(s1);

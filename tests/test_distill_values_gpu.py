@@ -1,0 +1,105 @@
+"""Distillation loss on the GPU at logits that are not centred on 0: rows of any shift, far peaks, values of
+the type's lowest, gradients replayed from graphs.
+
+Bounds as in test_distill_gpu (a distance d from the row's maximum costs |d| 2^-24 in units of log 2, which
+does not grow with the row's shift); a probability below fp32's normal range may be flushed to zero."""
+import math
+
+import pytest
+import torch
+
+from test_distill import inputs
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+E = 2.0 ** -17
+BF, HF, FP = torch.bfloat16, torch.float16, torch.float32
+
+
+@pytest.fixture(autouse=True)
+def _native():
+    from trustworthy_dl.ops import _lib
+    _lib.lib()
+
+
+def definition(z, idx, t, labels, V, tau, alpha):
+    """(loss, dz [M, W], sum of the absolute terms of dz [M, W]) in 64 bits"""
+    M, W = z.shape
+    zd = z.detach()[:, :V].double()
+    use = (idx >= 0) & (idx < V) & (t != -math.inf)
+    n_t = max(1, int(((idx >= 0) & (idx < V)).any(1).sum()))
+    ok = (labels >= 0) & (labels < V)
+    n_l = max(1, int(ok.sum()))
+    x = torch.where(use, t.double() / tau, -math.inf)
+    live = use.any(1)[:, None].double()
+    q = torch.nan_to_num(torch.softmax(x, 1), nan=0.0)
+    lp = torch.log_softmax(zd / tau, 1)
+    at = torch.where(use, idx, 0).long()
+    kd = torch.where(q > 0, q * (torch.log(q) - lp.gather(1, at)), 0.0).sum()
+    c = alpha * tau / n_t
+    target = torch.zeros(M, V, dtype=torch.float64, device=z.device).scatter_add_(1, at, q)
+    g = torch.zeros(M, W, dtype=torch.float64, device=z.device)
+    size = torch.zeros_like(g)
+    g[:, :V] = c * (live * lp.exp() - target)
+    size[:, :V] = c * (live * lp.exp() + target)
+    loss = alpha * tau * tau * float(kd) / n_t
+    if alpha < 1:
+        lp = torch.log_softmax(zd, 1)
+        hot = torch.zeros(M, V, dtype=torch.float64, device=z.device)
+        hot[ok, labels[ok]] = 1.0
+        b = (1 - alpha) / n_l
+        loss -= b * float(torch.where(hot > 0, hot * lp, 0.0).sum())
+        g[:, :V] += b * (ok[:, None].double() * lp.exp() - hot)
+        size[:, :V] += b * (ok[:, None].double() * lp.exp() + hot)
+    return loss, g, size
+
+
+def check(z, idx, t, labels, V, tau, alpha, spread=32.0, extra=0.0):
+    """spread: the largest distance of a teacher's entry or a label from its row's maximum"""
+    from trustworthy_dl import ops
+    print(f"case {tuple(z.shape)} {z.dtype} V={V} K={idx.shape[1]} tau={tau} alpha={alpha}", flush=True)
+    z = z.detach().requires_grad_(True)
+    loss = ops.distillation_loss(z, idx, t, labels, V, temperature=tau, alpha=alpha)
+    (g,) = torch.autograd.grad(loss, z)
+    want, dz, mag = definition(z, idx, t, labels, V, tau, alpha)
+    size = alpha * tau * tau * (math.log(idx.shape[1]) + math.log(V) + spread / tau) + (1 - alpha) * (math.log(V) + spread)
+    assert abs(float(loss) - want) <= (E + extra) * size, (float(loss), want)
+    u = torch.finfo(z.dtype).eps / 2
+    tiny = torch.finfo(z.dtype).smallest_normal * torch.finfo(z.dtype).eps + torch.finfo(FP).smallest_normal
+    off = (g.double() - dz).abs() - (u * dz.abs() + (1 + u) * (E + extra) * mag + tiny)
+    assert not torch.isnan(g).any(), "NaN"
+    assert float(off.max()) <= 0, torch.nonzero(off == off.max())[0].tolist()
+
+
+def rows(M, V, K, dtype, shift, pad=0, seed=0):
+    z, idx, t, labels = inputs(M, V + pad, V, K, seed)
+    return (z + shift).to(dtype).to(DEV), idx.to(DEV), t.to(DEV), labels.to(DEV)
+
+
+FORMS = [(5, 700), (5, 7001), (5, 70001), (600, 9001)]     # a wave a row, in registers, streaming, many rows streaming
+MODES = [(1.0, 1.0), (1.0, 0.5), (2.0, 0.7), (4.0, 0.5), (1.5, 0.5)]
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+@pytest.mark.parametrize("M,V", FORMS)
+@pytest.mark.parametrize("tau,alpha", MODES)
+def test_shifted_rows(M, V, dtype, tau, alpha):
+    """A trained model's logits lie around -30 to -120; the loss does not depend on a row's shift."""
+    for shift in (-120.0, -700.0, 90.0):
+        # the row's and its waves' maxima, scaled, are rounded to 2^-24 of themselves: a few of those
+        check(*rows(M, V, 9, dtype, shift), V, tau, alpha, extra=abs(shift) * 2.0 ** -20)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("V,pad", [(9001, 0), (9001, 6), (8999, 9)])
+def test_peaks_in_the_last_pieces_of_negative_rows(dtype, V, pad):
+    """Row r has its maximum r columns before the end (or at the row's head): the edge elements and the
+    last, partly filled pieces."""
+    M = 640
+    z, idx, t, labels = rows(M, V, 9, dtype, 0.0, pad)
+    z = -200.0 - z.abs()
+    r = torch.arange(M, device=DEV)
+    z[r[:600], V - 1 - r[:600]] = -100.0
+    z[r[600:], r[600:] - 600] = -100.0
+    for tau, alpha in ((1.0, 1.0), (2.0, 0.5)):
+        check(z.to(dtype), idx, t, labels, V, tau, alpha, spread=110.0, extra=200 * 2.0 ** -20)
