@@ -111,11 +111,12 @@ __global__ __launch_bounds__(64 * NW, 2) void mattn_dq_kernel(const Args a) {
         }
     }
     delta += __shfl_xor(delta, 32, 64);
-    {   // for dK / dV: planes of lse log2(e) and -delta, zeros behind the last row of a head
+    {   // for dK / dV: planes of lse log2(e) and -delta; behind the last row of a head infinity (a weight of
+        // exactly 0, whatever bias its distance would have) and 0
         const int tp = (a.Tq + QT - 1) / QT * QT;
         float* st = a.delta + ((int64_t)at.b * a.H + at.h) * 2 * tp;
         if (h == 0 && qi < tp) {
-            st[qi] = qi < a.Tq ? lse2 : 0.f;
+            st[qi] = qi < a.Tq ? lse2 : INFINITY;
             st[tp + qi] = qi < a.Tq ? -delta : 0.f;
         }
     }
@@ -373,8 +374,8 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void mattn_dkdv_kernel(const
     auto whole = [&](const At& x, const Bounds& e) {
         return e.full_lo <= kbi * KT && e.full_hi >= (kbi + 1) * KT && a.D == DP && (x.t + 1) * QT <= a.Tq;
     };
-    // of a tile that has landed: the rows past the last are zeros, so whatever their constants say they
-    // add nothing (lse log2(e) is padded with zeros)
+    // of a tile that has landed: the rows past the last are zeros, and their weights too (lse log2(e) is
+    // padded with infinities), so whatever interval their constants say they add nothing
     auto mend = [&](const At& x, const Bounds& e, int buf) __attribute__((always_inline)) {
         if (whole(x, e)) return;
         CP::fix(tiles[buf], tid, 0, a.Tq - x.t * QT, a.D, qflag[buf]);   // (as K in dQ)
