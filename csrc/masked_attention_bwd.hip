@@ -11,42 +11,81 @@ using namespace mattn;
 // ============================================================================ fp16's range
 // dX is rounded to the inputs' type for the last product.  In fp16 it would leave the normal range where
 // probabilities (1 / T) and upstream gradients are small (1024 keys, |dO| ~ 1: steps of 6e-8 in values of
-// 1e-5; dQ and dK 1.8 times as far off as their own rounding) and overflow where a loss scale makes them
-// large, so it is scaled by a power of two that puts the largest |dO| into [2^6, 2^7): steps below 2^-25 of a
-// unit P |dO|, and no overflow while P |dO . (v - o)| stays below 500 times the largest |dO|.  The largest
-// finite |dO| of the rows that see something, one per workgroup:
+// 1e-5; dQ and dK 1.8 times as far off as their own rounding) and overflow where values or a loss scale make
+// them large, so it is scaled by a power of two that follows from a bound of it:
+//   dS_ij = P_ij dO_i . (v_j - o_i),   v_j - o_i = sum_{k != j} P_ik (v_j - v_k)
+//   |dX_ij| <= |dS_ij| <= P (1 - P) |dO_i| 2 max|v| <= B = max|dO_i| max|v_j| / 2      (row norms, visible rows)
+// 2^n B in [2^14, 2^15): half of the range is left for the roundings in P and delta, and the steps are 2^-39 B.
+// First the largest squares of row norms (not finite elements left out: they make their rows NaN anyhow),
+// one of each kind per workgroup.
 constexpr int NMAX = 256;
+// whether some query of batch row b sees key j
+__device__ __forceinline__ bool key_seen(const Args& a, int b, int j) {
+    const int nq = (a.Tq + QT - 1) / QT, nk = (a.Tk + KT - 1) / KT;
+    const int2 range = a.ktab[(int64_t)b * nk + j / KT];
+    for (int t = range.x; t < range.y; ++t) {
+        const int4 e = a.qtab[(int64_t)b * nq + t];
+        if (j < e.x || j >= e.y) continue;
+        if (j >= e.z && j < e.w) return true;
+        for (int i = t * QT; i < min(t * QT + QT, a.Tq); ++i)
+            if (j >= a.lo[(int64_t)b * a.Tq + i] && j < a.hi[(int64_t)b * a.Tq + i]) return true;
+    }
+    return false;
+}
 template <class T>
-__global__ __launch_bounds__(256) void mattn_dout_max_kernel(const Args a) {
-    __shared__ uint32_t red[4];
-    const int nch = a.D / 8;
-    const int64_t rows = (int64_t)a.B * a.Tq, pieces = rows * a.H * nch;
-    uint32_t m = 0;
-    for (int64_t p = (int64_t)blockIdx.x * 256 + threadIdx.x; p < pieces; p += NMAX * 256) {
-        const int64_t x = p / nch, row = x / a.H, b = row / a.Tq;
-        const int c = (int)(p - x * nch), hh = (int)(x - row * a.H), t = (int)(row - b * a.Tq);
-        if (a.lo[row] >= a.hi[row]) continue;
-        const u32x4 u = *(const u32x4*)((const bf16_t*)a.dout + b * a.dos[0] + t * a.dos[1] + hh * a.dos[2] + 8 * c);
+__device__ __forceinline__ float row_square(const bf16_t* row, int D) {
+    float s = 0.f;
+    for (int c = 0; c < D; c += 8) {
+        const u32x4 u = finite_only<T>(*(const u32x4*)(row + c));
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const uint32_t v = (u[k >> 1] >> (16 * (k & 1))) & 0x7fffu;
-            m = v < T::INF && v > m ? v : m;
+        for (int k = 0; k < 4; ++k) {
+            float x, y;
+            T::unpack(u[k], x, y);
+            s = fmaf(x, x, fmaf(y, y, s));
         }
     }
-    m = (uint32_t)wave_max_i((int)m);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
-    __syncthreads();
-    if (threadIdx.x == 0) ((uint32_t*)a.ws)[blockIdx.x] = max(max(red[0], red[1]), max(red[2], red[3]));
+    return s;
 }
-// the exponent of the scale, 0 where all of dO is zero
+template <class T>
+__global__ __launch_bounds__(256) void mattn_norm_max_kernel(const Args a) {
+    __shared__ uint32_t red[2][4];
+    float m[2] = {0.f, 0.f};
+    const int64_t first = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    for (int64_t x = first; x < (int64_t)a.B * a.Tq * a.H; x += NMAX * 256) {
+        const int64_t row = x / a.H, b = row / a.Tq;
+        const int hh = (int)(x - row * a.H), t = (int)(row - b * a.Tq);
+        if (a.lo[row] >= a.hi[row]) continue;
+        m[0] = fmaxf(m[0], row_square<T>((const bf16_t*)a.dout + b * a.dos[0] + t * a.dos[1] + hh * a.dos[2], a.D));
+    }
+    for (int64_t x = first; x < (int64_t)a.B * a.Tk; x += NMAX * 256) {
+        const int b = (int)(x / a.Tk), j = (int)(x - (int64_t)b * a.Tk);
+        if (!key_seen(a, b, j)) continue;
+        for (int hh = 0; hh < a.Hk; ++hh)
+            m[1] = fmaxf(m[1], row_square<T>((const bf16_t*)a.v + b * a.vs[0] + j * a.vs[1] + hh * a.vs[2], a.D));
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {   // (not negative: ordered as their bits)
+        const int w = wave_max_i((int)__float_as_uint(m[k]));
+        if ((threadIdx.x & 63) == 0) red[k][threadIdx.x >> 6] = (uint32_t)w;
+    }
+    __syncthreads();
+    if (threadIdx.x < 2) {
+        const uint32_t* r = red[threadIdx.x];
+        ((uint32_t*)a.ws)[NMAX * threadIdx.x + blockIdx.x] = max(max(r[0], r[1]), max(r[2], r[3]));
+    }
+}
+// the exponent n of the scale, 0 where dO or V is zero
 template <class T>
 __device__ __forceinline__ int scale_exponent(const Args& a) {
     if constexpr (T::INF == 0x7f80) return 0;   // bf16 has fp32's range
-    const uint4 u = ((const uint4*)a.ws)[threadIdx.x & 63];
-    const uint32_t m = (uint32_t)wave_max_i((int)max(max(u.x, u.y), max(u.z, u.w)));
-    float v, z;
-    T::unpack(m, v, z);
-    return m == 0 ? 0 : 6 - (int)(((__float_as_uint(v) >> 23) & 0xffu) - 127u);
+    float big[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const uint4 u = ((const uint4*)a.ws)[64 * k + (threadIdx.x & 63)];
+        big[k] = __uint_as_float((uint32_t)wave_max_i((int)max(max(u.x, u.y), max(u.z, u.w))));
+    }
+    const float bound = 0.5f * sqrtf(big[0] * big[1]);   // (squares of fp16 norms: in [2^-48, 2^39], no product leaves fp32's range)
+    return bound == 0.f ? 0 : 14 - (int)((__float_as_uint(bound) >> 23) - 127u);
 }
 
 // ============================================================================ dQ
@@ -619,7 +658,7 @@ static int bwd_launch(const Args& a, hipStream_t s) {
     if (gq > 0x7fffffff || gk > 0x7fffffff) return (int)hipErrorInvalidValue;
     int rc = 0;
     if (T::INF != 0x7f80) {
-        mattn_dout_max_kernel<T><<<NMAX, 256, 0, s>>>(a);
+        mattn_norm_max_kernel<T><<<NMAX, 256, 0, s>>>(a);
         rc = (int)hipGetLastError();
         if (rc) return rc;
     }
@@ -640,7 +679,7 @@ static int bwd_score(const Args& a, hipStream_t s) {
 }
 
 // args: mattn::Args with o, lse and rest from the forward; delta: planes of [B H][2][Tq padded to 32]
-// floats, ws: 256 words (fp16), both written and read
+// floats, ws: 512 words (fp16), both written and read
 TDL_API int tdl_masked_attn_bwd(const void* args, hipStream_t s) {
     const Args& a = *(const Args*)args;
     if (a.B <= 0 || a.Tq <= 0 || a.Tk <= 0 || a.H <= 0 || a.Hk <= 0 || a.H % a.Hk || a.D <= 0 || a.D > 128 || a.D % 8 ||

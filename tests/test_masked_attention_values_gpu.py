@@ -48,3 +48,36 @@ def test_bias_towards_far_keys(T, D, cap, dtype):
     for n, g in got.items():
         assert torch.isfinite(g).all(), n
         oracle.check(g, want[n], n)
+
+
+@pytest.mark.parametrize("cap", [None, 20.0])
+@pytest.mark.parametrize("D", [8, 64, 128])
+@pytest.mark.parametrize("size,T", [(16.0, 2), (16.0, 161), (64.0, 70), (1000.0, 300), (1e-3, 161)])
+@pytest.mark.parametrize("aligned", [True, False])
+def test_fp16_gradients_of_large_values(aligned, size, T, D, cap):
+    """|dO . (v - o)| far above |dO|: no gradient overflows that fp16 can hold."""
+    from trustworthy_dl import ops
+    print(f"case aligned={aligned} size={size} T={T} D={D} cap={cap}", flush=True)
+    H, Hk = 4, 2
+    q, k = _rand(0, 2, T, H, D, dtype=HF, mul=0.5), _rand(1, 2, T, Hk, D, dtype=HF, mul=1.0 / max(1.0, size / 32))
+    if aligned:
+        v = (torch.sign(_rand(2, 2, T, Hk, 1, dtype=HF)) * size).expand(2, T, Hk, D).contiguous()
+        do = torch.ones(2, T, H, D, dtype=HF, device=DEV)
+    else:
+        v, do = _rand(2, 2, T, Hk, D, dtype=HF, mul=size), _rand(3, 2, T, H, D, dtype=HF)
+    mask = ops.attention_mask(2, T, device=DEV, causal=T > 2)
+    got = _grads(q, k, v, do, mask, softcap=cap)
+    scale = 1 / math.sqrt(D)
+    seen = mask.dense()
+    want = oracle.run(q, k, v, seen, mask.pos.long(), scale, cap or 0.0, None, do)
+    assert all(float(want[n][0].abs().max()) < 60000 for n in got)      # representable
+    # dX is kept times a power of two 2^n with 2^n max|dO_i| max|v_j| / 2 in [2^14, 2^15) (row norms: P (1 - P) times
+    # twice them bounds |dX|), so below fp16's normal range it is off by 2^-25 2^-n a visible pair
+    step = 2.0 ** -25 * 2.0 ** -14 * 0.5 * float(do.double().norm(dim=-1).max() * v.double().norm(dim=-1).max())
+    s = seen.double()[:, None]
+    kk, qq = k.double().abs().transpose(1, 2).repeat_interleave(H // Hk, 1), q.double().abs().transpose(1, 2)
+    more = {"dq": (s @ kk).transpose(1, 2) * scale * step * (4 if cap else 1),
+            "dk": (s.transpose(-1, -2) @ qq).view(2, Hk, H // Hk, T, D).sum(2).transpose(1, 2) * scale * step * (4 if cap else 1)}
+    for n, g in got.items():
+        assert torch.isfinite(g).all(), n
+        oracle.check(g, (want[n][0], want[n][1] + more.get(n, 0.0)), n)

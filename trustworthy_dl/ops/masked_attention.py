@@ -233,11 +233,11 @@ def _backward(q, k, v, out, lse, rest, dout, mask, scale, cap, slopes, dq, dk, d
                 g.zero_()
         return
     B, Tq, H, D = q.shape
-    # 256 words of scratch, then the rows' statistics, padded to whole tiles: lse log2(e) and -rowsum(dout out)
-    ws = torch.empty(256 + B * H * 2 * (-(-Tq // _Q_TILE) * _Q_TILE), dtype=torch.float32, device=q.device)
+    # 512 words of scratch, then the rows' statistics, padded to whole tiles: lse log2(e) and -rowsum(dout out)
+    ws = torch.empty(512 + B * H * 2 * (-(-Tq // _Q_TILE) * _Q_TILE), dtype=torch.float32, device=q.device)
     keys = dk is not None
     a = _Args(q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(), out.data_ptr(), dq.data_ptr(), dk.data_ptr() if keys else 0,
-              dv.data_ptr() if keys else 0, lse.data_ptr(), ws.data_ptr() + 1024, ws.data_ptr(), rest.data_ptr(),
+              dv.data_ptr() if keys else 0, lse.data_ptr(), ws.data_ptr() + 2048, ws.data_ptr(), rest.data_ptr(),
               0 if slopes is None else slopes.data_ptr(), mask.lo.data_ptr(), mask.hi.data_ptr(), mask.pos.data_ptr(),
               mask.q_table.data_ptr(), mask.k_table.data_ptr(), *_strides(q), *_strides(k), *_strides(v), *_strides(out),
               *_strides(dout), *_strides(dq), *(_strides(dk) if keys else _UNUSED), *(_strides(dv) if keys else _UNUSED),
