@@ -144,3 +144,17 @@ def test_few_queries_rule():
     for args in ((1, 12, 1, 1, 1), (48, 8, 4, 1, 8191), (1, 1, 8, 16, 1 << 20), (4096, 8, 1, 1, 100)):
         n = few_queries(*args)
         assert 1 <= n <= 64 and (n == 1 or n <= -(-args[4] // 128))
+
+
+def test_operands_start_at_16_bytes():
+    """Dense tensors cut from a flat buffer at an odd offset, which contiguous() returns as they are."""
+    from trustworthy_dl.ops.masked_attention import _aligned
+    for off in (1, 4, 8):
+        flat = torch.randn(3 * 5 * 2 * 64 + off).bfloat16()
+        t = flat[off:].view(3, 5, 2, 64)
+        a = _aligned(t)
+        assert a.data_ptr() % 16 == 0 and torch.equal(a, t) and a.is_contiguous()
+        assert (a is t) == (t.data_ptr() % 16 == 0)
+    rows = torch.zeros(3, 5, 2, 72).bfloat16()[..., :64]
+    assert _aligned(rows) is rows
+    assert _aligned(rows.transpose(2, 3)[..., :1].expand(3, 5, 64, 2)).is_contiguous()

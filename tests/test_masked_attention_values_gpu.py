@@ -81,3 +81,22 @@ def test_fp16_gradients_of_large_values(aligned, size, T, D, cap):
     for n, g in got.items():
         assert torch.isfinite(g).all(), n
         oracle.check(g, (want[n][0], want[n][1] + more.get(n, 0.0)), n)
+
+
+def test_operands_cut_from_a_flat_buffer():
+    """q, k, v and the upstream gradient, dense and at an odd offset, give what aligned copies give."""
+    from trustworthy_dl import ops
+    B, T, D = 2, 100, 64
+    mask = ops.attention_mask(B, T, device=DEV)
+    want_in = [_rand(i, B, T, h, D) for i, h in enumerate((4, 2, 2, 4))]
+    cut = []
+    for t in want_in:
+        flat = torch.zeros(t.numel() + 3, dtype=BF, device=DEV)
+        flat[3:] = t.flatten()
+        cut.append(flat[3:].view(t.shape))
+    a, b = _grads(*want_in, mask), _grads(*cut, mask)
+    assert all(torch.equal(a[n], b[n]) for n in a)
+    x = torch.cat(want_in[:3], 2).reshape(B, T, -1)
+    flat = torch.zeros(x.numel() + 1, dtype=BF, device=DEV)
+    flat[1:] = x.flatten()
+    assert torch.equal(ops.masked_attention_packed(flat[1:].view(x.shape), 4, mask, n_kv_head=2).view(B, T, 4, D), a["out"])

@@ -177,13 +177,14 @@ def _strides(t: torch.Tensor):
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
-    """``t`` [B, T, heads, D] with unit column stride and 16-byte rows (64 of which span less than 2 GiB):
-    as it is, or a contiguous copy."""
+    """``t`` [B, T, heads, D] with unit column stride and rows that start at 16 bytes (64 of which span less
+    than 2 GiB): as it is, or a contiguous copy."""
     s = t.stride()
     if s[3] == 1 and t.data_ptr() % 16 == 0 and s[1] < 1 << 24:
         if not (s[0] | s[1] | s[2]) % 8 or all(s[i] % 8 == 0 for i in range(3) if t.shape[i] > 1):
             return t
-    return t.contiguous()
+    c = t.contiguous()     # (``t`` itself where it is dense, wherever it starts)
+    return c if c.data_ptr() % 16 == 0 else c.clone(memory_format=torch.contiguous_format)
 
 
 def few_queries(batch: int, kv_heads: int, group: int, q_len: int, k_len: int) -> int:
