@@ -100,3 +100,43 @@ def test_operands_cut_from_a_flat_buffer():
     flat = torch.zeros(x.numel() + 1, dtype=BF, device=DEV)
     flat[1:] = x.flatten()
     assert torch.equal(ops.masked_attention_packed(flat[1:].view(x.shape), 4, mask, n_kv_head=2).view(B, T, 4, D), a["out"])
+
+
+@pytest.mark.parametrize("packed", [True, False])
+def test_hooks_that_change_layouts(packed):
+    """Saved-tensor hooks that bring every tensor back with other strides and at an odd offset: the same
+    gradients.  Ones that bring it back on another device, in another type or shape are refused."""
+    from trustworthy_dl import ops
+    B, T, H, Hk, D = 2, 150, 4, 2, 64
+    x, do = _rand(11, B, T, (H + 2 * Hk) * D), _rand(12, B, T, H * D)
+    slopes = torch.tensor([0.1, 0.2, 0.3, 0.4], device=DEV)
+    mask = ops.attention_mask(B, T, device=DEV)
+
+    def grad(unpack):
+        z = x.clone().requires_grad_(True)
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+            if packed:
+                out = ops.masked_attention_packed(z, H, mask, n_kv_head=Hk, slopes=slopes)
+            else:
+                out = ops.masked_attention(*z.view(B, T, H + 2 * Hk, D).split((H, Hk, Hk), 2), mask, slopes=slopes).reshape(B, T, -1)
+        return torch.autograd.grad(out, z, do)[0]
+
+    def strided(t):     # one column in two, from an odd element
+        store = torch.full((2 * t.numel() + 1,), 7, dtype=t.dtype, device=t.device)
+        back = store[1:].view(*t.shape, 2)[..., 0]
+        back.copy_(t)
+        return back
+
+    def shifted(t):
+        store = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)
+        store[1:] = t.flatten()
+        return store[1:].view(t.shape)
+
+    def last_first(t):
+        return t.transpose(0, -1).contiguous().transpose(0, -1)
+    want = grad(lambda t: t)
+    for f in (strided, shifted, last_first):
+        assert torch.equal(grad(f), want), f.__name__
+    for f in (lambda t: t.cpu(), lambda t: t[:1], lambda t: t.double()):
+        with pytest.raises(RuntimeError, match="came back"):
+            grad(f)

@@ -230,4 +230,23 @@ def call_on(device: torch.device, name: str, *args):
             call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
+def kept(*tensors):
+    """What ``came_back`` compares saved tensors with."""
+    return [None if t is None else (t.shape, t.dtype) for t in tensors]
+
+
+def came_back(name: str, tensors, was, device: torch.device):
+    """The tensors that autograd kept for a backward pass: saved-tensor hooks may bring back others, and a
+    kernel reads what it is given, so they have to be of the same shapes and types and on the device."""
+    for t, w in zip(tensors, was):
+        if t is not None and ((t.shape, t.dtype) != w or t.device != device):
+            raise RuntimeError(f"{name}: a saved tensor of {tuple(w[0])} {w[1]} on {device} came back as {tuple(t.shape)} {t.dtype} on {t.device}")
+
+
+def dense(t: torch.Tensor) -> torch.Tensor:
+    """``t``, contiguous and starting at 16 bytes: as it is, or a copy."""
+    c = t.contiguous()     # (``t`` itself where it is contiguous, wherever it starts)
+    return c if c.data_ptr() % 16 == 0 else c.clone(memory_format=torch.contiguous_format)
+
+
 DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}

@@ -183,8 +183,7 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     if s[3] == 1 and t.data_ptr() % 16 == 0 and s[1] < 1 << 24:
         if not (s[0] | s[1] | s[2]) % 8 or all(s[i] % 8 == 0 for i in range(3) if t.shape[i] > 1):
             return t
-    c = t.contiguous()     # (``t`` itself where it is dense, wherever it starts)
-    return c if c.data_ptr() % 16 == 0 else c.clone(memory_format=torch.contiguous_format)
+    return _lib.dense(t)
 
 
 def few_queries(batch: int, kv_heads: int, group: int, q_len: int, k_len: int) -> int:
@@ -227,7 +226,7 @@ def _forward(q, k, v, mask, scale, cap, slopes, want_lse: bool, want_rest: bool)
 
 
 def _backward(q, k, v, out, lse, rest, dout, mask, scale, cap, slopes, dq, dk, dv):
-    """Writes dq and, unless both are None, dk and dv."""
+    """Writes dq and, unless both are None, dk and dv.  ``lse``, ``rest``, ``slopes``: dense."""
     if q.numel() == 0:
         for g in (dk, dv):
             if g is not None:
@@ -246,6 +245,14 @@ def _backward(q, k, v, out, lse, rest, dout, mask, scale, cap, slopes, dq, dk, d
     _lib.call_on(q.device, "tdl_masked_attn_bwd", ctypes.addressof(a))
 
 
+def _saved(name, ctx, operands, device):
+    """The saved tensors as the kernels take them, whatever layout hooks gave them: first ``operands`` ones
+    with strides of their own, then dense ones."""
+    saved = ctx.saved_tensors
+    _lib.came_back(name, saved, ctx.kept, device)
+    return [None if t is None else _aligned(t) if i < operands else _lib.dense(t) for i, t in enumerate(saved)]
+
+
 class _MaskedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, mask, scale, cap, slopes, want_lse):
@@ -254,6 +261,7 @@ class _MaskedAttention(torch.autograd.Function):
         out, lse, rest = _forward(q, k, v, mask, scale, cap, slopes, want_lse or grad, grad)
         ctx.save_for_backward(q, k, v, out, lse, rest, slopes)
         ctx.mask, ctx.scale, ctx.cap = mask, scale, cap
+        ctx.kept = _lib.kept(q, k, v, out, lse, rest, slopes)
         ctx.set_materialize_grads(False)   # (no zeros for the statistics)
         if lse is not None:
             ctx.mark_non_differentiable(lse)
@@ -264,7 +272,7 @@ class _MaskedAttention(torch.autograd.Function):
     def backward(ctx, dout, _dlse):
         if dout is None:
             return (None,) * 8
-        q, k, v, out, lse, rest, slopes = ctx.saved_tensors
+        q, k, v, out, lse, rest, slopes = _saved("masked_attention", ctx, 4, dout.device)
         keys = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
         dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         dk = torch.empty(k.shape, dtype=k.dtype, device=k.device) if keys else None
@@ -283,12 +291,13 @@ class _MaskedAttentionPacked(torch.autograd.Function):
         out, lse, rest = _forward(q, k, v, mask, scale, cap, slopes, ctx.needs_input_grad[0], ctx.needs_input_grad[0])
         ctx.save_for_backward(qkv, out, lse, rest, slopes)
         ctx.mask, ctx.scale, ctx.cap, ctx.heads = mask, scale, cap, (n_head, n_kv_head, n_kv_head)
+        ctx.kept = _lib.kept(qkv, out, lse, rest, slopes)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        qkv, out, lse, rest, slopes = ctx.saved_tensors
+        qkv, out, lse, rest, slopes = _saved("masked_attention_packed", ctx, 2, dout.device)
         dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
         _backward(*qkv.split(ctx.heads, dim=2), out, lse, rest, _aligned(dout), ctx.mask, ctx.scale, ctx.cap, slopes,
                   *dqkv.split(ctx.heads, dim=2))
