@@ -103,3 +103,35 @@ def test_peaks_in_the_last_pieces_of_negative_rows(dtype, V, pad):
     z[r[600:], r[600:] - 600] = -100.0
     for tau, alpha in ((1.0, 1.0), (2.0, 0.5)):
         check(z.to(dtype), idx, t, labels, V, tau, alpha, spread=110.0, extra=200 * 2.0 ** -20)
+
+
+@pytest.mark.parametrize("upstream", [1.0, 3.0])
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_hooks_that_change_layouts(dtype, upstream):
+    """Saved-tensor hooks that bring every tensor back transposed or with a column stride of 2, or on another
+    device, in another type or shape."""
+    from trustworthy_dl import ops
+    base, idx, t, labels = rows(37, 1003, 9, dtype, 0.0)
+
+    def grad(unpack):
+        z = base.clone().requires_grad_(True)
+        with torch.autograd.graph.saved_tensors_hooks(lambda x: x, unpack):
+            loss = ops.distillation_loss(z, idx, t, labels, temperature=2.0, alpha=0.4)
+        return torch.autograd.grad(loss, z, torch.tensor(upstream, device=DEV))[0]
+
+    def strided(x):
+        store = torch.full((2 * x.numel(),), 7, dtype=x.dtype, device=x.device)
+        back = store.view(*x.shape, 2)[..., 0]
+        back.copy_(x)
+        return back
+
+    def last_first(x):
+        return x.transpose(0, -1).contiguous().transpose(0, -1)
+    want = grad(lambda x: x)
+    for f in (strided, last_first):
+        # (rows that start elsewhere are added in another order: two roundings of the value, 2^-20 of the sums)
+        assert ((grad(f).double() - want.double()).abs()
+                <= torch.finfo(dtype).eps * want.double().abs() + 2.0 ** -20 * want.double().abs().max()).all(), f.__name__
+    for f in (lambda x: x.cpu(), lambda x: x[:1], lambda x: x.double()):
+        with pytest.raises(RuntimeError, match="came back"):
+            grad(f)

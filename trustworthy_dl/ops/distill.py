@@ -31,6 +31,12 @@ class _Args(ctypes.Structure):
                 + [("tau", ctypes.c_float), ("alpha", ctypes.c_float), ("beta", ctypes.c_float)])
 
 
+def _rows(z: torch.Tensor) -> torch.Tensor:
+    """``z`` [M, W] with unit column stride and rows that do not overlap: as it is, or a copy."""
+    M, W = z.shape
+    return z.contiguous() if z.stride(1) != 1 or (M > 1 and z.stride(0) < W) else z
+
+
 def _grad_like(z: torch.Tensor) -> torch.Tensor:
     """Uninitialised [M, W] whose rows stand at the same offset from 16 bytes as the logits' rows."""
     M, W = z.shape
@@ -73,13 +79,16 @@ class _Distill(torch.autograd.Function):
         ctx.grad = _grad_like(z) if ctx.needs_input_grad[0] else None
         _launch(z, index, teacher, labels, V, tau, alpha, counts, grad=ctx.grad, rows=rows, loss=loss)
         ctx.save_for_backward(z, index, teacher, labels, counts)
+        ctx.kept = _lib.kept(z, index, teacher, labels, counts)
         ctx.how = (V, tau, alpha)
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        z, index, teacher, labels, counts = ctx.saved_tensors
+        saved = ctx.saved_tensors
+        _lib.came_back("distillation_loss", saved, ctx.kept, g.device)
+        z, (index, teacher, labels, counts) = _rows(saved[0]), [None if t is None else t.contiguous() for t in saved[1:]]
         grad, ctx.grad = ctx.grad, None
         # a second backward through the same node gets its own buffer, and so do logits that saved-tensor
         # hooks brought back with other rows
@@ -171,6 +180,4 @@ def distillation_loss(logits: torch.Tensor, teacher_index: torch.Tensor, teacher
         raise ValueError(f"native distillation_loss supports float32, bfloat16 and float16 logits (got {z.dtype})")
     if teacher.dtype not in _lib.DTYPE_CODE:
         raise ValueError(f"native distillation_loss supports float32, bfloat16 and float16 teacher logits (got {teacher.dtype})")
-    if z.stride(1) != 1 or (z.shape[0] > 1 and z.stride(0) < W):
-        z = z.contiguous()
-    return _Distill.apply(z, index.contiguous(), teacher.contiguous(), None if labels is None else labels.contiguous(), V, tau, alpha)
+    return _Distill.apply(_rows(z), index.contiguous(), teacher.contiguous(), None if labels is None else labels.contiguous(), V, tau, alpha)
