@@ -140,3 +140,26 @@ def test_hooks_that_change_layouts(packed):
     for f in (lambda t: t.cpu(), lambda t: t[:1], lambda t: t.double()):
         with pytest.raises(RuntimeError, match="came back"):
             grad(f)
+
+
+@pytest.mark.parametrize("what", ["lo", "hi", "pos", "q_table", "k_table"])
+def test_a_mask_changed_before_the_backward_pass(what):
+    from trustworthy_dl import ops
+    mask = ops.attention_mask(1, 40, device=DEV)
+    x = _rand(0, 1, 40, 3 * 64).requires_grad_(True)
+    outs = [ops.masked_attention_packed(x, 1, mask), ops.masked_attention(*x.view(1, 40, 3, 64).split(1, 2), mask)]
+    getattr(mask, what).zero_()
+    for out in outs:
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            out.sum().backward()
+
+
+def test_a_mask_made_in_inference_mode_serves_training():
+    from trustworthy_dl import ops
+    x = _rand(0, 1, 40, 3 * 64).requires_grad_(True)
+    with torch.inference_mode():
+        mask = ops.attention_mask(1, 40, device=DEV)
+        seen = ops.masked_attention_packed(x, 1, mask)
+    out = ops.masked_attention_packed(x, 1, mask)
+    out.sum().backward()
+    assert torch.equal(out, seen) and torch.isfinite(x.grad).all()

@@ -45,6 +45,9 @@ class AttentionMask:
     def device(self) -> torch.device:
         return self.lo.device
 
+    def _tensors(self):   # as _forward and _backward take them
+        return self.lo, self.hi, self.pos, self.q_table, self.k_table
+
     def dense(self) -> torch.Tensor:
         """[batch, q_len, k_len] booleans (for inspection and the CPU path)."""
         j = torch.arange(self.k_len, device=self.device)
@@ -114,8 +117,9 @@ def attention_mask(batch: int, q_len: int, k_len: Optional[int] = None, *, causa
     def ints(*shape):
         return torch.empty(shape, dtype=torch.int32, device=device)
     nq, nk = -(-q_len // _Q_TILE), -(-k_len // _K_TILE)
-    m = AttentionMask(batch, q_len, k_len, ints(batch, q_len), ints(batch, q_len), ints(batch), ints(batch, nq, 4),
-                      ints(batch, nk, 2))
+    with torch.inference_mode(False):     # (a mask may be kept for training: autograd saves its tensors)
+        m = AttentionMask(batch, q_len, k_len, ints(batch, q_len), ints(batch, q_len), ints(batch), ints(batch, nq, 4),
+                          ints(batch, nk, 2))
     if batch == 0 or q_len == 0:
         return m
     ws = ints(batch * 3 * k_len) if documents is not None or marks is not None else None
@@ -218,15 +222,14 @@ def _forward(q, k, v, mask, scale, cap, slopes, want_lse: bool, want_rest: bool)
         ws = torch.empty(B * H * Tq * nsplit * ((64 if D <= 64 else 128) + 2), dtype=torch.float32, device=dev)
     a = _Args(q.data_ptr(), k.data_ptr(), v.data_ptr(), 0, out.data_ptr(), 0, 0, 0, 0 if lse is None else lse.data_ptr(), 0,
               0 if ws is None else ws.data_ptr(), 0 if rest is None else rest.data_ptr(), 0 if slopes is None else slopes.data_ptr(),
-              mask.lo.data_ptr(), mask.hi.data_ptr(), mask.pos.data_ptr(), mask.q_table.data_ptr(), mask.k_table.data_ptr(),
-              *_strides(q), *_strides(k), *_strides(v), *_strides(out), *_UNUSED, *_UNUSED, *_UNUSED, *_UNUSED,
+              *[t.data_ptr() for t in mask], *_strides(q), *_strides(k), *_strides(v), *_strides(out), *_UNUSED, *_UNUSED, *_UNUSED, *_UNUSED,
               B, Tq, Tk, H, Hk, D, _lib.DTYPE_CODE[q.dtype], nsplit, scale, cap)
     _lib.call_on(dev, "tdl_masked_attn_fwd", ctypes.addressof(a))
     return out, lse, rest
 
 
-def _backward(q, k, v, out, lse, rest, dout, mask, scale, cap, slopes, dq, dk, dv):
-    """Writes dq and, unless both are None, dk and dv.  ``lse``, ``rest``, ``slopes``: dense."""
+def _backward(q, k, v, out, lse, rest, slopes, mask, dout, scale, cap, dq, dk, dv):
+    """Writes dq and, unless both are None, dk and dv.  ``lse``, ``rest``, ``slopes`` and the mask's tensors: dense."""
     if q.numel() == 0:
         for g in (dk, dv):
             if g is not None:
@@ -238,11 +241,16 @@ def _backward(q, k, v, out, lse, rest, dout, mask, scale, cap, slopes, dq, dk, d
     keys = dk is not None
     a = _Args(q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(), out.data_ptr(), dq.data_ptr(), dk.data_ptr() if keys else 0,
               dv.data_ptr() if keys else 0, lse.data_ptr(), ws.data_ptr() + 2048, ws.data_ptr(), rest.data_ptr(),
-              0 if slopes is None else slopes.data_ptr(), mask.lo.data_ptr(), mask.hi.data_ptr(), mask.pos.data_ptr(),
-              mask.q_table.data_ptr(), mask.k_table.data_ptr(), *_strides(q), *_strides(k), *_strides(v), *_strides(out),
-              *_strides(dout), *_strides(dq), *(_strides(dk) if keys else _UNUSED), *(_strides(dv) if keys else _UNUSED),
+              0 if slopes is None else slopes.data_ptr(), *[t.data_ptr() for t in mask], *_strides(q), *_strides(k), *_strides(v),
+              *_strides(out), *_strides(dout), *_strides(dq), *(_strides(dk) if keys else _UNUSED), *(_strides(dv) if keys else _UNUSED),
               B, Tq, k.shape[1], H, k.shape[2], D, _lib.DTYPE_CODE[q.dtype], 0, scale, cap)
     _lib.call_on(q.device, "tdl_masked_attn_bwd", ctypes.addressof(a))
+
+
+def _save(ctx, *tensors):
+    # (the mask's tensors too: a change of them before the backward pass is noticed like one of an operand's)
+    ctx.save_for_backward(*tensors)
+    ctx.kept = _lib.kept(*tensors)
 
 
 def _saved(name, ctx, operands, device):
@@ -258,10 +266,10 @@ class _MaskedAttention(torch.autograd.Function):
     def forward(ctx, q, k, v, mask, scale, cap, slopes, want_lse):
         q, k, v = _aligned(q), _aligned(k), _aligned(v)
         grad = any(ctx.needs_input_grad[:3])
+        mask = mask._tensors()
         out, lse, rest = _forward(q, k, v, mask, scale, cap, slopes, want_lse or grad, grad)
-        ctx.save_for_backward(q, k, v, out, lse, rest, slopes)
-        ctx.mask, ctx.scale, ctx.cap = mask, scale, cap
-        ctx.kept = _lib.kept(q, k, v, out, lse, rest, slopes)
+        ctx.scale, ctx.cap = scale, cap
+        _save(ctx, q, k, v, out, lse, rest, slopes, *mask)
         ctx.set_materialize_grads(False)   # (no zeros for the statistics)
         if lse is not None:
             ctx.mark_non_differentiable(lse)
@@ -272,12 +280,12 @@ class _MaskedAttention(torch.autograd.Function):
     def backward(ctx, dout, _dlse):
         if dout is None:
             return (None,) * 8
-        q, k, v, out, lse, rest, slopes = _saved("masked_attention", ctx, 4, dout.device)
+        q, k, v, out, lse, rest, slopes, *mask = _saved("masked_attention", ctx, 4, dout.device)
         keys = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
         dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         dk = torch.empty(k.shape, dtype=k.dtype, device=k.device) if keys else None
         dv = torch.empty(v.shape, dtype=v.dtype, device=v.device) if keys else None
-        _backward(q, k, v, out, lse, rest, _aligned(dout), ctx.mask, ctx.scale, ctx.cap, slopes, dq, dk, dv)
+        _backward(q, k, v, out, lse, rest, slopes, mask, _aligned(dout), ctx.scale, ctx.cap, dq, dk, dv)
         return dq, dk, dv, None, None, None, None, None
 
 
@@ -288,18 +296,18 @@ class _MaskedAttentionPacked(torch.autograd.Function):
     def forward(ctx, qkv, n_head, n_kv_head, mask, scale, cap, slopes):
         qkv = _aligned(qkv)
         q, k, v = qkv.split((n_head, n_kv_head, n_kv_head), dim=2)
+        mask = mask._tensors()
         out, lse, rest = _forward(q, k, v, mask, scale, cap, slopes, ctx.needs_input_grad[0], ctx.needs_input_grad[0])
-        ctx.save_for_backward(qkv, out, lse, rest, slopes)
-        ctx.mask, ctx.scale, ctx.cap, ctx.heads = mask, scale, cap, (n_head, n_kv_head, n_kv_head)
-        ctx.kept = _lib.kept(qkv, out, lse, rest, slopes)
+        ctx.scale, ctx.cap, ctx.heads = scale, cap, (n_head, n_kv_head, n_kv_head)
+        _save(ctx, qkv, out, lse, rest, slopes, *mask)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        qkv, out, lse, rest, slopes = _saved("masked_attention_packed", ctx, 2, dout.device)
+        qkv, out, lse, rest, slopes, *mask = _saved("masked_attention_packed", ctx, 2, dout.device)
         dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
-        _backward(*qkv.split(ctx.heads, dim=2), out, lse, rest, _aligned(dout), ctx.mask, ctx.scale, ctx.cap, slopes,
+        _backward(*qkv.split(ctx.heads, dim=2), out, lse, rest, slopes, mask, _aligned(dout), ctx.scale, ctx.cap,
                   *dqkv.split(ctx.heads, dim=2))
         return dqkv, None, None, None, None, None, None
 
@@ -388,7 +396,7 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: At
     if q.is_cuda and torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         out, lse = _MaskedAttention.apply(q, k, v, mask, scale, cap, slopes, return_lse)
     elif q.is_cuda:   # (a single token's call is bound by the host: no autograd node)
-        out, lse, _ = _forward(_aligned(q), _aligned(k), _aligned(v), mask, scale, cap, slopes, return_lse, False)
+        out, lse, _ = _forward(_aligned(q), _aligned(k), _aligned(v), mask._tensors(), scale, cap, slopes, return_lse, False)
     else:
         out, lse = _reference(q, k, v, mask, scale, cap, slopes)
     return (out, lse) if return_lse else out
