@@ -163,3 +163,28 @@ def test_a_mask_made_in_inference_mode_serves_training():
     out = ops.masked_attention_packed(x, 1, mask)
     out.sum().backward()
     assert torch.equal(out, seen) and torch.isfinite(x.grad).all()
+
+
+def test_forward_mode_is_refused():
+    """A tangent would be lost where no input wants a gradient."""
+    from torch.autograd import forward_ad
+
+    from trustworthy_dl import ops
+    mask = ops.attention_mask(1, 40, device=DEV)
+    t = [_rand(i, 1, 40, 1, 64) for i in range(3)]
+    slopes = torch.tensor([0.1], device=DEV)
+    want = ops.masked_attention(*t, mask, slopes=slopes)
+    with forward_ad.dual_level():
+        assert torch.equal(ops.masked_attention(*t, mask, slopes=slopes), want)
+        for i in range(3):
+            dual = [forward_ad.make_dual(x, torch.ones_like(x)) if j == i else x for j, x in enumerate(t)]
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                ops.masked_attention(*dual, mask)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            ops.masked_attention(*t, mask, slopes=forward_ad.make_dual(slopes, slopes))
+        x = torch.cat(t, 2).reshape(1, 40, -1)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            ops.masked_attention_packed(forward_ad.make_dual(x, x), 1, mask)
+        z = _rand(5, 4, 9).float()
+        with pytest.raises(NotImplementedError):
+            ops.distillation_loss(forward_ad.make_dual(z, z), torch.zeros(4, 2, dtype=torch.long, device=DEV), z[:, :2])

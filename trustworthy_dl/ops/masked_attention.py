@@ -19,6 +19,7 @@ import math
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -378,6 +379,9 @@ def _check(name: str, q, k, v, mask, scale, softcap, slopes):
         if slopes.requires_grad:
             raise ValueError(f"{name}: slopes are constants (no gradient is computed for them); pass slopes.detach()")
         slopes = slopes.to(torch.float32).contiguous()
+    if q.is_cuda and forward_ad._current_level >= 0 and any(
+            t is not None and forward_ad.unpack_dual(t).tangent is not None for t in (q, k, v, slopes)):
+        raise NotImplementedError(f"native {name} has no forward-mode derivative; use reverse mode")
     return scale, cap, slopes
 
 
