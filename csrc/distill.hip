@@ -88,7 +88,19 @@ struct DistillArgs {
     int M, V, W, K, G;          // W: columns of the gradient (V real ones, zeros behind them)
     int dtype, index64, teacher_dtype, written;   // written: grad holds the gradient for gscale 1 already
     float tau, alpha, beta;     // beta = 1 - alpha, rounded from more than 32 bits
+    uint64_t capture;           // written by every call: the graph capture that its launches belong to (0: none)
 };
+
+// the capture that a stream's launches go into: 0 for none, ~0 where that cannot be told
+uint64_t capture_of(hipStream_t s) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (hipStreamGetCaptureInfo(s, &status, &id) != hipSuccess) {
+        (void)hipGetLastError();
+        return ~0ull;
+    }
+    return status == hipStreamCaptureStatusNone ? 0 : id;
+}
 
 __device__ __forceinline__ int entry_at(const DistillArgs& a, int64_t i) {   // -1 where unused
     if (a.index64) {
@@ -515,8 +527,14 @@ int by_length(const DistillArgs& a, hipStream_t s) {
 
 // args: DistillArgs.  rows not null: counts, loss rows, loss and (grad not null) the gradient.  rows
 // null: the gradient alone, from counts that an earlier call left.
-TDL_API int tdl_distill(const void* args, hipStream_t s) {
-    const DistillArgs& a = *(const DistillArgs*)args;
+// written, with the capture of the call that wrote: it is believed only where both calls run eagerly or are nodes of one
+// graph.  A graph of the gradient alone is replayed without that call, over what the last replay and its
+// user left in grad.
+TDL_API int tdl_distill(void* args, hipStream_t s) {
+    const uint64_t capture = capture_of(s), before = ((DistillArgs*)args)->capture;
+    ((DistillArgs*)args)->capture = capture;
+    DistillArgs a = *(const DistillArgs*)args;
+    if (capture != before || capture == ~0ull) a.written = 0;
     if (a.M <= 0 || a.V <= 0 || a.W < a.V || a.K <= 0 || a.K > MAX_K || a.G <= 0 || a.dtype < 0 || a.dtype > 2 || !(a.tau > 0.f) ||
         !(a.alpha >= 0.f && a.alpha <= 1.f) ||
         !(a.beta >= 0.f && a.beta <= 1.f) || (a.beta > 0.f && a.labels == nullptr) || (a.rows == nullptr && a.grad == nullptr))

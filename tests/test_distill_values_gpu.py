@@ -105,6 +105,31 @@ def test_peaks_in_the_last_pieces_of_negative_rows(dtype, V, pad):
         check(z.to(dtype), idx, t, labels, V, tau, alpha, spread=110.0, extra=200 * 2.0 ** -20)
 
 
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_backward_replayed_by_itself(dtype):
+    """Forward and backward as two graphs: each replay of the backward gives the gradient of the upstream
+    gradient it is given, whatever the replay before left and whatever happened to its output."""
+    from trustworthy_dl import ops
+    z, idx, t, labels = rows(37, 3000, 6, dtype, 0.0)
+    z.requires_grad_(True)
+
+    def loss(x):
+        return ops.distillation_loss(x, idx, t, labels, temperature=2.0, alpha=0.5)
+
+    def eager(x, c):
+        y = x.detach().clone().requires_grad_(True)
+        return torch.autograd.grad(loss(y), y, torch.tensor(c, device=DEV))[0]
+    graphed = torch.cuda.make_graphed_callables(loss, (z,))
+    for trial in range(2):
+        x = (z.detach() + trial).to(dtype).requires_grad_(True)
+        out = graphed(x)
+        for c in (3.0, 1.0, 1.0, 0.5, 1.0):
+            (g,) = torch.autograd.grad(out, x, torch.tensor(c, device=DEV), retain_graph=True)
+            torch.cuda.synchronize()
+            assert torch.equal(g, eager(x, c)), c
+            g.mul_(0.25)       # (a user's clipping, in place)
+
+
 @pytest.mark.parametrize("upstream", [1.0, 3.0])
 @pytest.mark.parametrize("dtype", [BF, FP])
 def test_hooks_that_change_layouts(dtype, upstream):

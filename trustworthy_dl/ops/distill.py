@@ -28,7 +28,7 @@ class _Args(ctypes.Structure):
     _fields_ = ([(n, ctypes.c_void_p) for n in ("logits", "grad", "index", "teacher", "labels", "gscale", "rows", "counts", "loss")]
                 + [(n, ctypes.c_int64) for n in ("ld", "gld")]
                 + [(n, ctypes.c_int) for n in ("M", "V", "W", "K", "G", "dtype", "index64", "teacher_dtype", "written")]
-                + [("tau", ctypes.c_float), ("alpha", ctypes.c_float), ("beta", ctypes.c_float)])
+                + [("tau", ctypes.c_float), ("alpha", ctypes.c_float), ("beta", ctypes.c_float), ("capture", ctypes.c_uint64)])
 
 
 def _rows(z: torch.Tensor) -> torch.Tensor:
@@ -54,20 +54,23 @@ def _alike(z: torch.Tensor, grad: torch.Tensor) -> bool:
             and (z.shape[0] == 1 or (z.stride(0) - grad.stride(0)) * z.element_size() % 16 == 0))
 
 
-def _launch(z, index, teacher, labels, V, tau, alpha, counts, grad=None, rows=None, loss=None, gscale=None, written=False):
+def _launch(z, index, teacher, labels, V, tau, alpha, counts, grad=None, rows=None, loss=None, gscale=None, written=False, capture=0):
+    """Returns the graph capture that the launches went into (0: none)."""
     M, W = z.shape
     gptr, gld = (0, 0) if grad is None else (grad.data_ptr(), grad.stride(0))
     a = _Args(z.data_ptr(), gptr, index.data_ptr(), teacher.data_ptr(), 0 if labels is None else labels.data_ptr(),
               0 if gscale is None else gscale.data_ptr(), 0 if rows is None else rows.data_ptr(), counts.data_ptr(),
               0 if loss is None else loss.data_ptr(), z.stride(0), gld, M, V, W, index.shape[1], counts.shape[0],
-              _lib.DTYPE_CODE[z.dtype], index.dtype is torch.int64, _lib.DTYPE_CODE[teacher.dtype], written, tau, alpha, 1.0 - alpha)
+              _lib.DTYPE_CODE[z.dtype], index.dtype is torch.int64, _lib.DTYPE_CODE[teacher.dtype], written, tau, alpha, 1.0 - alpha, capture)
     _lib.call_on(z.device, "tdl_distill", ctypes.addressof(a))
+    return a.capture
 
 
 class _Distill(torch.autograd.Function):
     """The forward leaves the gradient for an upstream gradient of 1 (loss.backward()); the backward
     launches a pass that reads the upstream gradient on the device and, where it is another, computes
-    the gradient again from the logits (one rounding either way, no host synchronisation)."""
+    the gradient again from the logits (one rounding either way, no host synchronisation).  A backward
+    captured into a graph without its forward always computes it."""
 
     @staticmethod
     def forward(ctx, z, index, teacher, labels, V, tau, alpha):
@@ -77,7 +80,7 @@ class _Distill(torch.autograd.Function):
         loss = torch.empty((), dtype=torch.float32, device=dev)
         counts = torch.empty(max(1, min(256, -(-M // 256))), 2, dtype=torch.int32, device=dev)
         ctx.grad = _grad_like(z) if ctx.needs_input_grad[0] else None
-        _launch(z, index, teacher, labels, V, tau, alpha, counts, grad=ctx.grad, rows=rows, loss=loss)
+        ctx.capture = _launch(z, index, teacher, labels, V, tau, alpha, counts, grad=ctx.grad, rows=rows, loss=loss)
         ctx.save_for_backward(z, index, teacher, labels, counts)
         ctx.kept = _lib.kept(z, index, teacher, labels, counts)
         ctx.how = (V, tau, alpha)
@@ -95,7 +98,7 @@ class _Distill(torch.autograd.Function):
         written = grad is not None and _alike(z, grad)
         if not written:
             grad = _grad_like(z)
-        _launch(z, index, teacher, labels, *ctx.how, counts, grad=grad, gscale=g, written=written)
+        _launch(z, index, teacher, labels, *ctx.how, counts, grad=grad, gscale=g, written=written, capture=ctx.capture)
         return (grad,) + (None,) * 6
 
 
