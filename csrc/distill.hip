@@ -182,13 +182,14 @@ __device__ __forceinline__ void keep_packed(u32x4 (&q)[N]) {
 // cross-entropy, the first alone.  An exponential issues for 8 cycles where a product takes 4, so where
 // the temperature allows the second one is a power of the first, e^d = (e^(d / tau))^tau: MODE 1, 2, 4
 // for those temperatures.  MODE 0, any other one, takes both.
-// 16-bit logits take z c - m c in one fma (its rounding is 2^-24 of |m c|, alike in numerator and
-// sum); fp32 ones subtract first.
+// The distance is taken before its product: a fma of z c with the rounded m c would leave that rounding,
+// 2^-24 of |m c|, in the exponent, which differs from wave to wave and grows with the row's shift without
+// bound (a row of bf16's lowest values: infinite).
 template <class T, int MODE>
 struct Soft {
     float ct;
     static __device__ __forceinline__ float one(float f, float m, float c) {
-        return T::E == 8 ? exp2_(fmaf(f, c, -(m * c))) : exp2_((f - m) * c);
+        return exp2_((f - m) * c);
     }
     // t = 2^((f - m) ct), o = 2^((f - m) log2 e)
     __device__ __forceinline__ void operator()(float f, float m, float& t, float& o) const {
