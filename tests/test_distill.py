@@ -111,3 +111,16 @@ def test_refusals():
     bad("needs labels", z, idx, t, alpha=0.5)
     bad("labels must be", z, idx, t, labels[:3], alpha=0.5)
     bad("labels must be", z, idx, t, labels.float(), alpha=0.5)
+
+
+def test_temperatures_out_of_range():
+    z, idx, t, labels = inputs(4, 9, 9, 3)
+    for x in (1e-50, 1e-30, 1e-7, 1001.0, 1e20, 1e300):     # (1e-50 is 0 in 32 bits, 1e20 squared infinite)
+        with pytest.raises(ValueError, match="temperature"):
+            ops.distillation_loss(z, idx, t, temperature=x)
+    for x in (1e-6, 1000.0):
+        want, dz = formula(z, idx, t, None, 9, x, 1.0)
+        y = z.double().requires_grad_(True)
+        loss = ops.distillation_loss(y, idx, t, temperature=x)
+        (g,) = torch.autograd.grad(loss, y)
+        assert math.isclose(float(loss.detach()), want, rel_tol=1e-8) and torch.allclose(g, dz, rtol=1e-8, atol=1e-12)

@@ -190,3 +190,22 @@ def test_hooks_that_change_layouts(dtype, upstream):
     for f in (lambda x: x.cpu(), lambda x: x[:1], lambda x: x.double()):
         with pytest.raises(RuntimeError, match="came back"):
             grad(f)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("M,V", FORMS)
+@pytest.mark.parametrize("tau", [1e-6, 1e-2, 1000.0])
+def test_temperatures_at_their_bounds(tau, M, V, dtype):
+    z, idx, t, labels = rows(M, V, 9, dtype, -40.0)
+    # (at low ones a row has a few classes with all the weight: the distances of its entries, 32 / tau, are known
+    # to 2^-24 of themselves, and so are the logarithms of weights no smaller than that)
+    from trustworthy_dl import ops
+    z = z.detach().requires_grad_(True)
+    loss = ops.distillation_loss(z, idx, t, labels, V, temperature=tau, alpha=0.5)
+    (g,) = torch.autograd.grad(loss, z)
+    want, dz, mag = definition(z, idx, t, labels, V, tau, 0.5)
+    size = 0.5 * tau * tau * (math.log(9) + math.log(V) + 32 / tau) + 0.5 * (math.log(V) + 32)
+    assert abs(float(loss.detach()) - want) <= E * size
+    # a weight of e^(-d / tau): d 2^-24 / tau, for what is not yet zero (d / tau < 104); entries as well
+    off = (g.double() - dz).abs() - (torch.finfo(dtype).eps / 2 * dz.abs() + 1.01 * 2 * E * mag + 2.0 ** -126)
+    assert float(off.max()) <= 0, torch.nonzero(off == off.max())[0].tolist()

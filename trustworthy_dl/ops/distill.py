@@ -21,6 +21,7 @@ from torch.autograd.function import once_differentiable
 from . import _lib
 
 MAX_ENTRIES = 1024   # csrc/distill.hip MAX_K
+MIN_TEMPERATURE, MAX_TEMPERATURE = 1e-6, 1000.0
 
 
 class _Args(ctypes.Structure):
@@ -136,7 +137,8 @@ def distillation_loss(logits: torch.Tensor, teacher_index: torch.Tensor, teacher
     ``teacher_logits`` [..., K], K <= 1024, in any order: an index outside [0, num_classes) marks an
     unused entry, a row without entries takes no part in the first mean (a row whose entries are all
     -inf counts, but has nothing to teach); an index that stands twice counts twice.  ``labels``
-    (int64 [...], needed for alpha < 1): one outside [0, num_classes) takes no part in the second mean.
+    (int32 / int64 [...], needed for alpha < 1): one outside [0, num_classes) takes no part in the second mean.
+    ``temperature`` in [1e-6, 1000] (the first mean carries tau^2 times an error of 2^-20 or so).
     The gradient flows to ``logits`` (their type, zeros in the padding)."""
     if logits.dim() < 1 or not logits.dtype.is_floating_point:
         raise ValueError(f"distillation_loss: floating-point logits [..., classes], got {logits.dtype} {tuple(logits.shape)}")
@@ -157,15 +159,17 @@ def distillation_loss(logits: torch.Tensor, teacher_index: torch.Tensor, teacher
     if teacher_logits.requires_grad:
         raise ValueError("distillation_loss: the teacher gets no gradient; pass teacher_logits.detach()")
     tau, alpha = float(temperature), float(alpha)
-    if not 0 < tau < float("inf"):
-        raise ValueError(f"distillation_loss: temperature must be positive, got {temperature}")
+    if not MIN_TEMPERATURE <= tau <= MAX_TEMPERATURE:
+        # (kd is tau^2 times a difference of logarithms in 32 bits: beyond this its rounding is all that is left; below
+        # it 1 / tau would bring distances out of fp32's range)
+        raise ValueError(f"distillation_loss: temperature must lie in [{MIN_TEMPERATURE:g}, {MAX_TEMPERATURE:g}], got {temperature}")
     if not 0 <= alpha <= 1:
         raise ValueError(f"distillation_loss: alpha must lie in [0, 1], got {alpha}")
     if alpha < 1:
         if labels is None:
             raise ValueError("distillation_loss: alpha < 1 needs labels")
         if labels.shape != logits.shape[:-1] or labels.dtype not in (torch.int32, torch.int64):
-            raise ValueError(f"distillation_loss: labels must be int64 {tuple(logits.shape[:-1])}, got {labels.dtype} {tuple(labels.shape)}")
+            raise ValueError(f"distillation_loss: labels must be int32 or int64 {tuple(logits.shape[:-1])}, got {labels.dtype} {tuple(labels.shape)}")
     else:
         labels = None
     for name, t in (("teacher_index", teacher_index), ("teacher_logits", teacher_logits), ("labels", labels)):
