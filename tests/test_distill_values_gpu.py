@@ -209,3 +209,18 @@ def test_temperatures_at_their_bounds(tau, M, V, dtype):
     # a weight of e^(-d / tau): d 2^-24 / tau, for what is not yet zero (d / tau < 104); entries as well
     off = (g.double() - dz).abs() - (torch.finfo(dtype).eps / 2 * dz.abs() + 1.01 * 2 * E * mag + 2.0 ** -126)
     assert float(off.max()) <= 0, torch.nonzero(off == off.max())[0].tolist()
+
+
+def test_no_grad_makes_no_gradient():
+    """Under no_grad, of logits that require a gradient: no buffer of their size."""
+    from trustworthy_dl import ops
+    z, idx, t, labels = rows(64, 50257, 9, BF, 0.0)
+    z.requires_grad_(True)
+    want = ops.distillation_loss(z, idx, t, labels, alpha=0.5).detach()
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    with torch.no_grad():
+        got = ops.distillation_loss(z, idx, t, labels, alpha=0.5)
+    assert torch.cuda.max_memory_allocated() - before < z.numel()
+    assert torch.equal(got, want) and not got.requires_grad

@@ -74,13 +74,13 @@ class _Distill(torch.autograd.Function):
     captured into a graph without its forward always computes it."""
 
     @staticmethod
-    def forward(ctx, z, index, teacher, labels, V, tau, alpha):
+    def forward(ctx, z, index, teacher, labels, V, tau, alpha, grad):
         M = z.shape[0]
         dev = z.device
         rows = torch.empty(M, dtype=torch.float32, device=dev)
         loss = torch.empty((), dtype=torch.float32, device=dev)
         counts = torch.empty(max(1, min(256, -(-M // 256))), 2, dtype=torch.int32, device=dev)
-        ctx.grad = _grad_like(z) if ctx.needs_input_grad[0] else None
+        ctx.grad = _grad_like(z) if grad else None
         ctx.capture = _launch(z, index, teacher, labels, V, tau, alpha, counts, grad=ctx.grad, rows=rows, loss=loss)
         ctx.save_for_backward(z, index, teacher, labels, counts)
         ctx.kept = _lib.kept(z, index, teacher, labels, counts)
@@ -100,7 +100,7 @@ class _Distill(torch.autograd.Function):
         if not written:
             grad = _grad_like(z)
         _launch(z, index, teacher, labels, *ctx.how, counts, grad=grad, gscale=g, written=written, capture=ctx.capture)
-        return (grad,) + (None,) * 6
+        return (grad,) + (None,) * 7
 
 
 def _reference(z, index, teacher, labels, V, tau, alpha):
@@ -187,4 +187,7 @@ def distillation_loss(logits: torch.Tensor, teacher_index: torch.Tensor, teacher
         raise ValueError(f"native distillation_loss supports float32, bfloat16 and float16 logits (got {z.dtype})")
     if teacher.dtype not in _lib.DTYPE_CODE:
         raise ValueError(f"native distillation_loss supports float32, bfloat16 and float16 teacher logits (got {teacher.dtype})")
-    return _Distill.apply(_rows(z), index.contiguous(), teacher.contiguous(), None if labels is None else labels.contiguous(), V, tau, alpha)
+    # (under no_grad an input that requires a gradient still counts as one that needs it)
+    grad = z.requires_grad and torch.is_grad_enabled()
+    return _Distill.apply(_rows(z), index.contiguous(), teacher.contiguous(), None if labels is None else labels.contiguous(), V, tau, alpha,
+                          grad)
