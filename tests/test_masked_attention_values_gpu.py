@@ -188,3 +188,18 @@ def test_forward_mode_is_refused():
         z = _rand(5, 4, 9).float()
         with pytest.raises(NotImplementedError):
             ops.distillation_loss(forward_ad.make_dual(z, z), torch.zeros(4, 2, dtype=torch.long, device=DEV), z[:, :2])
+
+
+def test_no_grad_keeps_nothing_for_a_backward_pass():
+    """Under no_grad, of an input that requires a gradient: the output's memory and no more."""
+    from trustworthy_dl import ops
+    x = _rand(0, 4, 512, 3 * 8 * 64).requires_grad_(True)
+    mask = ops.attention_mask(4, 512, device=DEV)
+    want = ops.masked_attention_packed(x, 8, mask)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    with torch.no_grad():
+        got = ops.masked_attention_packed(x, 8, mask)
+    assert torch.cuda.max_memory_allocated() - before < 1.25 * want.numel() * 2
+    assert torch.equal(got, want.detach()) and not got.requires_grad

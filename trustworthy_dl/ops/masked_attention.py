@@ -294,11 +294,11 @@ class _MaskedAttentionPacked(torch.autograd.Function):
     """The gradients of q, k and v are written straight into one packed gradient."""
 
     @staticmethod
-    def forward(ctx, qkv, n_head, n_kv_head, mask, scale, cap, slopes):
+    def forward(ctx, qkv, n_head, n_kv_head, mask, scale, cap, slopes, grad):
         qkv = _aligned(qkv)
         q, k, v = qkv.split((n_head, n_kv_head, n_kv_head), dim=2)
         mask = mask._tensors()
-        out, lse, rest = _forward(q, k, v, mask, scale, cap, slopes, ctx.needs_input_grad[0], ctx.needs_input_grad[0])
+        out, lse, rest = _forward(q, k, v, mask, scale, cap, slopes, grad, grad)
         ctx.scale, ctx.cap, ctx.heads = scale, cap, (n_head, n_kv_head, n_kv_head)
         _save(ctx, qkv, out, lse, rest, slopes, *mask)
         return out
@@ -310,7 +310,7 @@ class _MaskedAttentionPacked(torch.autograd.Function):
         dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
         _backward(*qkv.split(ctx.heads, dim=2), out, lse, rest, slopes, mask, _aligned(dout), ctx.scale, ctx.cap,
                   *dqkv.split(ctx.heads, dim=2))
-        return dqkv, None, None, None, None, None, None
+        return (dqkv,) + (None,) * 7
 
 
 # ============================================================== CPU definition
@@ -420,7 +420,8 @@ def masked_attention_packed(qkv: torch.Tensor, n_head: int, mask: AttentionMask,
     q, k, v = x.split((n_head, hk, hk), dim=2)
     scale, cap, slopes = _check("masked_attention_packed", q, k, v, mask, scale, softcap, slopes)
     if qkv.is_cuda:
-        out = _MaskedAttentionPacked.apply(x, n_head, hk, mask, scale, cap, slopes)
+        # (under no_grad an input that requires a gradient still counts as one that needs it)
+        out = _MaskedAttentionPacked.apply(x, n_head, hk, mask, scale, cap, slopes, x.requires_grad and torch.is_grad_enabled())
     else:
         out, _ = _reference(q, k, v, mask, scale, cap, slopes)
     return out.reshape(B, T, -1)
