@@ -20,6 +20,7 @@
 namespace {
 
 constexpr int MAX_K = 1024;
+constexpr int MAX_DIM = 1 << 30;   // rows and columns stay below: an index plus a stride of the grid fits an int
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 struct F32 {
@@ -495,8 +496,9 @@ __global__ __launch_bounds__(NT, 4) void distill_kernel(const DistillArgs a) {
 template <class T, int NT, int NV, int MODE>
 int launch_mode(const DistillArgs& a, hipStream_t s) {
     const size_t lds = (size_t)(a.K + 1) * 16;
-    // one workgroup a row; the pass that most often has nothing to do (written) as few as fill the chip
-    const int grid = a.written && a.M > 1024 ? 1024 : a.M;
+    // one workgroup a row (up to what a launch takes, 2^32 threads less one); the pass that most often has nothing
+    // to do (written) as few as fill the chip
+    const int most = a.written ? 1024 : 1 << 21, grid = a.M < most ? a.M : most;
     if (a.grad != nullptr) distill_kernel<T, NT, NV, MODE, true><<<grid, NT, lds, s>>>(a);
     else distill_kernel<T, NT, NV, MODE, false><<<grid, NT, lds, s>>>(a);
     return (int)hipGetLastError();
@@ -536,7 +538,7 @@ TDL_API int tdl_distill(void* args, hipStream_t s) {
     ((DistillArgs*)args)->capture = capture;
     DistillArgs a = *(const DistillArgs*)args;
     if (capture != before || capture == ~0ull) a.written = 0;
-    if (a.M <= 0 || a.V <= 0 || a.W < a.V || a.K <= 0 || a.K > MAX_K || a.G <= 0 || a.dtype < 0 || a.dtype > 2 || !(a.tau > 0.f) ||
+    if (a.M <= 0 || a.M >= MAX_DIM || a.V <= 0 || a.W < a.V || a.W >= MAX_DIM || a.K <= 0 || a.K > MAX_K || a.G <= 0 || a.dtype < 0 || a.dtype > 2 || !(a.tau > 0.f) ||
         !(a.alpha >= 0.f && a.alpha <= 1.f) ||
         !(a.beta >= 0.f && a.beta <= 1.f) || (a.beta > 0.f && a.labels == nullptr) || (a.rows == nullptr && a.grad == nullptr))
         return (int)hipErrorInvalidValue;

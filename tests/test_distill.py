@@ -124,3 +124,21 @@ def test_temperatures_out_of_range():
         loss = ops.distillation_loss(y, idx, t, temperature=x)
         (g,) = torch.autograd.grad(loss, y)
         assert math.isclose(float(loss.detach()), want, rel_tol=1e-8) and torch.allclose(g, dz, rtol=1e-8, atol=1e-12)
+
+
+def test_library_refuses_sizes_out_of_range():
+    """The C entry point itself, before any launch (it needs no GPU for that)."""
+    import ctypes
+
+    from trustworthy_dl.ops import _lib
+    from trustworthy_dl.ops.distill import MAX_DIM, _Args
+    if not _lib.available():
+        pytest.skip("the native library is not built")
+    sizes = dict(rows=8, M=4, V=9, W=9, K=3, G=1, dtype=0, tau=1.0, alpha=1.0)
+
+    def refused(**kw):
+        a = _Args(**{**sizes, **kw})
+        return _lib.lib().tdl_distill(ctypes.addressof(a), None) == 1      # hipErrorInvalidValue
+    for kw in (dict(M=0), dict(M=MAX_DIM + 1), dict(W=MAX_DIM + 1), dict(V=10), dict(V=0), dict(K=0), dict(K=1025), dict(G=0), dict(dtype=3),
+               dict(tau=0.0), dict(alpha=1.5), dict(alpha=0.5, beta=0.5), dict(rows=0)):
+        assert refused(**kw), kw

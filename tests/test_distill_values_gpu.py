@@ -224,3 +224,17 @@ def test_no_grad_makes_no_gradient():
         got = ops.distillation_loss(z, idx, t, labels, alpha=0.5)
     assert torch.cuda.max_memory_allocated() - before < z.numel()
     assert torch.equal(got, want) and not got.requires_grad
+
+
+def test_sizes_out_of_range_are_refused():
+    from trustworthy_dl import ops
+    one, idx = torch.zeros(1, 1, dtype=BF, device=DEV), torch.zeros(1, 1, dtype=torch.int32, device=DEV)
+    n = 1 << 30
+    with pytest.raises(ValueError, match="rows and columns"):
+        ops.distillation_loss(one.expand(n, 1), idx.expand(n, 1), one.expand(n, 1))
+    with pytest.raises(ValueError, match="rows and columns"):
+        ops.distillation_loss(one.expand(1, n), idx, one)
+
+
+def test_more_rows_than_workgroups():
+    check(*rows((1 << 21) + 777, 8, 2, FP, 0.0), 8, 2.0, 0.5)

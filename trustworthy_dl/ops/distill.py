@@ -21,6 +21,7 @@ from torch.autograd.function import once_differentiable
 from . import _lib
 
 MAX_ENTRIES = 1024   # csrc/distill.hip MAX_K
+MAX_DIM = (1 << 30) - 1   # csrc/distill.hip MAX_DIM - 1
 MIN_TEMPERATURE, MAX_TEMPERATURE = 1e-6, 1000.0
 
 
@@ -187,6 +188,8 @@ def distillation_loss(logits: torch.Tensor, teacher_index: torch.Tensor, teacher
         raise ValueError(f"native distillation_loss supports float32, bfloat16 and float16 logits (got {z.dtype})")
     if teacher.dtype not in _lib.DTYPE_CODE:
         raise ValueError(f"native distillation_loss supports float32, bfloat16 and float16 teacher logits (got {teacher.dtype})")
+    if max(z.shape) > MAX_DIM:
+        raise ValueError(f"native distillation_loss supports up to {MAX_DIM} rows and columns (got {tuple(z.shape)})")
     # (under no_grad an input that requires a gradient still counts as one that needs it)
     grad = z.requires_grad and torch.is_grad_enabled()
     return _Distill.apply(_rows(z), index.contiguous(), teacher.contiguous(), None if labels is None else labels.contiguous(), V, tau, alpha,
