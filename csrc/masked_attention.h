@@ -26,6 +26,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr int QT = 32;    // queries per qtab entry
 constexpr int KT = 128;   // keys per ktab entry
+constexpr int64_t MAX_GRID = (1 << 24) - 1;   // workgroups of 256 threads: a launch takes less than 2^32 threads
 
 // one argument block for every entry point (ops/masked_attention.py fills the same layout)
 struct Args {

@@ -655,7 +655,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void mattn_dkdv_kernel(const
 template <class T, int DP, bool CAP, bool ALIBI>
 static int bwd_launch(const Args& a, hipStream_t s) {
     const int64_t gq = (int64_t)a.B * a.H * ((a.Tq + 127) / 128), gk = (int64_t)a.B * a.Hk * ((a.Tk + KT - 1) / KT);
-    if (gq > 0x7fffffff || gk > 0x7fffffff) return (int)hipErrorInvalidValue;
+    if (gq > MAX_GRID || gk > MAX_GRID) return (int)hipErrorInvalidValue;
     int rc = 0;
     if (T::INF != 0x7f80) {
         mattn_norm_max_kernel<T><<<NMAX, 256, 0, s>>>(a);

@@ -144,7 +144,7 @@ __global__ __launch_bounds__(PT) void attn_mask_kernel(const Id* __restrict__ do
 TDL_API int tdl_attn_mask(const void* documents, int wide, const int* prefix_rows, const void* prefix_marks, const int* lengths,
                           const int* q_start, int B, int Tq, int Tk, int causal, int* ws, int* lo, int* hi, int* pos, void* qtab,
                           void* ktab, hipStream_t s) {
-    if (B <= 0 || Tq <= 0 || Tk < Tq || ((documents != nullptr || prefix_marks != nullptr) && ws == nullptr))
+    if (B <= 0 || B >= 1 << 22 || Tq <= 0 || Tk < Tq || ((documents != nullptr || prefix_marks != nullptr) && ws == nullptr))
         return (int)hipErrorInvalidValue;
     const uint8_t* marks = (const uint8_t*)prefix_marks;
     if (wide)
@@ -611,18 +611,19 @@ static int fwd_launch(const Args& a, hipStream_t s) {
     if (a.nsplit > 0) {
         const int R = (a.H / a.Hk) * a.Tq, rt = (R + 31) / 32;   // rows, tiles of 32
         const int64_t grid = (int64_t)a.B * a.Hk * a.nsplit * rt;
-        if (grid > 0x7fffffff) return (int)hipErrorInvalidValue;
+        const int rpb = 256 / (DP / 4);   // rows of the join per workgroup
+        const int64_t joins = ((int64_t)a.B * a.H * a.Tq + rpb - 1) / rpb;
+        if (grid > MAX_GRID || joins > MAX_GRID) return (int)hipErrorInvalidValue;
         mattn_few_kernel<T, DP, CAP, ALIBI><<<(int)grid, 256, 0, s>>>(a);
         if (a.nsplit > 1) {
             const int rc = (int)hipGetLastError();
             if (rc) return rc;
-            const int rpb = 256 / (DP / 4);
-            mattn_join_kernel<T, DP><<<(int)(((int64_t)a.B * a.H * a.Tq + rpb - 1) / rpb), 256, 0, s>>>(a);
+            mattn_join_kernel<T, DP><<<(int)joins, 256, 0, s>>>(a);
         }
         TDL_LAUNCH_CHECK();
     }
     const int64_t grid = (int64_t)a.B * a.H * ((a.Tq + 127) / 128);
-    if (grid > 0x7fffffff) return (int)hipErrorInvalidValue;
+    if (grid > MAX_GRID) return (int)hipErrorInvalidValue;
     mattn_fwd_kernel<T, DP, CAP, ALIBI><<<(int)grid, 256, 0, s>>>(a);
     TDL_LAUNCH_CHECK();
 }

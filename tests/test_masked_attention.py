@@ -158,3 +158,36 @@ def test_operands_start_at_16_bytes():
     rows = torch.zeros(3, 5, 2, 72).bfloat16()[..., :64]
     assert _aligned(rows) is rows
     assert _aligned(rows.transpose(2, 3)[..., :1].expand(3, 5, 64, 2)).is_contiguous()
+
+
+def test_largest_launch_and_rows():
+    from trustworthy_dl.ops.masked_attention import MAX_GROUPS, few_queries, largest_launch
+    for B, Tq, Tk, H, Hk, D in ((2, 8192, 8192, 16, 4, 128), (64, 32768, 32768, 64, 64, 64), (1 << 16, 1, 4096, 32, 8, 128), (1, 1, (1 << 30) - 1, 1, 1, 8)):
+        G, n = H // Hk, few_queries(B, Hk, H // Hk, Tq, Tk)
+        parts = [B * H * math.ceil(Tq / 128), B * Hk * math.ceil(Tk / 128)]
+        if n:
+            parts += [B * Hk * n * math.ceil(G * Tq / 32), math.ceil(B * H * Tq / (256 // ((64 if D <= 64 else 128) // 4)))]
+        assert largest_launch(B, Tq, Tk, H, Hk, D) == max(parts)
+        # (the cheap test in front never hides a launch that is too large)
+        assert max(parts) <= B * H * (Tq + Tk)
+    assert largest_launch(1 << 22, 512, 512, 1, 1, 64) > MAX_GROUPS or largest_launch(1 << 22, 512, 512, 8, 8, 64) > MAX_GROUPS
+    _bad(lambda: ops.attention_mask(1 << 22, 0, 0), "rows")
+
+
+def test_library_refuses_arguments_out_of_range():
+    """The C entry points themselves, before any launch (they need no GPU for that)."""
+    import ctypes
+
+    from trustworthy_dl.ops import _lib
+    from trustworthy_dl.ops.masked_attention import _Args
+    if not _lib.available():
+        pytest.skip("the native library is not built")
+    good = dict(B=1, Tq=1, Tk=1, H=4, Hk=2, D=64, dtype=1, nsplit=1, scale=1.0, dk=8)
+    for kw in (dict(B=0), dict(Tq=0), dict(Tk=0), dict(H=3), dict(D=136), dict(D=12), dict(dtype=0), dict(scale=0.0), dict(cap=-1.0),
+               dict(B=1 << 23, nsplit=1), dict(B=1 << 22, nsplit=0), dict(B=1 << 26, nsplit=0)):
+        a = _Args(**{**good, **kw})
+        fwd = _lib.lib().tdl_masked_attn_fwd(ctypes.addressof(a), None)
+        assert fwd == 1, kw      # hipErrorInvalidValue
+        if "nsplit" not in kw or kw["B"] > 1 << 23:
+            assert _lib.lib().tdl_masked_attn_bwd(ctypes.addressof(a), None) == 1, kw
+    assert _lib.lib().tdl_attn_mask(None, 0, None, None, None, None, 1 << 22, 1, 1, 1, None, None, None, None, None, None, None) == 1

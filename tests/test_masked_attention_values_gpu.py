@@ -203,3 +203,17 @@ def test_no_grad_keeps_nothing_for_a_backward_pass():
         got = ops.masked_attention_packed(x, 8, mask)
     assert torch.cuda.max_memory_allocated() - before < 1.25 * want.numel() * 2
     assert torch.equal(got, want.detach()) and not got.requires_grad
+
+
+def test_sizes_out_of_range_are_refused():
+    from trustworthy_dl import ops
+    mask = ops.attention_mask(1, 1, device=DEV)
+    one = torch.zeros(1, 1, 1, 8, dtype=BF, device=DEV)
+    q = one.expand(1, 1, 1 << 21, 8)
+    with pytest.raises(ValueError, match="2\\^24 elements"):
+        ops.masked_attention(q, q, q, mask)
+    n = 1 << 20
+    mask = ops.attention_mask(n, 1, device=DEV)
+    q, k = one.expand(n, 1, 512, 8), one.expand(n, 1, 32, 8)
+    with pytest.raises(ValueError, match="split the batch"):
+        ops.masked_attention(q, k, k, mask)

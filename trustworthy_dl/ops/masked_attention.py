@@ -89,8 +89,8 @@ def attention_mask(batch: int, q_len: int, k_len: Optional[int] = None, *, causa
     k_len = q_len if k_len is None else k_len
     if batch < 0 or q_len < 0 or k_len < q_len:
         raise ValueError(f"attention_mask needs 0 <= q_len <= k_len, got batch {batch}, q_len {q_len}, k_len {k_len}")
-    if max(q_len, k_len) >= 1 << 30:
-        raise ValueError("attention_mask: at most 2^30 - 1 positions")
+    if max(q_len, k_len) >= 1 << 30 or batch >= 1 << 22:
+        raise ValueError("attention_mask: at most 2^30 - 1 positions and 2^22 - 1 rows")
     if device is None:
         device = next((t.device for t in (documents, prefix, lengths, q_start) if isinstance(t, torch.Tensor)), torch.device("cpu"))
     device = torch.device(device)
@@ -205,6 +205,16 @@ def few_queries(batch: int, kv_heads: int, group: int, q_len: int, k_len: int) -
         return 0
     tiles = batch * kv_heads * -(-(group * q_len) // 32)
     return max(1, min(max(-(-512 // tiles), 4), k_len // 512, 64))
+
+
+MAX_GROUPS = (1 << 24) - 1     # workgroups of 256 threads in a launch (csrc/masked_attention.h MAX_GRID)
+
+
+def largest_launch(B: int, Tq: int, Tk: int, H: int, Hk: int, D: int) -> int:
+    """Workgroups of the largest launch of a forward or backward pass."""
+    n = few_queries(B, Hk, H // Hk, Tq, Tk)
+    fwd = max(B * Hk * n * -(-(H // Hk * Tq) // 32), -(-(B * H * Tq) // (16 if D <= 64 else 8))) if n else 0
+    return max(fwd, B * H * -(-Tq // 128), B * Hk * -(-Tk // 128))
 
 
 def _forward(q, k, v, mask, scale, cap, slopes, want_lse: bool, want_rest: bool):
@@ -348,12 +358,12 @@ def _check(name: str, q, k, v, mask, scale, softcap, slopes):
     if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape:
         raise ValueError(f"{name}: q [B, Tq, H, D], k and v [B, Tk, Hk, D], got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
     B, Tq, H, D = q.shape
-    Hk = k.shape[2]
+    Tk, Hk = k.shape[1], k.shape[2]
     if k.shape[0] != B or k.shape[3] != D or Hk == 0 or H == 0 or H % Hk:
         raise ValueError(f"{name}: {H} query heads of {tuple(q.shape)} do not share the KV heads of {tuple(k.shape)}")
-    if (mask.batch, mask.q_len, mask.k_len) != (B, Tq, k.shape[1]):
+    if (mask.batch, mask.q_len, mask.k_len) != (B, Tq, Tk):
         raise ValueError(f"{name}: the mask is for (batch, q_len, k_len) = {(mask.batch, mask.q_len, mask.k_len)}, the tensors have "
-                         f"{(B, Tq, k.shape[1])}")
+                         f"{(B, Tq, Tk)}")
     if not (q.dtype == k.dtype == v.dtype):
         raise ValueError(f"{name}: q, k and v differ in type ({q.dtype}, {k.dtype}, {v.dtype})")
     if not (q.device == k.device == v.device == mask.device):
@@ -363,6 +373,10 @@ def _check(name: str, q, k, v, mask, scale, softcap, slopes):
             raise ValueError(f"native {name} supports bfloat16 and float16 (got {q.dtype})")
         if D % 8 or not 8 <= D <= 128:
             raise ValueError(f"native {name} supports head dims that are multiples of 8 up to 128 (got {D})")
+        if (H + 2 * Hk) * D >= 1 << 24:    # (64 rows have to span less than 2 GiB, packed ones too)
+            raise ValueError(f"native {name} supports tokens of less than 2^24 elements (got {H} + 2 x {Hk} heads of {D})")
+        if B * H * (Tq + Tk) > MAX_GROUPS and largest_launch(B, Tq, Tk, H, Hk, D) > MAX_GROUPS:
+            raise ValueError(f"native {name}: {B} x {Tq} queries of {H} heads over {Tk} keys are more than one launch takes; split the batch")
     elif not q.dtype.is_floating_point:
         raise ValueError(f"{name}: floating-point inputs, got {q.dtype}")
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
