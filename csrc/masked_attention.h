@@ -268,6 +268,7 @@ struct Score {
     // capped score less its bound, -2 capl / (1 + e^(2 u)): the factor rides in the sum's fma
     __device__ __forceinline__ float below(float dot) const { return __builtin_amdgcn_rcpf(fmaf(exp2_fast(dot * c2), c1, c1)); }
     __device__ __forceinline__ float capped(float r) const { return fmaf(-2.f * capl, r, capl); }
+    // dist: the positions' difference, taken in integers (past 2^24 a float does not tell neighbours apart)
     __device__ __forceinline__ float biased(float y, float dist) const {
         return ALIBI ? fmaf(-slope, fabsf(dist), y) : y;
     }

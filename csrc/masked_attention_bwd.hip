@@ -161,7 +161,7 @@ __global__ __launch_bounds__(64 * NW, 2) void mattn_dq_kernel(const Args a) {
     }
     Score<CAP, ALIBI> sc;
     sc.init(a.scale, a.cap, ALIBI ? a.slopes[at.h] : 0.f);
-    const float qpos = ALIBI ? (float)(a.pos[at.b] + qi) : 0.f;
+    const int qpos = ALIBI ? a.pos[at.b] + qi : 0;
 
     const int nq = (a.Tq + QT - 1) / QT, t0 = at.blk * NW;
     int bl = 0x7fffffff, bh = 0, bfl = 0, bfh = 0x7fffffff;
@@ -227,7 +227,7 @@ __global__ __launch_bounds__(64 * NW, 2) void mattn_dq_kernel(const Args a) {
                 s = T::mfma(as_vec<T>(*(const u32x4*)(K_ + at_)), qf[d], s);
                 p = T::mfma(as_vec<T>(*(const u32x4*)(V_ + at_)), df[d], p);
             }
-            const float d0 = ALIBI ? (float)(kb * BN + 32 * t + 4 * h) - qpos : 0.f;
+            const float d0 = ALIBI ? (float)(kb * BN + 32 * t + 4 * h - qpos) : 0.f;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int kk = (i & 3) + 8 * (i >> 2);
@@ -344,7 +344,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void mattn_dkdv_kernel(const
     sc.init(a.scale, a.cap, 0.f);
     const int ex = scale_exponent<T>(a);
     const float up = ldexpf(1.f, ex);
-    const float kpos = ALIBI ? (float)(kj - a.pos[b]) : 0.f;   // the distance to query i is i - kpos
+    const int kpos = ALIBI ? kj - a.pos[b] : 0;   // the distance to query i is i - kpos
 
     const bf16_t* qbase = (const bf16_t*)a.q + b * a.qs[0] + (int64_t)hk * G * a.qs[2];
     const bf16_t* dbase = (const bf16_t*)a.dout + b * a.dos[0] + (int64_t)hk * G * a.dos[2];
@@ -440,7 +440,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void mattn_dkdv_kernel(const
     auto init_b = [&](const At& x) {
         if (ALIBI) {
             sc.slope = a.slopes[hk * G + x.g] * LOG2E;
-            d0 = (float)(x.t * QT + 4 * h) - kpos;
+            d0 = (float)(x.t * QT + 4 * h - kpos);
         }
     };
     auto score = [&](Scores& y, auto xc, float ls) __attribute__((always_inline)) {

@@ -194,7 +194,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void mattn_fwd_kernel(const 
     if (qi >= a.Tq) lo = hi = 0;
     Score<CAP, ALIBI> sc;
     sc.init(a.scale, a.cap, ALIBI ? a.slopes[at.h] : 0.f);
-    const float qpos = ALIBI ? (float)(a.pos[at.b] + qi) : 0.f;
+    const int qpos = ALIBI ? a.pos[at.b] + qi : 0;
 
     // bounds of the intervals over the workgroup's and the wave's queries
     const int nq = (a.Tq + QT - 1) / QT, t0 = at.blk * NW;
@@ -265,7 +265,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void mattn_fwd_kernel(const 
 #pragma unroll
                 for (int i = 0; i < 16; ++i) s[t][i] = sc.below(s[t][i]);
         } else if constexpr (!Score<CAP, ALIBI>::PLAIN) {
-            const float d0 = (float)(kb * BN + 4 * h) - qpos;
+            const float d0 = (float)(kb * BN + 4 * h - qpos);
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -416,7 +416,7 @@ __global__ __launch_bounds__(256, 2) void mattn_few_kernel(const Args a) {
     const int fl = wave_max_i(r < nr ? lo : 0), fh = wave_min_i(r < nr ? hi : 0x7fffffff);   // every row sees [fl, fh)
     Score<CAP, ALIBI> sc;
     sc.init(a.scale, a.cap, ALIBI ? a.slopes[hq] : 0.f);
-    const float qpos = ALIBI ? (float)(a.pos[b] + i0) : 0.f;
+    const int qpos = ALIBI ? a.pos[b] + i0 : 0;
     f32x16 o[NO];
 #pragma unroll
     for (int i = 0; i < NO; ++i) o[i] = (f32x16){};
@@ -461,7 +461,7 @@ __global__ __launch_bounds__(256, 2) void mattn_few_kernel(const Args a) {
         for (int d = 0; d < NS; ++d) s = T::mfma(as_vec<T>(kr[d]), qf[d], s);
         if (u + NW < u1) gload(u + NW);
         if constexpr (!Score<CAP, ALIBI>::PLAIN) {
-            const float d0 = (float)(kb + 4 * h) - qpos;
+            const float d0 = (float)(kb + 4 * h - qpos);
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] = sc(s[i], d0 + (float)((i & 3) + 8 * (i >> 2)));
         }

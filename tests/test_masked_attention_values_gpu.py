@@ -83,6 +83,31 @@ def test_fp16_gradients_of_large_values(aligned, size, T, D, cap):
         oracle.check(g, (want[n][0], want[n][1] + more.get(n, 0.0)), n)
 
 
+@pytest.mark.parametrize("Tq", [3, 70])
+@pytest.mark.parametrize("cap", [None, 10.0])
+def test_distances_at_far_positions(Tq, cap):
+    """Positions past 2^24, where neighbours are the same number in 32 bits: the distances are those of the
+    same tokens at the start of a row."""
+    from trustworthy_dl import ops
+    D, far, n = 8, (1 << 24) + 12345, 150
+    Tk = far + n
+    q, do = _rand(0, 1, Tq, 2, D), _rand(3, 1, Tq, 2, D)
+    ks, vs = _rand(1, 1, n, 1, D), _rand(2, 1, n, 1, D)
+    k, v = (torch.zeros(1, Tk, 1, D, dtype=BF, device=DEV) for _ in range(2))
+    k[:, far:], v[:, far:] = ks, vs
+    ids = torch.zeros(1, Tk, dtype=torch.int32, device=DEV)
+    ids[:, far:] = 1
+    slopes = torch.tensor([0.7, 0.21], device=DEV)
+    got = _grads(q, k, v, do, ops.attention_mask(1, Tq, Tk, documents=ids), softcap=cap, slopes=slopes)
+    near = ops.attention_mask(1, Tq, n, device=DEV)
+    want = oracle.run(q, ks, vs, near.dense(), near.pos.long(), 1 / math.sqrt(D), cap or 0.0, slopes, do)
+    for name in ("out", "dq"):
+        oracle.check(got[name], want[name], name)
+    for name in ("dk", "dv"):
+        assert (got[name][:, :far] == 0).all()
+        oracle.check(got[name][:, far:], want[name], name)
+
+
 def test_operands_cut_from_a_flat_buffer():
     """q, k, v and the upstream gradient, dense and at an odd offset, give what aligned copies give."""
     from trustworthy_dl import ops
