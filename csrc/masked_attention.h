@@ -43,8 +43,10 @@ struct Args {
     float scale, cap;
 };
 
+// UP: a softmax's weights are rounded times 2^UP; bf16 has fp32's range
 struct Bf16 {
     typedef bf16x8 vec;
+    static constexpr int UP = 0;
     static constexpr uint32_t INF = 0x7f80, NANBITS = 0x7fc0;
     static __device__ __forceinline__ f32x16 mfma(vec a, vec b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
@@ -58,8 +60,13 @@ struct Bf16 {
         b = __uint_as_float(w & 0xffff0000u);
     }
 };
+// Weights are at most 1, and fp16 rounds those below 2^-14 to steps of 2^-24: a long row's small weights were off by
+// half a step each, all alike where they are equal.  2^12 times the weight leaves its normal range at 2^-26, for
+// the price of a constant in the exponent; the factor cancels against the row's sum (forward) or goes with
+// the last scale (backward), and room for weights up to 15 is left (a log-sum-exp rounded low).
 struct F16 {
     typedef f16x8 vec;
+    static constexpr int UP = 12;
     static constexpr uint32_t INF = 0x7c00, NANBITS = 0x7e00;
     static __device__ __forceinline__ f32x16 mfma(vec a, vec b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);

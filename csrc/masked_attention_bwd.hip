@@ -155,7 +155,7 @@ __global__ __launch_bounds__(64 * NW, 2) void mattn_dq_kernel(const Args a) {
         const int tp = (a.Tq + QT - 1) / QT * QT;
         float* st = a.delta + ((int64_t)at.b * a.H + at.h) * 2 * tp;
         if (h == 0 && qi < tp) {
-            st[qi] = qi < a.Tq ? lse2 : INFINITY;
+            st[qi] = qi < a.Tq ? lse2 - (float)T::UP : INFINITY;   // (dK / dV's weights: times 2^UP)
             st[tp + qi] = qi < a.Tq ? -delta : 0.f;
         }
     }
@@ -310,7 +310,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void mattn_dkdv_kernel(const
     typedef typename T::vec vec;
     constexpr int IMG = QT * DP;
     __shared__ __attribute__((aligned(16))) bf16_t tiles[RING][2 * IMG];   // Q, then dO
-    // per query row: lse log2(e), -delta, lo, hi
+    // per query row: lse log2(e) - UP, -delta, lo, hi
     __shared__ __attribute__((aligned(16))) uint32_t rowc[RING][4 * QT];
     __shared__ __attribute__((aligned(16))) uint8_t qflag[RING][QT * (DP / 8)], dflag[RING][QT * (DP / 8)];
     const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, r = lane & 31;
@@ -343,7 +343,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void mattn_dkdv_kernel(const
     Score<CAP, ALIBI> sc;
     sc.init(a.scale, a.cap, 0.f);
     const int ex = scale_exponent<T>(a);
-    const float up = ldexpf(1.f, ex);
+    const float up = ldexpf(1.f, ex - T::UP);   // (the weights have the rest)
     const int kpos = ALIBI ? kj - a.pos[b] : 0;   // the distance to query i is i - kpos
 
     const bf16_t* qbase = (const bf16_t*)a.q + b * a.qs[0] + (int64_t)hk * G * a.qs[2];
@@ -622,7 +622,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void mattn_dkdv_kernel(const
     }
     if (total > 0) run(Y, N, N, cur, e0, y0, y1, (total - 1) & (RING - 1), 0, 0);
     if constexpr (DP == 128) acc_done(dk, dv);
-    const float gscale = (CAP ? 4.f * a.scale : a.scale) * ldexpf(1.f, -ex);
+    const float gscale = (CAP ? 4.f * a.scale : a.scale) * ldexpf(1.f, -ex), vscale = ldexpf(1.f, -T::UP);
     if (kj < a.Tk) {
         bf16_t* dkr = (bf16_t*)a.dk + b * a.dks[0] + hk * a.dks[2] + (int64_t)kj * a.dks[1];
         bf16_t* dvr = (bf16_t*)a.dv + b * a.dvs[0] + hk * a.dvs[2] + (int64_t)kj * a.dvs[1];
@@ -640,8 +640,8 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void mattn_dkdv_kernel(const
                 uint2 u, v;
                 u.x = T::pack(dk[i][4 * g] * gscale, dk[i][4 * g + 1] * gscale);
                 u.y = T::pack(dk[i][4 * g + 2] * gscale, dk[i][4 * g + 3] * gscale);
-                v.x = T::pack(dv[i][4 * g], dv[i][4 * g + 1]);
-                v.y = T::pack(dv[i][4 * g + 2], dv[i][4 * g + 3]);
+                v.x = T::pack(dv[i][4 * g] * vscale, dv[i][4 * g + 1] * vscale);
+                v.y = T::pack(dv[i][4 * g + 2] * vscale, dv[i][4 * g + 3] * vscale);
                 if (poison) u.x = u.y = v.x = v.y = T::NANBITS | T::NANBITS << 16;
                 if (d < a.D) {
                     *(uint2*)(dkr + d) = u;

@@ -299,11 +299,12 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void mattn_fwd_kernel(const 
             m = mn;
         }
         float rs = 0.f;
+        const float mu = ms - (float)T::UP;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                s[t][i] = exp2_fast(Score<CAP, ALIBI>::PLAIN ? fmaf(s[t][i], sc.mul, -ms) : fixed ? s[t][i] : s[t][i] - ms);
+                s[t][i] = exp2_fast(Score<CAP, ALIBI>::PLAIN ? fmaf(s[t][i], sc.mul, -mu) : fixed ? s[t][i] : s[t][i] - mu);
                 rs += s[t][i];
             }
         l += rs;   // this half's keys; the halves are added at the end
@@ -361,7 +362,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void mattn_fwd_kernel(const 
                 }
             }
         if (h == 0 && a.lse != nullptr)
-            a.lse[((int64_t)at.b * a.H + at.h) * a.Tq + qi] = l == 0.f ? -INFINITY : (m + (SAT ? sc.capl : 0.f) + log2f(l)) * LN2;
+            a.lse[((int64_t)at.b * a.H + at.h) * a.Tq + qi] = l == 0.f ? -INFINITY : (m + (SAT ? sc.capl : 0.f) + (log2f(l) - T::UP)) * LN2;
     }
 }
 
@@ -486,9 +487,10 @@ __global__ __launch_bounds__(256, 2) void mattn_few_kernel(const Args a) {
             for (int i = 0; i < NO; ++i) o[i] *= alpha;
         }
         m = mn;
+        const float mu = ms - (float)T::UP;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            s[i] = exp2_fast(Score<CAP, ALIBI>::PLAIN ? fmaf(s[i], sc.mul, -ms) : s[i] - ms);
+            s[i] = exp2_fast(Score<CAP, ALIBI>::PLAIN ? fmaf(s[i], sc.mul, -mu) : s[i] - mu);
             l += s[i];
         }
         if (part) {
@@ -563,7 +565,7 @@ __global__ __launch_bounds__(256, 2) void mattn_few_kernel(const Args a) {
         } else {
             const float inv = L == 0.f ? 0.f : 1.f / L;
             put_out<T>(a, acc, inv, b, hh, ii, d);
-            if (d == 0 && a.lse != nullptr) a.lse[out] = L == 0.f ? -INFINITY : (M + log2f(L)) * LN2;
+            if (d == 0 && a.lse != nullptr) a.lse[out] = L == 0.f ? -INFINITY : (M + (log2f(L) - T::UP)) * LN2;
         }
     }
     }
@@ -597,7 +599,7 @@ __global__ __launch_bounds__(256) void mattn_join_kernel(const Args a) {
     const int64_t bh = out / a.Tq;
     const int ii = (int)(out - bh * a.Tq), b = (int)(bh / a.H), hh = (int)(bh - (int64_t)b * a.H);
     put_out<T>(a, acc, inv, b, hh, ii, d);
-    if (d == 0 && a.lse != nullptr) a.lse[out] = L == 0.f ? -INFINITY : (M + log2f(L)) * LN2;
+    if (d == 0 && a.lse != nullptr) a.lse[out] = L == 0.f ? -INFINITY : (M + (log2f(L) - T::UP)) * LN2;
 }
 
 // ============================================================================ host

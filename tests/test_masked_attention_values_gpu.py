@@ -83,6 +83,38 @@ def test_fp16_gradients_of_large_values(aligned, size, T, D, cap):
         oracle.check(g, (want[n][0], want[n][1] + more.get(n, 0.0)), n)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_fp16_weights_of_long_rows(D):
+    """166937 keys of equal weight, 2^24 / 100.5 of them: a weight rounded below fp16's normal range would be
+    half a step, 0.5 %, off in every term alike."""
+    from trustworthy_dl import ops
+    Tq, Tk = 40, 166937
+    q = torch.zeros(1, Tq, 1, D, dtype=HF, device=DEV)
+    k, v = _rand(1, 1, Tk, 1, D, dtype=HF), _rand(2, 1, Tk, 1, D, dtype=HF)
+    do = torch.ones(1, Tq, 1, D, dtype=HF, device=DEV)
+    mask = ops.attention_mask(1, Tq, Tk, causal=False, device=DEV)
+    dv = _grads(q, k, v, do, mask)["dv"].double()
+    exact = Tq / Tk
+    # P and the result are rounded once each (2^-11), the rest is in 32 bits (2^-13)
+    assert ((dv - exact).abs() <= (2.0 ** -10 + 2.0 ** -12) * exact).all()
+
+
+@pytest.mark.parametrize("Tq", [1, 5, 40, 130])
+@pytest.mark.parametrize("D", [64, 128])
+def test_fp16_small_weights_beside_a_large_one(Tq, D):
+    """One key has nearly all the weight, and the others, 2^-25 of it each, half a percent together."""
+    from trustworthy_dl import ops
+    Tk = 166937
+    q, k = torch.zeros(1, Tq, 2, D, dtype=HF, device=DEV), torch.zeros(1, Tk, 1, D, dtype=HF, device=DEV)
+    q[..., 0], k[:, 5, :, 0] = 8.0, 17.375 / 8.0 * math.sqrt(D)
+    v = torch.ones(1, Tk, 1, D, dtype=HF, device=DEV)
+    v[:, 5] = 0
+    mask = ops.attention_mask(1, Tq, Tk, causal=False, device=DEV)
+    got = ops.masked_attention(q, k, v, mask).double()
+    want = oracle.run(q, k, v, mask.dense(), mask.pos.long(), 1 / math.sqrt(D))["out"][0]
+    assert ((got - want).abs() <= (2.0 ** -10 + 2.0 ** -12) * want).all()
+
+
 @pytest.mark.parametrize("Tq", [3, 70])
 @pytest.mark.parametrize("cap", [None, 10.0])
 def test_distances_at_far_positions(Tq, cap):
