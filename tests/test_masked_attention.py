@@ -191,3 +191,14 @@ def test_library_refuses_arguments_out_of_range():
         if "nsplit" not in kw or kw["B"] > 1 << 23:
             assert _lib.lib().tdl_masked_attn_bwd(ctypes.addressof(a), None) == 1, kw
     assert _lib.lib().tdl_attn_mask(None, 0, None, None, None, None, 1 << 22, 1, 1, 1, None, None, None, None, None, None, None) == 1
+
+
+def test_scales_out_of_range_and_slopes_that_are_no_tensor():
+    m = ops.attention_mask(2, 4)
+    q, k = torch.zeros(2, 4, 4, 8), torch.zeros(2, 4, 2, 8)
+    for s in (1e-50, 1e-31, 1e31, 1e39, 1e300):      # (1e-50 is 0 in 32 bits, 1e39 infinite)
+        _bad(lambda: ops.masked_attention(q, k, k, m, scale=s), "scale")
+    for s in (1e-30, 1e30):
+        for c in (None, 1e-6, 1000.0):
+            assert torch.isfinite(ops.masked_attention(q, k, k, m, scale=s, softcap=c)).all()
+    _bad(lambda: ops.masked_attention(q, k, k, m, slopes=[0.1] * 4), "slopes must be")

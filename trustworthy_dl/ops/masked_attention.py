@@ -27,6 +27,7 @@ from ._lib import ptr
 
 _Q_TILE, _K_TILE = 32, 128     # csrc/masked_attention.h QT, KT
 MIN_SOFTCAP, MAX_SOFTCAP = 1e-6, 1000.0
+MIN_SCALE, MAX_SCALE = 1e-30, 1e30      # (with any softcap, the products of them that the kernels take stay in fp32's range)
 
 
 # ============================================================== the mask
@@ -380,14 +381,16 @@ def _check(name: str, q, k, v, mask, scale, softcap, slopes):
     elif not q.dtype.is_floating_point:
         raise ValueError(f"{name}: floating-point inputs, got {q.dtype}")
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    if not (scale > 0 and math.isfinite(scale)):
-        raise ValueError(f"{name}: scale must be positive, got {scale}")
+    if not MIN_SCALE <= scale <= MAX_SCALE:
+        raise ValueError(f"{name}: scale must lie in [{MIN_SCALE:g}, {MAX_SCALE:g}], got {scale}")
     cap = 0.0 if softcap is None else float(softcap)
     if softcap is not None and not MIN_SOFTCAP <= cap <= MAX_SOFTCAP:
         # cap tanh(x / cap) is evaluated to cap x 2^-21: beyond this the cap's own rounding would show (and
         # below it scale / cap would leave fp32's range)
         raise ValueError(f"{name}: softcap must lie in [{MIN_SOFTCAP:g}, {MAX_SOFTCAP:g}], got {softcap}")
     if slopes is not None:
+        if not isinstance(slopes, torch.Tensor):
+            raise ValueError(f"{name}: slopes must be a [{H}] tensor, got {type(slopes).__name__}")
         if slopes.shape != (H,) or slopes.device != q.device:
             raise ValueError(f"{name}: slopes must be a [{H}] tensor on {q.device}, got {tuple(slopes.shape)} on {slopes.device}")
         if slopes.requires_grad:
