@@ -142,3 +142,10 @@ def test_library_refuses_sizes_out_of_range():
     for kw in (dict(M=0), dict(M=MAX_DIM + 1), dict(W=MAX_DIM + 1), dict(V=10), dict(V=0), dict(K=0), dict(K=1025), dict(G=0), dict(dtype=3),
                dict(tau=0.0), dict(alpha=1.5), dict(alpha=0.5, beta=0.5), dict(rows=0)):
         assert refused(**kw), kw
+
+
+def test_a_single_row_and_a_single_entry():
+    z, idx, t, _ = inputs(1, 9, 9, 3)
+    assert torch.equal(ops.distillation_loss(z[0], idx[0], t[0]), ops.distillation_loss(z, idx, t))
+    with pytest.raises(ValueError, match="same rows"):
+        ops.distillation_loss(z[0], idx[0, 0], t[0, 0])

@@ -147,7 +147,7 @@ def distillation_loss(logits: torch.Tensor, teacher_index: torch.Tensor, teacher
     V = W if num_classes is None else int(num_classes)
     if not 1 <= V <= W:
         raise ValueError(f"distillation_loss: num_classes must lie in [1, {W}], got {V}")
-    if teacher_index.shape != teacher_logits.shape or teacher_index.shape[:-1] != logits.shape[:-1]:
+    if teacher_index.dim() == 0 or teacher_index.shape != teacher_logits.shape or teacher_index.shape[:-1] != logits.shape[:-1]:
         raise ValueError(f"distillation_loss: logits {tuple(logits.shape)}, teacher_index {tuple(teacher_index.shape)}, teacher_logits "
                          f"{tuple(teacher_logits.shape)} do not name the same rows")
     K = teacher_index.shape[-1]
