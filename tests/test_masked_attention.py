@@ -202,3 +202,23 @@ def test_scales_out_of_range_and_slopes_that_are_no_tensor():
         for c in (None, 1e-6, 1000.0):
             assert torch.isfinite(ops.masked_attention(q, k, k, m, scale=s, softcap=c)).all()
     _bad(lambda: ops.masked_attention(q, k, k, m, slopes=[0.1] * 4), "slopes must be")
+
+
+@pytest.mark.parametrize("cap", [None, 2.0])
+def test_padding_has_no_effect_on_gradients(cap):
+    """NaN and infinities in the queries, keys, values and upstream gradients of padded positions."""
+    ids = torch.tensor([[0, 0, 1, 1, 1, -1, -1], [2, 2, 2, 2, 3, 3, -1]], dtype=torch.int32)
+    m = ops.attention_mask(2, 7, documents=ids)
+    ins = [_rand(2, 7, h, 8, seed=i) for i, h in enumerate((4, 2, 2, 4))]
+    slopes = torch.tensor([0.1, 0.2, 0.3, 0.4])
+
+    def run():
+        q, k, v = (t.clone().requires_grad_(True) for t in ins[:3])
+        out = ops.masked_attention(q, k, v, m, softcap=cap, slopes=slopes)
+        return (out.detach(), *torch.autograd.grad(out, (q, k, v), ins[3]))
+    clean = run()
+    for bad in (math.nan, math.inf):
+        for t in ins:
+            t[ids < 0] = bad
+        for a, b in zip(clean, run()):
+            assert torch.equal(a, b)

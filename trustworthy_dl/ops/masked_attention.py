@@ -331,10 +331,12 @@ def _reference(q, k, v, mask, scale, cap, slopes):
     B, Tq, H, D = q.shape
     G = H // k.shape[2]
     seen = mask.dense()
-    # a key that no query of its row sees takes no part, whatever stands there
+    # a key that no query of its row sees takes no part, nor does a query that sees nothing or its upstream gradient,
+    # whatever stands there
     used = seen.any(1)[:, :, None, None] if Tq else torch.zeros(B, k.shape[1], 1, 1, dtype=torch.bool, device=k.device)
-    qf = q.to(wide).transpose(1, 2)
-    kf, vf = (torch.where(used, t.to(wide), torch.zeros((), dtype=wide)).transpose(1, 2).repeat_interleave(G, 1) for t in (k, v))
+    sees, none = seen.any(-1)[:, :, None, None], torch.zeros((), dtype=wide, device=q.device)
+    qf = torch.where(sees, q.to(wide), none).transpose(1, 2)
+    kf, vf = (torch.where(used, t.to(wide), none).transpose(1, 2).repeat_interleave(G, 1) for t in (k, v))
     s = (qf @ kf.transpose(-1, -2)) * scale
     if cap:
         s = cap * torch.tanh(s / cap)
@@ -349,7 +351,7 @@ def _reference(q, k, v, mask, scale, cap, slopes):
     z = e.sum(-1, keepdim=True)
     out = (e / torch.where(z == 0, torch.ones_like(z), z)) @ vf
     lse = torch.where(z == 0, torch.full_like(z, float("-inf")), top + torch.log(z))[..., 0].detach().float()
-    return out.transpose(1, 2).to(q.dtype), lse
+    return torch.where(sees, out.transpose(1, 2), none).to(q.dtype), lse
 
 
 # ============================================================== entry points
@@ -410,7 +412,8 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: At
     h // (H / Hk)); any batch / token / head strides.  ``scale`` defaults to 1 / sqrt(D); without
     ``softcap`` the scores are not capped, without ``slopes`` (fp32 [H]) there is no distance bias
     (p, j: positions of query and key).  Returns [B, Tq, H, D] in q's type; a query that sees nothing
-    gives zeros, and keys it does not see have no effect on it, whatever they hold.  With
+    gives zeros, and keys it does not see have no effect on it, whatever they hold (on the CPU: keys that no
+    query of the row sees).  Scores are kept in 32 bits: at a size of S their weights are known to S 2^-21.  With
     ``return_lse`` also the fp32 log-sum-exp of each query's scores [B, H, Tq] (-inf where it sees
     nothing; not differentiable)."""
     scale, cap, slopes = _check("masked_attention", q, k, v, mask, scale, softcap, slopes)
