@@ -274,3 +274,30 @@ def test_sizes_out_of_range_are_refused():
     q, k = one.expand(n, 1, 512, 8), one.expand(n, 1, 32, 8)
     with pytest.raises(ValueError, match="split the batch"):
         ops.masked_attention(q, k, k, mask)
+
+
+def test_a_mask_dropped_while_another_stream_uses_it():
+    """record_stream keeps the mask's memory from its own stream's next tensors until the other is done."""
+    from trustworthy_dl import ops
+    B, T = 2, 512
+    ids = (torch.arange(T, device=DEV) // 100).int().expand(B, T)
+    q, k, v = (_rand(i, B, T, 4, 64) for i in range(3))
+    want = ops.masked_attention(q, k, v, ops.attention_mask(B, T, documents=ids))
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    mask = ops.attention_mask(B, T, documents=ids)
+    held = {t.data_ptr() for t in (mask.lo, mask.hi, mask.pos, mask.q_table, mask.k_table)}
+    shapes = [(t.shape, t.dtype) for t in (mask.lo, mask.hi, mask.pos, mask.q_table, mask.k_table)]
+    side.wait_stream(torch.cuda.current_stream())
+    big = _rand(7, 4096, 4096)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(30):      # (work ahead of the call on the side stream)
+            big = (big @ big).clamp(-1, 1)
+        got = ops.masked_attention(q, k, v, mask)
+    mask.record_stream(side)
+    del mask
+    fresh = [torch.zeros(s, dtype=d, device=DEV) for s, d in shapes]
+    assert side.query() or not held & {t.data_ptr() for t in fresh}
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)

@@ -35,7 +35,8 @@ class AttentionMask:
     """Which keys each query of a batch sees: ``lo[b, i] <= j < hi[b, i]`` (``attention_mask``).
 
     Made from its inputs once; later changes of those tensors are not seen.  Like any tensor, a mask
-    built on one stream is used on another only after that stream has waited for the first."""
+    built on one stream is used on another only after that stream has waited for the first, and is told of it
+    (``record_stream``) where it may be dropped before the other stream's work is done."""
 
     def __init__(self, batch: int, q_len: int, k_len: int, lo: torch.Tensor, hi: torch.Tensor, pos: torch.Tensor,
                  q_table: Optional[torch.Tensor], k_table: Optional[torch.Tensor]):
@@ -46,6 +47,11 @@ class AttentionMask:
     @property
     def device(self) -> torch.device:
         return self.lo.device
+
+    def record_stream(self, stream: torch.cuda.Stream) -> None:
+        """``Tensor.record_stream`` for the mask's memory: it is not used again before ``stream``'s work so far is done."""
+        for t in self._tensors():
+            t.record_stream(stream)
 
     def _tensors(self):   # as _forward and _backward take them
         return self.lo, self.hi, self.pos, self.q_table, self.k_table
