@@ -267,7 +267,7 @@ __global__ __launch_bounds__(NT, 4) void distill_kernel(const DistillArgs a) {
                 const float t = i >= 0 ? teacher_at(a, at) : -INFINITY;
                 sidx[k] = i;
                 su[k] = t;
-                sz[k] = i >= 0 ? T::get(z[i]) : 0.f;   // (before the row is overwritten: grad may be the logits)
+                sz[k] = i >= 0 ? T::get(z[i]) : 0.f;
                 tm = fmaxf(tm, t);
                 nan += t == t ? 0.f : 1.f;
                 any += i >= 0 ? 1.f : 0.f;

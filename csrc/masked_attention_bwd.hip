@@ -93,9 +93,9 @@ __device__ __forceinline__ int scale_exponent(const Args& a) {
 // score, 48 of them products.  Two waves a SIMD (three, for heads of 64: 88 against 85 us on 16 x 1024).
 // 2 x 8192, 16 heads of 128 on 4, cap 50: 942 us (one wave a SIMD, tiles through registers: 1656 us);
 // 16 x 1024 in documents, 16 heads of 64: 70 us.
-template <class T, int DP, bool CAP, bool ALIBI, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void mattn_dq_kernel(const Args a) {
-    constexpr int BM = QT * NW, BN = 64, NS = DP / 16, NO = DP / 32, NTHR = 64 * NW;
+template <class T, int DP, bool CAP, bool ALIBI>
+__global__ __launch_bounds__(256, 2) void mattn_dq_kernel(const Args a) {
+    constexpr int NW = 4, BM = QT * NW, BN = 64, NS = DP / 16, NO = DP / 32, NTHR = 64 * NW;
     typedef Copy<T, DP, BN, NTHR> CP;
     __shared__ __attribute__((aligned(16))) bf16_t Ks[2][BN * DP];
     __shared__ __attribute__((aligned(16))) bf16_t Vs[2][BN * DP];
@@ -662,7 +662,7 @@ static int bwd_launch(const Args& a, hipStream_t s) {
         rc = (int)hipGetLastError();
         if (rc) return rc;
     }
-    mattn_dq_kernel<T, DP, CAP, ALIBI, 4><<<(int)gq, 256, 0, s>>>(a);
+    mattn_dq_kernel<T, DP, CAP, ALIBI><<<(int)gq, 256, 0, s>>>(a);
     rc = (int)hipGetLastError();
     if (rc || a.dk == nullptr) return rc;   // no gradient of the keys and values wanted
     mattn_dkdv_kernel<T, DP, CAP, ALIBI><<<(int)gk, 256, 0, s>>>(a);
