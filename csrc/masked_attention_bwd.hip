@@ -19,54 +19,67 @@ using namespace mattn;
 // First the largest squares of row norms (not finite elements left out: they make their rows NaN anyhow),
 // one of each kind per workgroup.
 constexpr int NMAX = 256;
-// whether some query of batch row b sees key j
-__device__ __forceinline__ bool key_seen(const Args& a, int b, int j) {
-    const int nq = (a.Tq + QT - 1) / QT, nk = (a.Tk + KT - 1) / KT;
-    const int2 range = a.ktab[(int64_t)b * nk + j / KT];
-    for (int t = range.x; t < range.y; ++t) {
-        const int4 e = a.qtab[(int64_t)b * nq + t];
-        if (j < e.x || j >= e.y) continue;
-        if (j >= e.z && j < e.w) return true;
-        for (int i = t * QT; i < min(t * QT + QT, a.Tq); ++i)
-            if (j >= a.lo[(int64_t)b * a.Tq + i] && j < a.hi[(int64_t)b * a.Tq + i]) return true;
-    }
-    return false;
-}
-template <class T>
+// A wave takes 64 rows: (token, head) of dO, then neighbouring keys of a head of V, all loads of a row on their
+// way at once.  Bound by latency: 4 x 777, 12 heads of 64: 10 us (a thread per key over all heads: 48 us).
+template <class T, int DP>
 __device__ __forceinline__ float row_square(const bf16_t* row, int D) {
+    u32x4 u[DP / 8];
+#pragma unroll
+    for (int c = 0; c < DP / 8; ++c) u[c] = *(const u32x4*)(row + (8 * c < D ? 8 * c : 0));
     float s = 0.f;
-    for (int c = 0; c < D; c += 8) {
-        const u32x4 u = finite_only<T>(*(const u32x4*)(row + c));
+#pragma unroll
+    for (int c = 0; c < DP / 8; ++c) {
+        u[c] = finite_only<T>(u[c]);
+        float t = 0.f;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             float x, y;
-            T::unpack(u[k], x, y);
-            s = fmaf(x, x, fmaf(y, y, s));
+            T::unpack(u[c][k], x, y);
+            t = fmaf(x, x, fmaf(y, y, t));
         }
+        s += 8 * c < D ? t : 0.f;
     }
     return s;
 }
-template <class T>
+// whether some query of batch row b sees the lane's key j (64 neighbours of one ktab block, j < Tk)
+__device__ __forceinline__ bool key_seen(const Args& a, int b, int block, int j) {
+    const int nq = (a.Tq + QT - 1) / QT, nk = (a.Tk + KT - 1) / KT, lane = threadIdx.x & 63;
+    const int2 range = a.ktab[(int64_t)b * nk + block];
+    bool seen = false;
+    for (int t = range.x; t < range.y && !__all(seen || j >= a.Tk); ++t) {
+        const int4 e = a.qtab[(int64_t)b * nq + t];
+        seen |= j >= e.z && j < e.w;                          // all rows of the tile see it
+        if (!__any(!seen && j >= e.x && j < e.y)) continue;   // (no row sees any other)
+        const int i = min(t * QT + (lane & 31), a.Tq - 1);
+        const int lo = a.lo[(int64_t)b * a.Tq + i], hi = a.hi[(int64_t)b * a.Tq + i];
+#pragma unroll
+        for (int r = 0; r < QT; ++r) seen |= j >= __builtin_amdgcn_readlane(lo, r) && j < __builtin_amdgcn_readlane(hi, r);
+    }
+    return seen && j < a.Tk;
+}
+template <class T, int DP>
 __global__ __launch_bounds__(256) void mattn_norm_max_kernel(const Args a) {
     __shared__ uint32_t red[2][4];
     float m[2] = {0.f, 0.f};
-    const int64_t first = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    for (int64_t x = first; x < (int64_t)a.B * a.Tq * a.H; x += NMAX * 256) {
+    const int64_t rows = (int64_t)a.B * a.Tq * a.H;
+    for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < rows; x += NMAX * 256) {
         const int64_t row = x / a.H, b = row / a.Tq;
         const int hh = (int)(x - row * a.H), t = (int)(row - b * a.Tq);
-        if (a.lo[row] >= a.hi[row]) continue;
-        m[0] = fmaxf(m[0], row_square<T>((const bf16_t*)a.dout + b * a.dos[0] + t * a.dos[1] + hh * a.dos[2], a.D));
+        const float q = row_square<T, DP>((const bf16_t*)a.dout + b * a.dos[0] + t * a.dos[1] + hh * a.dos[2], a.D);
+        m[0] = fmaxf(m[0], a.lo[row] < a.hi[row] ? q : 0.f);
     }
-    for (int64_t x = first; x < (int64_t)a.B * a.Tk; x += NMAX * 256) {
-        const int b = (int)(x / a.Tk), j = (int)(x - (int64_t)b * a.Tk);
-        if (!key_seen(a, b, j)) continue;
-        for (int hh = 0; hh < a.Hk; ++hh)
-            m[1] = fmaxf(m[1], row_square<T>((const bf16_t*)a.v + b * a.vs[0] + j * a.vs[1] + hh * a.vs[2], a.D));
+    const int nb = (a.Tk + 63) / 64;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    for (int64_t x = (int64_t)blockIdx.x * 4 + w; x < (int64_t)a.B * nb * a.Hk; x += NMAX * 4) {
+        const int64_t y = x / nb;
+        const int kb = (int)(x - y * nb), b = (int)(y / a.Hk), hh = (int)(y - (int64_t)b * a.Hk), j = kb * 64 + (threadIdx.x & 63);
+        const float q = row_square<T, DP>((const bf16_t*)a.v + b * a.vs[0] + min(j, a.Tk - 1) * a.vs[1] + hh * a.vs[2], a.D);
+        m[1] = fmaxf(m[1], key_seen(a, b, kb * 64 / KT, j) ? q : 0.f);
     }
 #pragma unroll
     for (int k = 0; k < 2; ++k) {   // (not negative: ordered as their bits)
-        const int w = wave_max_i((int)__float_as_uint(m[k]));
-        if ((threadIdx.x & 63) == 0) red[k][threadIdx.x >> 6] = (uint32_t)w;
+        const int v = wave_max_i((int)__float_as_uint(m[k]));
+        if ((threadIdx.x & 63) == 0) red[k][w] = (uint32_t)v;
     }
     __syncthreads();
     if (threadIdx.x < 2) {
@@ -658,7 +671,7 @@ static int bwd_launch(const Args& a, hipStream_t s) {
     if (gq > MAX_GRID || gk > MAX_GRID) return (int)hipErrorInvalidValue;
     int rc = 0;
     if (T::INF != 0x7f80) {
-        mattn_norm_max_kernel<T><<<NMAX, 256, 0, s>>>(a);
+        mattn_norm_max_kernel<T, DP><<<NMAX, 256, 0, s>>>(a);
         rc = (int)hipGetLastError();
         if (rc) return rc;
     }
