@@ -15,6 +15,7 @@ from __future__ import annotations
 import ctypes
 import os
 import threading
+import weakref
 from typing import Optional
 
 import torch
@@ -230,17 +231,25 @@ def call_on(device: torch.device, name: str, *args):
             call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
-def kept(*tensors):
-    """What ``came_back`` compares saved tensors with."""
-    return [None if t is None else (t.shape, t.dtype) for t in tensors]
+def keep(ctx, *tensors):
+    """``ctx.save_for_backward``, with a note of which tensors they were (``came_back``)."""
+    ctx.save_for_backward(*tensors)
+    ctx.kept = [None if t is None else weakref.ref(t) for t in tensors]
 
 
-def came_back(name: str, tensors, was, device: torch.device):
-    """The tensors that autograd kept for a backward pass: saved-tensor hooks may bring back others, and a
-    kernel reads what it is given, so they have to be of the same shapes and types and on the device."""
-    for t, w in zip(tensors, was):
-        if t is not None and ((t.shape, t.dtype) != w or t.device != device):
-            raise RuntimeError(f"{name}: a saved tensor of {tuple(w[0])} {w[1]} on {device} came back as {tuple(t.shape)} {t.dtype} on {t.device}")
+def came_back(name: str, ctx, device: torch.device, was, layout):
+    """The tensors of ``keep``.  Saved-tensor hooks may bring back others, and a kernel reads what it is given: one
+    that is not the tensor that was kept (an output never is) has to be of the same shape and type, ``was(i)``, and on
+    the device, and goes through ``layout(i, t)``.  (Small calls are bound by the host: identity is the cheapest test.)"""
+    saved = list(ctx.saved_tensors)
+    for i, (t, ref) in enumerate(zip(saved, ctx.kept)):
+        if ref is not None and ref() is not t:
+            shape, dtype = was(i)
+            if t.shape != shape or t.dtype is not dtype or t.device != device:
+                raise RuntimeError(f"{name}: a saved tensor of {tuple(shape)} {dtype} on {device} came back as {tuple(t.shape)} {t.dtype} "
+                                   f"on {t.device}")
+            saved[i] = layout(i, t)
+    return saved
 
 
 def dense(t: torch.Tensor) -> torch.Tensor:

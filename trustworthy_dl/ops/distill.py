@@ -56,16 +56,11 @@ def _alike(z: torch.Tensor, grad: torch.Tensor) -> bool:
             and (z.shape[0] == 1 or (z.stride(0) - grad.stride(0)) * z.element_size() % 16 == 0))
 
 
-def _launch(z, index, teacher, labels, V, tau, alpha, counts, grad=None, rows=None, loss=None, gscale=None, written=False, capture=0):
-    """Returns the graph capture that the launches went into (0: none)."""
-    M, W = z.shape
-    gptr, gld = (0, 0) if grad is None else (grad.data_ptr(), grad.stride(0))
-    a = _Args(z.data_ptr(), gptr, index.data_ptr(), teacher.data_ptr(), 0 if labels is None else labels.data_ptr(),
-              0 if gscale is None else gscale.data_ptr(), 0 if rows is None else rows.data_ptr(), counts.data_ptr(),
-              0 if loss is None else loss.data_ptr(), z.stride(0), gld, M, V, W, index.shape[1], counts.shape[0],
-              _lib.DTYPE_CODE[z.dtype], index.dtype is torch.int64, _lib.DTYPE_CODE[teacher.dtype], written, tau, alpha, 1.0 - alpha, capture)
-    _lib.call_on(z.device, "tdl_distill", ctypes.addressof(a))
-    return a.capture
+def _was(a: _Args, i: int):
+    """(shape, type) of the i-th saved tensor"""
+    types = {code: t for t, code in _lib.DTYPE_CODE.items()}
+    return (((a.M, a.W), types[a.dtype]), ((a.M, a.K), torch.int64 if a.index64 else torch.int32), ((a.M, a.K), types[a.teacher_dtype]),
+            ((a.M,), torch.int64), ((a.G, 2), torch.int32))[i]
 
 
 class _Distill(torch.autograd.Function):
@@ -82,25 +77,32 @@ class _Distill(torch.autograd.Function):
         loss = torch.empty((), dtype=torch.float32, device=dev)
         counts = torch.empty(max(1, min(256, -(-M // 256))), 2, dtype=torch.int32, device=dev)
         ctx.grad = _grad_like(z) if grad else None
-        ctx.capture = _launch(z, index, teacher, labels, V, tau, alpha, counts, grad=ctx.grad, rows=rows, loss=loss)
-        ctx.save_for_backward(z, index, teacher, labels, counts)
-        ctx.kept = _lib.kept(z, index, teacher, labels, counts)
-        ctx.how = (V, tau, alpha)
+        a = _Args(z.data_ptr(), 0, index.data_ptr(), teacher.data_ptr(), 0 if labels is None else labels.data_ptr(), 0, rows.data_ptr(),
+                  counts.data_ptr(), loss.data_ptr(), z.stride(0), 0, M, V, z.shape[1], index.shape[1], counts.shape[0],
+                  _lib.DTYPE_CODE[z.dtype], index.dtype is torch.int64, _lib.DTYPE_CODE[teacher.dtype], False, tau, alpha, 1.0 - alpha, 0)
+        if grad:
+            a.grad, a.gld = ctx.grad.data_ptr(), ctx.grad.stride(0)
+        _lib.call_on(dev, "tdl_distill", ctypes.addressof(a))
+        _lib.keep(ctx, z, index, teacher, labels, counts)
+        ctx.args = a      # (and the graph capture that wrote the gradient)
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        saved = ctx.saved_tensors
-        _lib.came_back("distillation_loss", saved, ctx.kept, g.device)
-        z, (index, teacher, labels, counts) = _rows(saved[0]), [None if t is None else t.contiguous() for t in saved[1:]]
+        a = _Args.from_buffer_copy(ctx.args)
+        z, index, teacher, labels, counts = _lib.came_back("distillation_loss", ctx, g.device, lambda i: _was(a, i),
+                                                           lambda i, t: t.contiguous() if i else _rows(t))
         grad, ctx.grad = ctx.grad, None
         # a second backward through the same node gets its own buffer, and so do logits that saved-tensor
         # hooks brought back with other rows
         written = grad is not None and _alike(z, grad)
         if not written:
             grad = _grad_like(z)
-        _launch(z, index, teacher, labels, *ctx.how, counts, grad=grad, gscale=g, written=written, capture=ctx.capture)
+        a.logits, a.ld, a.grad, a.gld = z.data_ptr(), z.stride(0), grad.data_ptr(), grad.stride(0)
+        a.index, a.teacher, a.labels, a.counts = index.data_ptr(), teacher.data_ptr(), 0 if labels is None else labels.data_ptr(), counts.data_ptr()
+        a.gscale, a.rows, a.loss, a.written = g.data_ptr(), 0, 0, written
+        _lib.call_on(z.device, "tdl_distill", ctypes.addressof(a))
         return (grad,) + (None,) * 7
 
 

@@ -38,23 +38,33 @@ class AttentionMask:
     built on one stream is used on another only after that stream has waited for the first, and is told of it
     (``record_stream``) where it may be dropped before the other stream's work is done."""
 
-    def __init__(self, batch: int, q_len: int, k_len: int, lo: torch.Tensor, hi: torch.Tensor, pos: torch.Tensor,
-                 q_table: Optional[torch.Tensor], k_table: Optional[torch.Tensor]):
+    def __init__(self, batch: int, q_len: int, k_len: int, memory: torch.Tensor, nq: int, nk: int):
         self.batch, self.q_len, self.k_len = batch, q_len, k_len
-        self.lo, self.hi, self.pos = lo, hi, pos
-        self.q_table, self.k_table = q_table, k_table
+        # One tensor of 32-bit words (a version for autograd to watch, an allocation per batch).  Tables first: they are
+        # read 16 and 8 bytes at a time
+        self.memory = memory
+        self._tiles = nq, nk
+        k_table = 4 * batch * nq
+        lo = k_table + 2 * batch * nk
+        self._at = lo, lo + batch * q_len, lo + 2 * batch * q_len, 0, k_table     # words: lo, hi, pos, q_table, k_table
+
+    def _part(self, i: int, *shape: int) -> torch.Tensor:
+        return self.memory[self._at[i]:self._at[i] + math.prod(shape)].view(shape)
+
+    lo = property(lambda self: self._part(0, self.batch, self.q_len), doc="int32 [batch, q_len]")
+    hi = property(lambda self: self._part(1, self.batch, self.q_len), doc="int32 [batch, q_len]")
+    pos = property(lambda self: self._part(2, self.batch), doc="int32 [batch]: position of the first query")
+    # what lets the kernels skip tiles (on the GPU; csrc/masked_attention.h qtab, ktab)
+    q_table = property(lambda self: self._part(3, self.batch, self._tiles[0], 4), doc="int32 [batch, tiles of 32 queries, 4]")
+    k_table = property(lambda self: self._part(4, self.batch, self._tiles[1], 2), doc="int32 [batch, blocks of 128 keys, 2]")
 
     @property
     def device(self) -> torch.device:
-        return self.lo.device
+        return self.memory.device
 
     def record_stream(self, stream: torch.cuda.Stream) -> None:
         """``Tensor.record_stream`` for the mask's memory: it is not used again before ``stream``'s work so far is done."""
-        for t in self._tensors():
-            t.record_stream(stream)
-
-    def _tensors(self):   # as _forward and _backward take them
-        return self.lo, self.hi, self.pos, self.q_table, self.k_table
+        self.memory.record_stream(stream)
 
     def dense(self) -> torch.Tensor:
         """[batch, q_len, k_len] booleans (for inspection and the CPU path)."""
@@ -122,19 +132,21 @@ def attention_mask(batch: int, q_len: int, k_len: Optional[int] = None, *, causa
     if device.type != "cuda":
         return _mask_reference(batch, q_len, k_len, causal, documents, rows, marks, lengths, q_start, device)
 
-    def ints(*shape):
-        return torch.empty(shape, dtype=torch.int32, device=device)
     nq, nk = -(-q_len // _Q_TILE), -(-k_len // _K_TILE)
-    with torch.inference_mode(False):     # (a mask may be kept for training: autograd saves its tensors)
-        m = AttentionMask(batch, q_len, k_len, ints(batch, q_len), ints(batch, q_len), ints(batch), ints(batch, nq, 4),
-                          ints(batch, nk, 2))
+    with torch.inference_mode(False):     # (a mask may be kept for training: autograd saves its tensor)
+        memory = torch.empty(batch * (4 * nq + 2 * nk + 2 * q_len + 1), dtype=torch.int32, device=device)
+    m = AttentionMask(batch, q_len, k_len, memory, nq, nk)
     if batch == 0 or q_len == 0:
         return m
-    ws = ints(batch * 3 * k_len) if documents is not None or marks is not None else None
+    ws = torch.empty(batch * 3 * k_len, dtype=torch.int32, device=device) if documents is not None or marks is not None else None
     _lib.call_on(device, "tdl_attn_mask", ptr(documents), int(documents is not None and documents.dtype == torch.int64), ptr(rows),
-                 ptr(marks), ptr(lengths), ptr(q_start), batch, q_len, k_len, int(causal), ptr(ws), ptr(m.lo), ptr(m.hi),
-                 ptr(m.pos), ptr(m.q_table), ptr(m.k_table))
+                 ptr(marks), ptr(lengths), ptr(q_start), batch, q_len, k_len, int(causal), ptr(ws), *_pointers(memory, m._at))
     return m
+
+
+def _pointers(memory: torch.Tensor, at) -> list:
+    base = memory.data_ptr()
+    return [base + 4 * x for x in at]
 
 
 def _mask_reference(B, Tq, Tk, causal, documents, rows, marks, lengths, q_start, device) -> AttentionMask:
@@ -153,8 +165,8 @@ def _mask_reference(B, Tq, Tk, causal, documents, rows, marks, lengths, q_start,
     if Tk and documents is not None:
         ok &= documents.gather(1, pc) >= 0
     if Tk == 0 or B == 0 or Tq == 0:
-        lo = hi = torch.zeros(B, Tq, dtype=torch.int32, device=device)
-        return AttentionMask(B, Tq, Tk, lo, hi, p0.int(), None, None)
+        none = torch.zeros(2 * B * Tq, dtype=torch.int32, device=device)
+        return AttentionMask(B, Tq, Tk, torch.cat([none, p0.int()]), 0, 0)
     e = torch.minimum(end.gather(1, pc), length[:, None])
     lo, hi = start.gather(1, pc), e
     if causal:
@@ -166,7 +178,8 @@ def _mask_reference(B, Tq, Tk, causal, documents, rows, marks, lengths, q_start,
             pe = rows.long()[:, None].expand_as(e)
         hi = torch.maximum(p + 1, torch.minimum(pe, e))
     zero = torch.zeros_like(lo)
-    return AttentionMask(B, Tq, Tk, torch.where(ok, lo, zero).int(), torch.where(ok, hi, zero).int(), p0.int(), None, None)
+    lo, hi = torch.where(ok, lo, zero), torch.where(ok, hi, zero)
+    return AttentionMask(B, Tq, Tk, torch.cat([lo.flatten(), hi.flatten(), p0]).int(), 0, 0)
 
 
 # ============================================================== launches
@@ -225,7 +238,7 @@ def largest_launch(B: int, Tq: int, Tk: int, H: int, Hk: int, D: int) -> int:
 
 
 def _forward(q, k, v, mask, scale, cap, slopes, want_lse: bool, want_rest: bool):
-    """(out, lse or None, out's rounding remainder for the backward pass or None)"""
+    """(out, lse or None, out's rounding remainder for the backward pass or None, the call's arguments)"""
     B, Tq, H, D = q.shape
     Tk, Hk = k.shape[1], k.shape[2]
     dev = q.device
@@ -233,21 +246,29 @@ def _forward(q, k, v, mask, scale, cap, slopes, want_lse: bool, want_rest: bool)
     lse = torch.empty(B, H, Tq, dtype=torch.float32, device=dev) if want_lse else None
     rest = torch.empty(B, Tq, H, D, dtype=torch.uint8, device=dev) if want_rest else None
     if out.numel() == 0:
-        return out, lse, rest
+        return out, lse, rest, None
     nsplit = few_queries(B, Hk, H // Hk, Tq, Tk)
     ws = None
     if nsplit > 1:
         ws = torch.empty(B * H * Tq * nsplit * ((64 if D <= 64 else 128) + 2), dtype=torch.float32, device=dev)
     a = _Args(q.data_ptr(), k.data_ptr(), v.data_ptr(), 0, out.data_ptr(), 0, 0, 0, 0 if lse is None else lse.data_ptr(), 0,
               0 if ws is None else ws.data_ptr(), 0 if rest is None else rest.data_ptr(), 0 if slopes is None else slopes.data_ptr(),
-              *[t.data_ptr() for t in mask], *_strides(q), *_strides(k), *_strides(v), *_strides(out), *_UNUSED, *_UNUSED, *_UNUSED, *_UNUSED,
-              B, Tq, Tk, H, Hk, D, _lib.DTYPE_CODE[q.dtype], nsplit, scale, cap)
+              *_pointers(mask.memory, mask._at), *_strides(q), *_strides(k), *_strides(v), *_strides(out), *_UNUSED, *_UNUSED, *_UNUSED,
+              *_UNUSED, B, Tq, Tk, H, Hk, D, _lib.DTYPE_CODE[q.dtype], nsplit, scale, cap)
     _lib.call_on(dev, "tdl_masked_attn_fwd", ctypes.addressof(a))
-    return out, lse, rest
+    return out, lse, rest, a
 
 
-def _backward(q, k, v, out, lse, rest, slopes, mask, dout, scale, cap, dq, dk, dv):
-    """Writes dq and, unless both are None, dk and dv.  ``lse``, ``rest``, ``slopes`` and the mask's tensors: dense."""
+def _set(a: _Args, prefix: str, t: torch.Tensor):
+    s = _strides(t)
+    setattr(a, prefix + "0", s[0])
+    setattr(a, prefix + "1", s[1])
+    setattr(a, prefix + "2", s[2])
+
+
+def _backward(ctx, q, k, v, out, lse, rest, slopes, mask, moved, dout, dq, dk, dv):
+    """Writes dq and, unless both are None, dk and dv.  ``out``, ``lse``, ``rest``, ``slopes`` and the mask's memory: dense.
+    The forward's arguments serve again; ``moved``: the operands' strides are others."""
     if q.numel() == 0:
         for g in (dk, dv):
             if g is not None:
@@ -256,27 +277,41 @@ def _backward(q, k, v, out, lse, rest, slopes, mask, dout, scale, cap, dq, dk, d
     B, Tq, H, D = q.shape
     # 512 words of scratch, then the rows' statistics, padded to whole tiles: lse log2(e) and -rowsum(dout out)
     ws = torch.empty(512 + B * H * 2 * (-(-Tq // _Q_TILE) * _Q_TILE), dtype=torch.float32, device=q.device)
-    keys = dk is not None
-    a = _Args(q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(), out.data_ptr(), dq.data_ptr(), dk.data_ptr() if keys else 0,
-              dv.data_ptr() if keys else 0, lse.data_ptr(), ws.data_ptr() + 2048, ws.data_ptr(), rest.data_ptr(),
-              0 if slopes is None else slopes.data_ptr(), *[t.data_ptr() for t in mask], *_strides(q), *_strides(k), *_strides(v),
-              *_strides(out), *_strides(dout), *_strides(dq), *(_strides(dk) if keys else _UNUSED), *(_strides(dv) if keys else _UNUSED),
-              B, Tq, k.shape[1], H, k.shape[2], D, _lib.DTYPE_CODE[q.dtype], 0, scale, cap)
+    a = _Args.from_buffer_copy(ctx.args)
+    a.q, a.k, a.v, a.o, a.dout = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dout.data_ptr()
+    a.lse, a.rest, a.slopes = lse.data_ptr(), rest.data_ptr(), 0 if slopes is None else slopes.data_ptr()
+    a.lo, a.hi, a.pos, a.qtab, a.ktab = _pointers(mask, ctx.mask_at)
+    a.ws, a.delta, a.dq = ws.data_ptr(), ws.data_ptr() + 2048, dq.data_ptr()
+    _set(a, "dos", dout)
+    _set(a, "dqs", dq)
+    if dk is not None:
+        a.dk, a.dv = dk.data_ptr(), dv.data_ptr()
+        _set(a, "dks", dk)
+        _set(a, "dvs", dv)
+    if moved:
+        for prefix, t in (("qs", q), ("ks", k), ("vs", v)):
+            _set(a, prefix, t)
     _lib.call_on(q.device, "tdl_masked_attn_bwd", ctypes.addressof(a))
 
 
-def _save(ctx, *tensors):
-    # (the mask's tensors too: a change of them before the backward pass is noticed like one of an operand's)
-    ctx.save_for_backward(*tensors)
-    ctx.kept = _lib.kept(*tensors)
+def _saved(name, ctx, dout, inputs):
+    """The saved tensors as the kernels take them, whatever hooks made of them: operands (``inputs``: their shapes) with
+    strides of their own, the rest dense; and whether an operand is another.  (The mask's memory is one of them: a
+    change of it is noticed like one of an operand's.)"""
+    B, T, H, D = shape = dout.shape
+    n, moved = len(inputs), []
 
+    def was(i):
+        if i < n:
+            return inputs[i], dout.dtype
+        return ((shape, dout.dtype), ((B, H, T), torch.float32), (shape, torch.uint8), ((H,), torch.float32), (ctx.words, torch.int32))[i - n]
 
-def _saved(name, ctx, operands, device):
-    """The saved tensors as the kernels take them, whatever layout hooks gave them: first ``operands`` ones
-    with strides of their own, then dense ones."""
-    saved = ctx.saved_tensors
-    _lib.came_back(name, saved, ctx.kept, device)
-    return [None if t is None else _aligned(t) if i < operands else _lib.dense(t) for i, t in enumerate(saved)]
+    def layout(i, t):
+        if i >= n:
+            return _lib.dense(t)
+        moved.append(i)
+        return _aligned(t)
+    return (*_lib.came_back(name, ctx, dout.device, was, layout), bool(moved))
 
 
 class _MaskedAttention(torch.autograd.Function):
@@ -284,10 +319,9 @@ class _MaskedAttention(torch.autograd.Function):
     def forward(ctx, q, k, v, mask, scale, cap, slopes, want_lse):
         q, k, v = _aligned(q), _aligned(k), _aligned(v)
         grad = any(ctx.needs_input_grad[:3])
-        mask = mask._tensors()
-        out, lse, rest = _forward(q, k, v, mask, scale, cap, slopes, want_lse or grad, grad)
-        ctx.scale, ctx.cap = scale, cap
-        _save(ctx, q, k, v, out, lse, rest, slopes, *mask)
+        out, lse, rest, ctx.args = _forward(q, k, v, mask, scale, cap, slopes, want_lse or grad, grad)
+        ctx.keys, ctx.mask_at, ctx.words = k.shape, mask._at, mask.memory.shape
+        _lib.keep(ctx, q, k, v, out, lse, rest, slopes, mask.memory)
         ctx.set_materialize_grads(False)   # (no zeros for the statistics)
         if lse is not None:
             ctx.mark_non_differentiable(lse)
@@ -298,12 +332,12 @@ class _MaskedAttention(torch.autograd.Function):
     def backward(ctx, dout, _dlse):
         if dout is None:
             return (None,) * 8
-        q, k, v, out, lse, rest, slopes, *mask = _saved("masked_attention", ctx, 4, dout.device)
+        q, k, v, *rest = _saved("masked_attention", ctx, dout, (dout.shape, ctx.keys, ctx.keys))
         keys = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
         dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         dk = torch.empty(k.shape, dtype=k.dtype, device=k.device) if keys else None
         dv = torch.empty(v.shape, dtype=v.dtype, device=v.device) if keys else None
-        _backward(q, k, v, out, lse, rest, slopes, mask, _aligned(dout), ctx.scale, ctx.cap, dq, dk, dv)
+        _backward(ctx, q, k, v, *rest, _aligned(dout), dq, dk, dv)
         return dq, dk, dv, None, None, None, None, None
 
 
@@ -314,19 +348,18 @@ class _MaskedAttentionPacked(torch.autograd.Function):
     def forward(ctx, qkv, n_head, n_kv_head, mask, scale, cap, slopes, grad):
         qkv = _aligned(qkv)
         q, k, v = qkv.split((n_head, n_kv_head, n_kv_head), dim=2)
-        mask = mask._tensors()
-        out, lse, rest = _forward(q, k, v, mask, scale, cap, slopes, grad, grad)
-        ctx.scale, ctx.cap, ctx.heads = scale, cap, (n_head, n_kv_head, n_kv_head)
-        _save(ctx, qkv, out, lse, rest, slopes, *mask)
+        out, lse, rest, ctx.args = _forward(q, k, v, mask, scale, cap, slopes, grad, grad)
+        ctx.heads, ctx.mask_at, ctx.words = (n_head, n_kv_head, n_kv_head), mask._at, mask.memory.shape
+        _lib.keep(ctx, qkv, out, lse, rest, slopes, mask.memory)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        qkv, out, lse, rest, slopes, *mask = _saved("masked_attention_packed", ctx, 2, dout.device)
+        B, T, _, D = dout.shape
+        qkv, *rest = _saved("masked_attention_packed", ctx, dout, ((B, T, sum(ctx.heads), D),))
         dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
-        _backward(*qkv.split(ctx.heads, dim=2), out, lse, rest, slopes, mask, _aligned(dout), ctx.scale, ctx.cap,
-                  *dqkv.split(ctx.heads, dim=2))
+        _backward(ctx, *qkv.split(ctx.heads, dim=2), *rest, _aligned(dout), *dqkv.split(ctx.heads, dim=2))
         return (dqkv,) + (None,) * 7
 
 
@@ -426,7 +459,7 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: At
     if q.is_cuda and torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         out, lse = _MaskedAttention.apply(q, k, v, mask, scale, cap, slopes, return_lse)
     elif q.is_cuda:   # (a single token's call is bound by the host: no autograd node)
-        out, lse, _ = _forward(_aligned(q), _aligned(k), _aligned(v), mask._tensors(), scale, cap, slopes, return_lse, False)
+        out, lse, _, _ = _forward(_aligned(q), _aligned(k), _aligned(v), mask, scale, cap, slopes, return_lse, False)
     else:
         out, lse = _reference(q, k, v, mask, scale, cap, slopes)
     return (out, lse) if return_lse else out
