@@ -301,3 +301,60 @@ def test_a_mask_dropped_while_another_stream_uses_it():
     assert side.query() or not held & {t.data_ptr() for t in fresh}
     torch.cuda.synchronize()
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("packed", [True, False])
+def test_recomputed_under_checkpointing(packed):
+    """Activations that a checkpoint throws away and makes again, attention and loss inside: the same gradients."""
+    from torch.utils.checkpoint import checkpoint
+
+    from trustworthy_dl import ops
+    B, T, H, D, V = 2, 130, 4, 64, 96
+    x = _rand(0, B, T, 3 * H * D)
+    w = _rand(1, H * D, V, mul=0.05)
+    mask = ops.attention_mask(B, T, documents=(torch.arange(T, device=DEV) // 50).int().expand(B, T))
+    g = torch.Generator(device=DEV).manual_seed(2)
+    idx, t = torch.randint(0, V, (B, T, 5), generator=g, device=DEV), torch.randn(B, T, 5, generator=g, device=DEV)
+    slopes = torch.tensor([0.1, 0.2, 0.3, 0.4], device=DEV)
+
+    def loss(z):
+        if packed:
+            a = ops.masked_attention_packed(z, H, mask, slopes=slopes)
+        else:
+            a = ops.masked_attention(*(z * 1.0).view(B, T, 3 * H, D).split(H, 2), mask, slopes=slopes).reshape(B, T, -1)
+        return ops.distillation_loss(a @ w, idx, t, temperature=2.0)
+    grads = []
+    for again in (False, True):
+        for up in (1.0, 3.0):
+            z = x.clone().requires_grad_(True)
+            out = checkpoint(loss, z, use_reentrant=False) if again else loss(z)
+            grads.append(torch.autograd.grad(out, z, torch.tensor(up, device=DEV))[0])
+    assert torch.equal(grads[0], grads[2]) and torch.equal(grads[1], grads[3])
+    assert float(grads[0].abs().max()) > 0
+
+
+@pytest.mark.parametrize("what", ["q", "k", "v"])
+def test_forward_by_two_threads_backward_by_both(what):
+    """One graph kept for two backward passes, made by two threads at once."""
+    import threading
+
+    from trustworthy_dl import ops
+    mask = ops.attention_mask(2, 300, device=DEV)
+    ins = {n: _rand(i, 2, 300, 4, 64) for i, n in enumerate("qkv")}
+    ins[what].requires_grad_(True)
+    out = ops.masked_attention(*ins.values(), mask)
+    ups = [_rand(7 + i, 2, 300, 4, 64) for i in range(2)]
+    want = [torch.autograd.grad(out, ins[what], u, retain_graph=True)[0] for u in ups]
+    torch.cuda.synchronize()
+    got = [None, None]
+
+    def work(i):
+        for _ in range(5):
+            got[i] = torch.autograd.grad(out, ins[what], ups[i], retain_graph=True)[0]
+        torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
