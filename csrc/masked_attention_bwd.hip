@@ -670,7 +670,7 @@ static int bwd_launch(const Args& a, hipStream_t s) {
     const int64_t gq = (int64_t)a.B * a.H * ((a.Tq + 127) / 128), gk = (int64_t)a.B * a.Hk * ((a.Tk + KT - 1) / KT);
     if (gq > MAX_GRID || gk > MAX_GRID) return (int)hipErrorInvalidValue;
     int rc = 0;
-    if (T::INF != 0x7f80) {
+    if constexpr (T::INF != 0x7f80) {
         mattn_norm_max_kernel<T, DP><<<NMAX, 256, 0, s>>>(a);
         rc = (int)hipGetLastError();
         if (rc) return rc;
