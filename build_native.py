@@ -1,12 +1,13 @@
 #!/usr/bin/env python3
 """Build the native gfx950 kernel library and the C++ runtime helpers, in-tree.
 
-    python build_native.py [--jobs N] [--arch gfx950] [--debug]
+    python build_native.py [--jobs N] [--arch gfx950] [--debug] [--force]
 
 Outputs (git-ignored, but shipped to the GPU box with the tree):
     trustworthy_dl/_native/libtdl_kernels.so   HIP kernels (csrc/*.hip), C ABI, loaded by ops/_lib.py
     trustworthy_dl/_native/libtdl_runtime.so   host C++ runtime (csrc/runtime/*.cpp), loaded by runtime/native.py
-Incremental: a translation unit is rebuilt only when it or a header is newer than its object.
+Incremental: a translation unit is rebuilt only when it or a header is newer than its object (--force: all
+of them, also after a change of the flags below).
 """
 from __future__ import annotations
 
@@ -49,7 +50,8 @@ def _run(cmd):
     return p.returncode, " ".join(cmd), p.stdout
 
 
-def build(arch: str = "gfx950", jobs: int = 8, debug: bool = False, verbose: bool = False) -> dict:
+def build(arch: str = "gfx950", jobs: int = 8, debug: bool = False, verbose: bool = False, force: bool = False) -> dict:
+    """Compile what is out of date (``force``: everything) and link; {name: library}."""
     os.makedirs(OUT_DIR, exist_ok=True)
     os.makedirs(BUILD_DIR, exist_ok=True)
     cc = hipcc()
@@ -64,7 +66,7 @@ def build(arch: str = "gfx950", jobs: int = 8, debug: bool = False, verbose: boo
     for src in kernel_srcs:
         obj = os.path.join(BUILD_DIR, os.path.basename(src) + ".o")
         kobjs.append(obj)
-        if _newer(src, obj, headers):
+        if force or _newer(src, obj, headers):
             # MFMA accumulators in ArchVGPRs: the default AGPR form shuttles every softmax / epilogue
             # read through v_accvgpr_read/write and pushed the attention forward past 256 registers
             # (one wave per SIMD); the VGPR form holds it at 140 (three waves per SIMD)
@@ -79,7 +81,7 @@ def build(arch: str = "gfx950", jobs: int = 8, debug: bool = False, verbose: boo
     for src in rt_srcs:
         obj = os.path.join(BUILD_DIR, "rt_" + os.path.basename(src) + ".o")
         robjs.append(obj)
-        if _newer(src, obj, rt_headers):
+        if force or _newer(src, obj, rt_headers):
             jobs_list.append(["g++", "-std=c++17", "-fPIC", "-O2", "-Wall", "-pthread",
                               "-I", os.path.join(CSRC, "runtime"), "-c", src, "-o", obj])
 
@@ -94,7 +96,7 @@ def build(arch: str = "gfx950", jobs: int = 8, debug: bool = False, verbose: boo
     outputs = {}
     if kobjs:
         lib = os.path.join(OUT_DIR, "libtdl_kernels.so")
-        if not os.path.exists(lib) or any(os.path.getmtime(o) > os.path.getmtime(lib) for o in kobjs):
+        if force or not os.path.exists(lib) or any(os.path.getmtime(o) > os.path.getmtime(lib) for o in kobjs):
             rc, cmd, out = _run([cc, f"--offload-arch={arch}", "-shared", "-fPIC", *kobjs, "-o", lib + ".tmp"])
             if rc != 0:
                 print(cmd)
@@ -104,7 +106,7 @@ def build(arch: str = "gfx950", jobs: int = 8, debug: bool = False, verbose: boo
         outputs["kernels"] = lib
     if robjs:
         lib = os.path.join(OUT_DIR, "libtdl_runtime.so")
-        if not os.path.exists(lib) or any(os.path.getmtime(o) > os.path.getmtime(lib) for o in robjs):
+        if force or not os.path.exists(lib) or any(os.path.getmtime(o) > os.path.getmtime(lib) for o in robjs):
             rc, cmd, out = _run(["g++", "-shared", "-fPIC", "-pthread", *robjs, "-o", lib + ".tmp"])
             if rc != 0:
                 print(cmd)
@@ -120,9 +122,10 @@ def main():
     ap.add_argument("--arch", default=os.environ.get("PYTORCH_ROCM_ARCH", "gfx950"))
     ap.add_argument("--jobs", type=int, default=min(8, os.cpu_count() or 1))
     ap.add_argument("--debug", action="store_true")
+    ap.add_argument("--force", action="store_true")
     ap.add_argument("-v", "--verbose", action="store_true")
     a = ap.parse_args()
-    outs = build(a.arch, a.jobs, a.debug, a.verbose)
+    outs = build(a.arch, a.jobs, a.debug, a.verbose, a.force)
     for k, v in outs.items():
         print(f"{k}: {v}")
 
