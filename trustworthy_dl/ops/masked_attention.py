@@ -102,6 +102,7 @@ def attention_mask(batch: int, q_len: int, k_len: Optional[int] = None, *, causa
                    behind them see nothing.
     ``q_start``    int [batch]: position of each row's first query.  Default: the queries are the last
                    ``q_len`` valid positions of the row (a cache), or with q_len == k_len start at 0.
+    ``device``     where the mask is used (default: that of the tensors above, or the CPU).
     """
     k_len = q_len if k_len is None else k_len
     if batch < 0 or q_len < 0 or k_len < q_len:
@@ -449,8 +450,8 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: At
 
     q [B, Tq, H, D], k and v [B, Tk, Hk, D] with H a multiple of Hk (query head h reads KV head
     h // (H / Hk)); any batch / token / head strides.  ``scale`` defaults to 1 / sqrt(D); without
-    ``softcap`` the scores are not capped, without ``slopes`` (fp32 [H]) there is no distance bias
-    (p, j: positions of query and key).  Returns [B, Tq, H, D] in q's type; a query that sees nothing
+    ``softcap`` the scores are not capped, without ``slopes`` (fp32 [H], finite, of
+    either sign) there is no distance bias (p, j: positions of query and key).  Returns [B, Tq, H, D] in q's type; a query that sees nothing
     gives zeros, and keys it does not see have no effect on it, whatever they hold (on the CPU: keys that no
     query of the row sees).  Scores are kept in 32 bits: at a size of S their weights are known to S 2^-21.  With
     ``return_lse`` also the fp32 log-sum-exp of each query's scores [B, H, Tq] (-inf where it sees
