@@ -238,3 +238,37 @@ def test_sizes_out_of_range_are_refused():
 
 def test_more_rows_than_workgroups():
     check(*rows((1 << 21) + 777, 8, 2, FP, 0.0), 8, 2.0, 0.5)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("M,V", FORMS)
+def test_forbidden_classes(M, V, dtype):
+    """Rows that are -infinity but for a few classes (the first ones, the last one, one in the middle), and one that is
+    -infinity throughout: NaN there by the definition, and nowhere else."""
+    from trustworthy_dl import ops
+    z, idx, t, labels = rows(M, V, 9, dtype, -150.0)
+    few = {0: [0, 1, 2], 2: [V - 1], 3: [V // 2, V // 2 + 1]}
+    for r, cols in few.items():
+        keep = z[r, cols].clone()
+        z[r] = -math.inf
+        z[r, cols] = keep
+        idx[r] = torch.tensor([cols[i % len(cols)] for i in range(9)], device=DEV)
+        labels[r] = cols[0]
+    for tau, alpha in MODES:
+        check(z, idx, t, labels, V, tau, alpha)
+    x = z.clone()
+    x[4] = -math.inf
+    idx[4], labels[4] = 3, 3
+    x.requires_grad_(True)
+    loss = ops.distillation_loss(x, idx, t, labels, temperature=2.0, alpha=0.5)
+    (g,) = torch.autograd.grad(loss, x)
+    others = [r for r in range(M) if r != 4]
+    assert torch.isnan(loss) and torch.isnan(g[4]).all() and torch.isfinite(g[others]).all()
+
+
+def test_inference_mode():
+    from trustworthy_dl import ops
+    z, idx, t, labels = rows(5, 3000, 9, BF, 0.0)
+    want = ops.distillation_loss(z, idx, t, labels, temperature=2.0, alpha=0.5)
+    with torch.inference_mode():
+        assert torch.equal(ops.distillation_loss(z.clone(), idx, t, labels, temperature=2.0, alpha=0.5), want)

@@ -358,3 +358,28 @@ def test_forward_by_two_threads_backward_by_both(what):
     for t in threads:
         t.join()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("T", [1, 20, 200])
+def test_rows_that_all_see_nothing(T, dtype):
+    """Empty rows alone: zeros everywhere, whatever the operands hold."""
+    from trustworthy_dl import ops
+    for kw in ({"lengths": torch.zeros(2, dtype=torch.int32, device=DEV)}, {"documents": torch.full((2, T), -1, dtype=torch.int32, device=DEV)}):
+        mask = ops.attention_mask(2, T, **kw)
+        ins = [torch.full((2, T, h, 64), float("nan"), dtype=dtype, device=DEV) for h in (4, 2, 2, 4)]
+        got = _grads(*ins, mask, softcap=5.0)
+        assert all((g == 0).all() for g in got.values())
+        assert (ops.masked_attention(*ins[:3], mask, return_lse=True)[1] == -math.inf).all()
+
+
+@pytest.mark.parametrize("T", [20, 200])
+def test_inference_mode(T):
+    from trustworthy_dl import ops
+    t = [_rand(i, 2, T, h, 64) for i, h in enumerate((4, 2, 2))]
+    want = ops.masked_attention(*t, ops.attention_mask(2, T, device=DEV))
+    with torch.inference_mode():
+        u = [x.clone() for x in t]
+        mask = ops.attention_mask(2, T, device=DEV)
+        assert torch.equal(ops.masked_attention(*u, mask), want)
+        assert torch.equal(ops.masked_attention_packed(torch.cat(u, 2).reshape(2, T, -1), 4, mask, n_kv_head=2).view(want.shape), want)
