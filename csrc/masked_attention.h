@@ -310,6 +310,19 @@ __device__ __forceinline__ Where place(int L, const Args& a, int nblk, bool flip
     return w;
 }
 
+// the sum of 8 bf16 values and c, in 32 bits
+__device__ __forceinline__ float sum8(bf16x8 v, float c) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    const bf16x2 one = {(__bf16)1.f, (__bf16)1.f};
+    const u32x4 u = __builtin_bit_cast(u32x4, v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t w = u[i];
+        c = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), one, c, false);
+    }
+    return c;
+}
+
 // Staging of a [ROWS][DP] tile by NTHR threads: thread t takes the 16-B chunk t % (DP / 8) of rows
 // t / (DP / 8) + j RPP.  Rows past the tensor are clamped when loaded (every load stays in bounds)
 // and stored as zeros by put_masked.

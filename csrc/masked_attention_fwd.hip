@@ -165,7 +165,12 @@ TDL_API int tdl_attn_mask(const void* documents, int wide, const int* prefix_row
 // reciprocal, 8, and 3.5 others, 4, against 256 cycles of products for 64 columns), so three waves a SIMD
 // (two from 65 columns on) take turns.  2 x 8192, 16 heads of 128 on 4, cap 50: 716 us; 8 x 2048, 25 heads of
 // 64, cap 30: 200 us; 16 x 1024 in documents, 16 heads of 64: 57 us.
-template <class T, int DP, bool CAP, bool ALIBI>
+// FIXED: capped scores without a bias are taken less their bound, the cap (Score::below), so they lie in [-2 cap, 0].
+// Up to a cap of 32 a bf16 softmax needs no running maximum then: its smallest weight is e^-64, well in
+// bf16's range (not in fp16's).  The largest weight is not 1 as with a maximum, and its rounding, which a peaked row
+// carries whole (2.3e-3 instead of 1.8e-3 of error at a cap of 30), cancels against the sum of the rounded weights.
+// 8 x 2048, 25 heads of 64, whole calls: 191 us at a cap of 32, 208 at 33.
+template <class T, int DP, bool CAP, bool ALIBI, bool FIXED>
 __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void mattn_fwd_kernel(const Args a) {
     constexpr int NW = 4, BM = QT * NW, BN = 64, NS = DP / 16, NO = DP / 32, NTHR = 64 * NW;
     typedef Copy<T, DP, BN, NTHR> CP;
@@ -217,13 +222,10 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void mattn_fwd_kernel(const 
     f32x16 o[NO];
 #pragma unroll
     for (int i = 0; i < NO; ++i) o[i] = (f32x16){};
-    // Capped scores without a bias are taken less their bound, the cap (Score::below): in [-2 cap, 0].  Up
-    // to a cap of 32 a bf16 softmax needs no running maximum then: its smallest weight is e^-64, well in
-    // bf16's range (not in fp16's).  8 x 2048, 25 heads of 64: 220 us at
-    // a cap of 32, 229 at 33.
     constexpr bool SAT = CAP && !ALIBI;
-    const bool fixed = SAT && T::INF == 0x7f80 && a.cap <= 32.f;
-    float m = fixed ? 0.f : -INFINITY, l = 0.f;
+    static_assert(!FIXED || (SAT && T::INF == 0x7f80), "capped bf16 scores without a bias");
+    float m = FIXED ? 0.f : -INFINITY, l = 0.f;
+    float lr = 0.f;   // FIXED: the sum of the rounded weights
     NotFinite odd;
     const int kb0 = bh > bl ? bl / BN : 0, kb1 = bh > bl ? (bh + BN - 1) / BN : 0;
     const int tq = (lane & 15) >> 2, tcol = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
@@ -280,8 +282,8 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void mattn_fwd_kernel(const 
                 for (int i = 0; i < 16; ++i)
                     s[t][i] = (uint32_t)(k0 + 32 * t + (i & 3) + 8 * (i >> 2)) < n ? s[t][i] : -INFINITY;
         }
-        float ms = m;
-        if (!fixed) {
+        float mu = 0.f;   // what the exponents are less
+        if constexpr (!FIXED) {
             float mx = max3(s[0][0], s[1][0], s[0][1]);
 #pragma unroll
             for (int i = 1; i < 16; ++i) mx = max3(mx, s[1][i], i + 1 < 16 ? s[0][i + 1] : s[1][i]);
@@ -289,7 +291,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void mattn_fwd_kernel(const 
             mx = max3(mx, ot, ot);
             if constexpr (Score<CAP, ALIBI>::PLAIN) mx *= sc.mul;   // scale > 0: the maximum commutes with it
             const float mn = fmaxf(m, mx);
-            ms = mn == -INFINITY ? 0.f : mn;   // nothing visible yet: 2^(-inf - 0) = 0
+            const float ms = mn == -INFINITY ? 0.f : mn;   // nothing visible yet: 2^(-inf - 0) = 0
             if (__any(mn > m)) {   // the old sums keep their scale where no row's maximum rose
                 const float alpha = exp2_fast(m - ms);
                 l *= alpha;
@@ -297,14 +299,14 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void mattn_fwd_kernel(const 
                 for (int i = 0; i < NO; ++i) o[i] *= alpha;
             }
             m = mn;
+            mu = ms - (float)T::UP;
         }
         float rs = 0.f;
-        const float mu = ms - (float)T::UP;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                s[t][i] = exp2_fast(Score<CAP, ALIBI>::PLAIN ? fmaf(s[t][i], sc.mul, -mu) : fixed ? s[t][i] : s[t][i] - mu);
+                s[t][i] = exp2_fast(Score<CAP, ALIBI>::PLAIN ? fmaf(s[t][i], sc.mul, -mu) : FIXED ? s[t][i] : s[t][i] - mu);
                 rs += s[t][i];
             }
         l += rs;   // this half's keys; the halves are added at the end
@@ -321,6 +323,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void mattn_fwd_kernel(const 
 #pragma unroll
             for (int s2 = 0; s2 < 2; ++s2) {
                 const typename T::vec pf = round8<T>(s[t], s2);
+                if constexpr (FIXED) lr = sum8(pf, lr);
                 const int row = 32 * t + 16 * s2 + 4 * h + tq;
 #pragma unroll
                 for (int i = 0; i < NO; ++i) o[i] = T::mfma(tr_pair<T, DP>(V_, row, 32 * i + tcol), pf, o[i]);
@@ -338,8 +341,9 @@ __global__ __launch_bounds__(256, DP == 64 ? 3 : 2) void mattn_fwd_kernel(const 
         if (kb + 1 < kb1) mend(kb + 1, buf ^ 1);
     }
     l += __shfl_xor(l, 32, 64);
+    if constexpr (FIXED) lr += __shfl_xor(lr, 32, 64);
     if (qi < a.Tq) {
-        const float inv = l == 0.f ? 0.f : 1.f / l;   // nothing visible: 0
+        const float inv = l == 0.f ? 0.f : 1.f / (FIXED ? lr : l);   // nothing visible: 0
         bf16_t* orow = (bf16_t*)a.o + at.b * a.os[0] + at.h * a.os[2] + (int64_t)qi * a.os[1];
         if (odd.any()) {
 #pragma unroll
@@ -626,7 +630,13 @@ static int fwd_launch(const Args& a, hipStream_t s) {
     }
     const int64_t grid = (int64_t)a.B * a.H * ((a.Tq + 127) / 128);
     if (grid > MAX_GRID) return (int)hipErrorInvalidValue;
-    mattn_fwd_kernel<T, DP, CAP, ALIBI><<<(int)grid, 256, 0, s>>>(a);
+    if constexpr (CAP && !ALIBI && T::INF == 0x7f80) {
+        if (a.cap <= 32.f) {
+            mattn_fwd_kernel<T, DP, CAP, ALIBI, true><<<(int)grid, 256, 0, s>>>(a);
+            TDL_LAUNCH_CHECK();
+        }
+    }
+    mattn_fwd_kernel<T, DP, CAP, ALIBI, false><<<(int)grid, 256, 0, s>>>(a);
     TDL_LAUNCH_CHECK();
 }
 

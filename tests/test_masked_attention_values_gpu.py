@@ -383,3 +383,20 @@ def test_inference_mode(T):
         mask = ops.attention_mask(2, T, device=DEV)
         assert torch.equal(ops.masked_attention(*u, mask), want)
         assert torch.equal(ops.masked_attention_packed(torch.cat(u, 2).reshape(2, T, -1), 4, mask, n_kv_head=2).view(want.shape), want)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("cap", [20.0, 30.0, 32.0, 33.0, 50.0])
+@pytest.mark.parametrize("Tq", [5, 70])
+def test_a_capped_row_with_all_weight_on_one_key(Tq, cap, dtype):
+    """The result is that key's value: its weight's own rounding cancels against the sum's, whatever the weight is."""
+    from trustworthy_dl import ops
+    D, Tk = 64, 70
+    q, k = torch.zeros(1, Tq, 2, D, dtype=dtype, device=DEV), torch.zeros(1, Tk, 2, D, dtype=dtype, device=DEV)
+    # scores of +-x, x = 1.1 cap .. 1.9 cap: weights of e^(2 cap tanh(x / cap)) > e^30 of the others
+    q[..., 0] = torch.linspace(1.1, 1.9, Tq, device=DEV).to(dtype)[None, :, None] * cap
+    k[..., 0] = -8.0
+    k[:, 3, :, 0] = 8.0
+    v = _rand(5, 1, Tk, 2, D, dtype=dtype)
+    out = ops.masked_attention(q, k, v, ops.attention_mask(1, Tq, Tk, causal=False, device=DEV), softcap=cap)
+    assert torch.equal(out, v[:, 3:4].expand(out.shape))
