@@ -104,7 +104,7 @@ __device__ __forceinline__ int scale_exponent(const Args& a) {
 // ============================================================================ dQ
 // Workgroup and tiles as in the forward.  Bound by the vector ALU: 500 instructions for 64 keys of a capped
 // score, 48 of them products.  Two waves a SIMD (three, for heads of 64: 88 against 85 us on 16 x 1024).
-// 2 x 8192, 16 heads of 128 on 4, cap 50: 945 us (one wave a SIMD, tiles through registers: 1656 us);
+// 2 x 8192, 16 heads of 128 on 4, cap 50: 990 us (one wave a SIMD, tiles through registers: 1656 us);
 // 16 x 1024 in documents, 16 heads of 64: 70 us.
 template <class T, int DP, bool CAP, bool ALIBI>
 __global__ __launch_bounds__(256, 2) void mattn_dq_kernel(const Args a) {
@@ -312,7 +312,7 @@ __global__ __launch_bounds__(256, 2) void mattn_dq_kernel(const Args a) {
 // interleaves C(t - 1), B(t) and A(t + 1), two scores between every few products, each product's LDS
 // fragment read two products ahead.  Eight places for tiles of Q / dO are in LDS: t - 1 .. t + 1 are
 // read, t + 2 .. t + 4 are on their way (copies straight from memory); one barrier per tile.
-// 2 x 8192, 16 heads of 128 on 4, cap 50: 1624 us, 3500 cycles a tile of which 1024 are products (reading
+// 2 x 8192, 16 heads of 128 on 4, cap 50: 1613 us, 3500 cycles a tile of which 1024 are products (reading
 // fragments 4 or 5 products ahead gained nothing); 16 x 1024 in documents, 16 heads of 64: 105 us (115 without
 // the pipeline).
 template <class T, int DP, bool CAP, bool ALIBI>

@@ -163,8 +163,8 @@ TDL_API int tdl_attn_mask(const void* documents, int wide, const int* prefix_row
 // exchange their maximum), and the rounded S^T accumulator IS the B operand of O^T += V^T P^T.
 // Bound by the vector ALU (16 scores a lane and 32-key tile: with a cap two exponentials, of 8 cycles each, a
 // reciprocal, 8, and 3.5 others, 4, against 256 cycles of products for 64 columns), so three waves a SIMD
-// (two from 65 columns on) take turns.  2 x 8192, 16 heads of 128 on 4, cap 50: 716 us; 8 x 2048, 25 heads of
-// 64, cap 30: 200 us; 16 x 1024 in documents, 16 heads of 64: 57 us.
+// (two from 65 columns on) take turns.  2 x 8192, 16 heads of 128 on 4, cap 50: 742 us; 8 x 2048, 25 heads of
+// 64, cap 30: 201 us; 16 x 1024 in documents, 16 heads of 64: 56 us.
 // FIXED: capped scores without a bias are taken less their bound, the cap (Score::below), so they lie in [-2 cap, 0].
 // Up to a cap of 32 a bf16 softmax needs no running maximum then: its smallest weight is e^-64, well in
 // bf16's range (not in fp16's).  The largest weight is not 1 as with a maximum, and its rounding, which a peaked row
@@ -389,7 +389,7 @@ __device__ __forceinline__ void put_out(const Args& a, const float (&acc)[4], fl
 // other: a wave takes 32 keys at a time, K straight from memory into the operand registers, V through
 // its own LDS for the transposing read, the next keys' loads in flight meanwhile.  Each workgroup joins
 // its waves' (maximum, sum, O); mattn_join adds the splits.  48 caches of up to 8191 tokens, 32 heads of 128
-// on 8: 274 us and 5 of joining, 3.8 TB/s; 4 caches of 5003, 7 queries: 18 us and 6 us of joining.
+// on 8: 272 us and 5 of joining, 3.8 TB/s; 4 caches of 5003, 7 queries: 18 us and 6 us of joining.
 template <class T, int DP, bool CAP, bool ALIBI>
 __global__ __launch_bounds__(256, 2) void mattn_few_kernel(const Args a) {
     constexpr int NS = DP / 16, NO = DP / 32, NW = 4, NCH = DP / 8;
