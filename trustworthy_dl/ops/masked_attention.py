@@ -453,7 +453,8 @@ def masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: At
     ``softcap`` the scores are not capped, without ``slopes`` (fp32 [H], finite, of
     either sign) there is no distance bias (p, j: positions of query and key).  Returns [B, Tq, H, D] in q's type; a query that sees nothing
     gives zeros, and keys it does not see have no effect on it, whatever they hold (on the CPU: keys that no
-    query of the row sees).  Scores are kept in 32 bits: at a size of S their weights are known to S 2^-21.  With
+    query of the row sees).  Scores are kept in 32 bits: at a size of S their weights are known to S 2^-21 (past
+    2^21: not at all).  With
     ``return_lse`` also the fp32 log-sum-exp of each query's scores [B, H, Tq] (-inf where it sees
     nothing; not differentiable)."""
     scale, cap, slopes = _check("masked_attention", q, k, v, mask, scale, softcap, slopes)
