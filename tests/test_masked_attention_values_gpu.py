@@ -400,3 +400,35 @@ def test_a_capped_row_with_all_weight_on_one_key(Tq, cap, dtype):
     v = _rand(5, 1, Tk, 2, D, dtype=dtype)
     out = ops.masked_attention(q, k, v, ops.attention_mask(1, Tq, Tk, causal=False, device=DEV), softcap=cap)
     assert torch.equal(out, v[:, 3:4].expand(out.shape))
+
+
+@pytest.mark.parametrize("what", [("documents", "lengths"), ("prefix_rows", "lengths"), ("marks",), ("marks", "lengths"), ("documents", "marks", "lengths"),
+                                  ("q_start", "lengths"), ("q_start", "documents"), ("full", "documents", "lengths", "q_start"),
+                                  ("full", "lengths"), ("q_start", "prefix_rows")])
+@pytest.mark.parametrize("Tq,Tk", [(1, 1), (7, 150), (150, 150), (40, 2100)])
+def test_masks_put_together(what, Tq, Tk):
+    """Combinations of the masks' arguments, 64-bit ones among them: the CPU's intervals, and what they let through."""
+    from trustworthy_dl import ops
+    B, g = 4, torch.Generator().manual_seed(Tk + len(what))
+    kw = {"causal": "full" not in what}
+    if "documents" in what:
+        ids = torch.cumsum((torch.rand(B, Tk, generator=g) < 0.05).long(), 1) + (1 << 40)
+        ids[torch.rand(B, Tk, generator=g) < 0.02] = -1
+        kw["documents"] = ids
+    if "lengths" in what:
+        kw["lengths"] = torch.randint(-2, Tk + 5, (B,), generator=g)
+    if "prefix_rows" in what:
+        kw["prefix"] = torch.randint(-2, Tk + 5, (B,), generator=g)
+    if "marks" in what:
+        kw["prefix"] = (torch.rand(B, Tk, generator=g) < 0.8).to(torch.uint8) * 3
+    if "q_start" in what:
+        kw["q_start"] = torch.randint(-3, Tk, (B,), generator=g)
+    cpu = ops.attention_mask(B, Tq, Tk, **kw)
+    gpu = ops.attention_mask(B, Tq, Tk, **{n: v.to(DEV) if isinstance(v, torch.Tensor) else v for n, v in kw.items()}, device=DEV)
+    for n in ("lo", "hi", "pos"):
+        assert torch.equal(getattr(gpu, n).cpu(), getattr(cpu, n)), n
+    q, k, v, do = (_rand(i, B, t, h, 64) for i, (t, h) in enumerate(((Tq, 4), (Tk, 2), (Tk, 2), (Tq, 4))))
+    got = _grads(q, k, v, do, gpu)
+    want = oracle.run(q, k, v, gpu.dense(), gpu.pos.long(), 0.125, 0.0, None, do)
+    for n, x in got.items():
+        oracle.check(x, want[n], n)
